@@ -448,7 +448,7 @@ int v2a_opt_step(const int64_t* table_dev, const int* chunks_dev, int nchunks, v
    [Cout][taps][Cin] or 0, Cin, taps, channel-window pack (v2a_conv2d_fwd_window_f32) or 0, 16-bit side copy of the forward pack or 0, its
    format: 0 bf16 twin, 1 IEEE fp16 twin, 2 = three bf16 planes hi / mid / lo of the fp32 value, the tensor's element count apart
    (v2a_conv2d_fwd_p3's weight operand)}; the launch of v2a_pack_weights_multi that would read every parameter again is not needed for
-   those operands) */
+   those operands).
    presum_first / presum_count: chunks [first, first + count) of partial_dev already hold this step's sums of squares (written by
    v2a_opt_presum with the same range on a stream ordered before this call); 0 / 0: every chunk is summed here.  Explicit operands: nothing
    is remembered between the two calls. */
