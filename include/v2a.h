@@ -213,6 +213,38 @@ int v2a_mha_bwd(const float* q, const float* k, const float* v, const float* mas
  * mask -- element i of random stream `stream_id` under `seed` is kept iff hash(seed, stream_id, i) >= p; the same call on dy is the backward.
  * The attention kernels above apply the same rule to the probabilities (element index ((b*H + h)*Tq + i)*Tk + j). */
 int v2a_dropout(const float* x, float* y, size_t n, float p, uint64_t seed, uint64_t stream_id, v2a_stream_t s);
+/* ---------------------------------------------------------------------------------------------- token sequences (csrc/linattn.hip, embed.hip)
+ * Linear attention with a decay for each head, the constant-state counterpart of the attention above for long histories and for one token
+ * per control tick:  S_t = exp(g_t) S_{t-1} + k_t v_t^T  (fp32, [Dk][Dv] per batch row and head),  out_t = scale * S_t^T q_t.
+ *   q [B,T,Hq,Dk], k [B,T,Hk,Dk], v [B,T,Hv,Dv], dout [B,T,H,Dv]: dtype 0 fp32 / 1 bf16 / 2 fp16, any strides over (batch, token, head), last
+ *     dimension contiguous.  Hq, Hk, Hv divide H: head h reads shared head h / (H / Hx).  Dk, Dv <= 128.
+ *   g: fp32 log decays, strides over (batch, token, head); stride 0 over batch and token is one decay per head.  -inf clears the state.
+ *   state / dstate [B,H,Dk,Dv] fp32: the state before the first token (NULL = 0) and its gradient; state_out / dstate_out: after the last.
+ *   lens (NULL = T): int32 [B]; tokens from lens[b] on are not read, their out / gradient rows are 0 (values outside [0, T] are clamped).
+ *   out [B,T,H,Dv], dq / dk / dv like q / k / v: contiguous, in dtype.  dg: fp32, [B,T,H] with per_token_decay, else [H]; may be NULL.
+ *   strides: HOST array, elements: q, k, v, g (and dout for the backward) x (batch, token, head).
+ * v2a_linattn_step: one token for B rows.  state [N,H,Dk,Dv] is updated in place; row b uses state slots[b] (NULL: b).  Rows whose slot is
+ *   outside [0, N) give 0 and touch no state; rows that name the same slot are taken in row order, as successive tokens.
+ *   q [B,Hq,Dk], k [B,Hk,Dk], v [B,Hv,Dv], out [B,H,Dv] contiguous; strides: HOST array, q, k, v, g x (batch, head). */
+size_t v2a_linattn_fwd_workspace_bytes(int B, int T, int H, int Dk, int Dv, int dtype);
+int v2a_linattn_fwd(const void* q, const void* k, const void* v, const float* g, const float* state, const int32_t* lens, void* out, float* state_out,
+                    const int64_t* strides, int B, int T, int H, int Hq, int Hk, int Hv, int Dk, int Dv, int dtype, float scale, void* ws, size_t ws_bytes,
+                    v2a_stream_t s);
+size_t v2a_linattn_bwd_workspace_bytes(int B, int T, int H, int Hq, int Hk, int Hv, int Dk, int Dv, int dtype, int per_token_decay);
+int v2a_linattn_bwd(const void* q, const void* k, const void* v, const float* g, const float* state, const int32_t* lens, const void* dout,
+                    const float* dstate_out, void* dq, void* dk, void* dv, float* dg, float* dstate, const int64_t* strides, int B, int T, int H, int Hq, int Hk,
+                    int Hv, int Dk, int Dv, int dtype, int per_token_decay, float scale, void* ws, size_t ws_bytes, v2a_stream_t s);
+int v2a_linattn_step(const void* q, const void* k, const void* v, const float* g, float* state, const int32_t* slots, void* out, const int64_t* strides, int B,
+                     int N, int H, int Hq, int Hk, int Hv, int Dk, int Dv, int dtype, float scale, v2a_stream_t s);
+/* Token embedding: out[i] = scale * table[ids[i]] + pos[i mod T] for N ids in rows of T (pos NULL: none), and its gradient: dtable [V][D] =
+ * scale * sum of dout over the tokens of each row (every row written; fixed order), dpos [pos_rows][D] = sum over the N / T rows (NULL: none).
+ * ids int64 (ids64 = 1) or int32, contiguous; ids outside [0, V) are empty: a zero row (no pos either), no gradient.  table / pos rows at
+ * ld_table / ld_pos elements; out, dout, dtable, dpos contiguous; dtype 0 fp32 / 1 bf16 / 2 fp16, sums in fp32, rounded once. */
+int v2a_embed_fwd(const void* ids, int ids64, const void* table, const void* pos, void* out, long long N, long long T, long long V, int D, long long ld_table,
+                  long long ld_pos, int dtype, float scale, v2a_stream_t s);
+size_t v2a_embed_bwd_workspace_bytes(long long N, long long V, int D);
+int v2a_embed_bwd(const void* ids, int ids64, const void* dout, void* dtable, void* dpos, long long N, long long T, long long V, int D, long long pos_rows, int dtype,
+                  float scale, void* ws, size_t ws_bytes, v2a_stream_t s);
 /* video-model training (GoalGaussianDiffusion.forward / p_losses, flowdiffusion/flowdiffusion/goal_diffusion.py:674-724):
  * q_sample (:674-680) with the [0,1] -> [-1,1] normalisation of forward (:722) folded in; per-sample mean of l2 / l1 (objective 0 =
  * pred_noise, 1 = pred_x0, 2 = pred_v, :699-707) times loss_weight[t] then the batch mean (:709-713); and its gradient with respect to

@@ -107,6 +107,14 @@ SIGNATURES = {
     "v2a_mha_fwd": (I, [P, P, P, P, P, I, I, I, I, I, I, I, I, F, U64, U64, P]),
     "v2a_mha_bwd": (I, [P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, F, U64, U64, P]),
     "v2a_dropout": (I, [P, P, SZ, F, U64, U64, P]),
+    "v2a_linattn_fwd_workspace_bytes": (SZ, [I] * 6),
+    "v2a_linattn_fwd": (I, [P] * 9 + [I] * 9 + [F, P, SZ, P]),
+    "v2a_linattn_bwd_workspace_bytes": (SZ, [I] * 10),
+    "v2a_linattn_bwd": (I, [P] * 14 + [I] * 10 + [F, P, SZ, P]),
+    "v2a_linattn_step": (I, [P] * 8 + [I] * 9 + [F, P]),
+    "v2a_embed_fwd": (I, [P, I, P, P, P, LL, LL, LL, I, LL, LL, I, F, P]),
+    "v2a_embed_bwd_workspace_bytes": (SZ, [LL, LL, I]),
+    "v2a_embed_bwd": (I, [P, I, P, P, P, LL, LL, LL, I, LL, I, F, P, SZ, P]),
     "v2a_video_qsample": (I, [P, P, P, P, P, P, I, SZ, I, P]),
     "v2a_video_loss_workspace_bytes": (SZ, [I]),
     "v2a_video_loss_fwd": (I, [P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, P, SZ, P]),
