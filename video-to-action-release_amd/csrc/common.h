@@ -90,7 +90,7 @@ __device__ __forceinline__ float v2a_silu_fast(float x) {
     return x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504088896340736f * x));
 }
 
-// GroupNorm affine + activation on one packed pair of 16-bit elements, two-wide fp32 VALU (v_pk_fma / v_pk_mul / v_pk_add):
+// GroupNorm affine + activation on one packed pair of 16-bit elements:
 // z = x * a + b; SiLU: z * rcp(1 + exp2(-log2(e) * z)) -- the arithmetic of v2a_silu_fast.  Shared by gn_apply_h and the halo conv's
 // loader, which must agree bit for bit.
 template <bool F16> __device__ __forceinline__ unsigned int v2a_gn_act2(unsigned int u, v2a_f32x2 a, v2a_f32x2 b, bool silu) {
