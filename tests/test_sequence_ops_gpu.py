@@ -26,10 +26,10 @@ def ops():
     return ops
 
 
-def near(got, want, mag, intype, n, what):
+def near(got, want, mag, intype, n, what, times=1):
     got, want = got.detach().cpu(), want.cpu()
     assert got.shape == want.shape, (what, got.shape, want.shape)
-    tol = U[got.dtype] * want.abs() + (E[intype] + n * 2.0 ** -24) * mag.cpu() + 1e-37
+    tol = times * (U[got.dtype] * want.abs() + (E[intype] + n * 2.0 ** -24) * mag.cpu()) + 1e-37
     if got.dtype == FP:
         tol = tol + 2.0 ** -25                 # fp16 subnormals: half a step
     err = (got.double() - want).abs()
@@ -159,7 +159,9 @@ def test_decays_that_clear_the_state(low, dt):
     a = [c[x][:, 100:].contiguous() for x in ("q", "k", "v", "g")]
     alone, _ = ops().linear_attention_fwd(*(cu(x) for x in a))
     both, _ = ops().linear_attention_fwd(*(cu(c[x]) for x in ("q", "k", "v", "g")), state=cu(c["state"]))
-    near(both[:, 100:], alone.double(), O.attend(*(ab(x) for x in a[:3]), a[3])[0], dt, 300, "after a reset")
+    # both are computed: |both - alone| <= |both - true| + |alone - true|, twice the bound (and the value the bound goes by is itself off by one
+    # rounding u, which moves the bound by u^2 |value| <= 2^-16 |value| <= E mag of the 16-bit types, covered by the third)
+    near(both[:, 100:], alone.double(), O.attend(*(ab(x) for x in a[:3]), a[3])[0], dt, 300, "after a reset", times=3)
 
 
 @pytest.mark.parametrize("dt", [F32, BF, FP], ids=["fp32", "bf16", "fp16"])

@@ -28,143 +28,838 @@ __device__ __forceinline__ int la_len(const LaArgs& a, int b) {
 }
 __device__ __forceinline__ float la_clampg(float g) { return g < LA_GMIN ? LA_GMIN : g; }
 
-// one workgroup per (batch, head), token by token, the state in LDS
-template <int DT>
-__global__ __launch_bounds__(128) void la_fwd_simple(LaArgs a, void* out_, float* state_out) {
-    typedef typename LaT<DT>::T E;
-    __shared__ float S[LA_DMAX * LA_DMAX];
-    __shared__ float qb[LA_DMAX], kb[LA_DMAX];
-    const int b = blockIdx.x / a.H, h = blockIdx.x % a.H, x = threadIdx.x, Dk = a.Dk, Dv = a.Dv;
-    const int hq = h / (a.H / a.Hq), hk = h / (a.H / a.Hk), hv = h / (a.H / a.Hv), n = la_len(a, b);
-    const long long so = (long long)blockIdx.x * Dk * Dv;
-    for (int e = x; e < Dk * Dv; e += 128) S[e] = a.state ? a.state[so + e] : 0.f;
-    E* out = (E*)out_;
-    for (int t = 0; t < a.T; ++t) {
-        E* o = out + (((long long)b * a.T + t) * a.H + h) * Dv;
-        if (t >= n) { if (x < Dv) o[x] = LaT<DT>::st(0.f); continue; }
-        __syncthreads();
-        if (x < Dk) {
-            qb[x] = LaT<DT>::ld(((const E*)a.q)[b * a.qs[0] + t * a.qs[1] + hq * a.qs[2] + x]);
-            kb[x] = LaT<DT>::ld(((const E*)a.k)[b * a.ks[0] + t * a.ks[1] + hk * a.ks[2] + x]);
+// ---------------------------------------------------------------------------------------------------------------------- chunked form
+// A chunk is 64 tokens.  With G_i = g_1 + .. + g_i inside it, W_ij = exp(G_i - G_j) for j <= i and S the state before it,
+//     o_i = scale (exp(G_i) S^T q_i + sum_j W_ij (q_i . k_j) v_j),      S' = exp(G_64) S + sum_j exp(G_64 - G_j) k_j v_j^T,
+// all of it matrix products.  They run on 16 x 16 x 32 MFMA tiles whose 32-long reduction index is numbered so that no operand is ever
+// shuffled: slot e of lane group lane / 16 is element 4 (lane / 16) + e for e < 4 and 16 + 4 (lane / 16) + e - 4 above.  With that
+// numbering two stacked 16 x 16 accumulators ARE the next product's operand (rows of one index, lane % 16 the other): the pair scores and
+// the state go from accumulator to operand in registers, and a transposing LDS read (ds_read_b64_tr_b16) of a row-major tile gives the
+// operand of the transposed tile.
+// Number formats: bf16 inputs are one exact 8-bit plane, fp16 inputs two (8 + 3 bits, exact); factors computed in fp32 (scores, states)
+// are fed as two planes (off by at most 2^-17 of the value), decay-weighted values of the state update as three (exact fp32), because the
+// state is an fp32 result and lives long.  Sums are fp32.  fp32 inputs use the fp32 MFMA (16 x 16 x 4) in the same slot order.
+// Running log decays are summed in fp64 and kept as a float pair: W of two tokens behind a reset (g clamped at -1000) keeps its digits.
+constexpr int LA_C = 64;
+constexpr float LA_LOG2E = 1.44269504088896340736f;
+typedef __attribute__((ext_vector_type(4))) unsigned int la_u32x4;
+typedef __attribute__((ext_vector_type(2))) unsigned int la_u32x2;
+typedef __attribute__((ext_vector_type(4))) __bf16 la_bf16x4;
+typedef __attribute__((address_space(3))) la_bf16x4 la_lds_bf16x4;
+
+template <int NP> struct LaP { la_u32x4 p[NP]; };      // eight values as NP bf16 planes
+struct LaF { float x[8]; };                            // eight fp32 values
+template <int DT> struct LaOp {                        // operand of an input tile; LDS bytes of a tile element
+    typedef LaP<DT == 2 ? 2 : 1> In;
+    typedef LaP<2> C2;
+    typedef LaP<3> C3;
+    static constexpr int NP = DT == 2 ? 2 : 1;
+};
+template <> struct LaOp<0> {
+    typedef LaF In;
+    typedef LaF C2;
+    typedef LaF C3;
+    static constexpr int NP = 1;
+};
+
+template <int NP> __device__ __forceinline__ void la_split(const float* x, LaP<NP>& o) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        float a = x[2 * e], b = x[2 * e + 1];
+#pragma unroll
+        for (int n = 0; n < NP; ++n) {
+            const unsigned int h = v2a_pack_bf16x2(a, b);
+            o.p[n][e] = h;
+            a -= __uint_as_float(h << 16);
+            b -= __uint_as_float(h & 0xffff0000u);
         }
-        __syncthreads();
-        if (x < Dv) {
-            const float w = expf(la_clampg(a.g[b * a.gs[0] + t * a.gs[1] + h * a.gs[2]]));
-            const float vv = LaT<DT>::ld(((const E*)a.v)[b * a.vs[0] + t * a.vs[1] + hv * a.vs[2] + x]);
-            float s = 0.f;
-            for (int c = 0; c < Dk; ++c) {
-                const float y = S[c * Dv + x] * w + kb[c] * vv;
-                S[c * Dv + x] = y;
-                s += qb[c] * y;
+    }
+}
+__device__ __forceinline__ void la_split(const float* x, LaF& o) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o.x[e] = x[e];
+}
+template <int NP> __device__ __forceinline__ void la_join(const LaP<NP>& o, float* x) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        x[2 * e] = 0.f;
+        x[2 * e + 1] = 0.f;
+#pragma unroll
+        for (int n = NP - 1; n >= 0; --n) {
+            x[2 * e] += __uint_as_float(o.p[n][e] << 16);
+            x[2 * e + 1] += __uint_as_float(o.p[n][e] & 0xffff0000u);
+        }
+    }
+}
+__device__ __forceinline__ void la_join(const LaF& o, float* x) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = o.x[e];
+}
+
+// c[row: index of a][col: index of b] += sum over the 32 slots; small products first.  ALL: every pair of planes (both operands exact), else
+// those at least as large as the pieces that the more finely split operand still holds
+template <int NA, int NB, bool ALL = false> __device__ __forceinline__ void la_mma(f32x4& c, const LaP<NA>& a, const LaP<NB>& b) {
+    constexpr int TOP = ALL ? NA + NB - 2 : (NA > NB ? NA : NB) - 1;
+#pragma unroll
+    for (int o = TOP; o >= 0; --o)
+#pragma unroll
+        for (int i = 0; i < NA; ++i)
+            if (o - i >= 0 && o - i < NB)
+                c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v2a_bf16x8, a.p[i]), __builtin_bit_cast(v2a_bf16x8, b.p[o - i]), c, 0, 0, 0);
+}
+template <int A = 0, int B = 0, bool ALL = false> __device__ __forceinline__ void la_mma(f32x4& c, const LaF& a, const LaF& b) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.x[e], b.x[e], c, 0, 0, 0);
+}
+template <int DT> __device__ __forceinline__ void la_mma_in(f32x4& c, const typename LaOp<DT>::In& a, const typename LaOp<DT>::In& b) {
+    if constexpr (DT == 0) la_mma(c, a, b);
+    else la_mma<LaOp<DT>::NP, LaOp<DT>::NP, true>(c, a, b);
+}
+
+// A 64 x D tile in LDS, rows padded by 16 bytes.  nat: lane % 16 = row, slots along the row; tr: lane % 16 = column, slots down the rows
+template <int DT, int D> struct LaTile {
+    static constexpr int NP = LaOp<DT>::NP;
+    static constexpr int PITCH = DT == 0 ? (D + 4) * 4 : (D + 8) * 2;      // bytes
+    static constexpr int PLANE = LA_C * PITCH;
+    static constexpr int BYTES = PLANE * NP;
+    static __device__ __forceinline__ void nat(const char* t, int row0, int kk, int lane, typename LaOp<DT>::In& o) {
+        const char* q = t + (row0 + (lane & 15)) * PITCH;
+        if constexpr (DT == 0) {
+            const float4 a = *(const float4*)(q + (kk * 32 + (lane >> 4) * 4) * 4), b = *(const float4*)(q + (kk * 32 + 16 + (lane >> 4) * 4) * 4);
+            o.x[0] = a.x; o.x[1] = a.y; o.x[2] = a.z; o.x[3] = a.w; o.x[4] = b.x; o.x[5] = b.y; o.x[6] = b.z; o.x[7] = b.w;
+        } else {
+#pragma unroll
+            for (int n = 0; n < NP; ++n) {
+                const la_u32x2 a = *(const la_u32x2*)(q + n * PLANE + (kk * 32 + (lane >> 4) * 4) * 2);
+                const la_u32x2 b = *(const la_u32x2*)(q + n * PLANE + (kk * 32 + 16 + (lane >> 4) * 4) * 2);
+                o.p[n] = la_u32x4{a[0], a[1], b[0], b[1]};
             }
-            o[x] = LaT<DT>::st(s * a.scale);
         }
     }
-    __syncthreads();
-    if (state_out) for (int e = x; e < Dk * Dv; e += 128) state_out[so + e] = S[e];
-}
-
-// forward pass of the gradient: dq per head and the last state
-template <int DT>
-__global__ __launch_bounds__(128) void la_bwd_q_simple(LaArgs a, float* dqh, float* last) {
-    typedef typename LaT<DT>::T E;
-    __shared__ float S[LA_DMAX * LA_DMAX];
-    __shared__ float kb[LA_DMAX], vb[LA_DMAX], db[LA_DMAX];
-    const int b = blockIdx.x / a.H, h = blockIdx.x % a.H, x = threadIdx.x, Dk = a.Dk, Dv = a.Dv;
-    const int hk = h / (a.H / a.Hk), hv = h / (a.H / a.Hv), n = la_len(a, b);
-    const long long so = (long long)blockIdx.x * Dk * Dv;
-    for (int e = x; e < Dk * Dv; e += 128) S[e] = a.state ? a.state[so + e] : 0.f;
-    for (int t = 0; t < a.T; ++t) {
-        float* o = dqh + (((long long)b * a.T + t) * a.H + h) * Dk;
-        if (t >= n) { if (x < Dk) o[x] = 0.f; continue; }
-        __syncthreads();
-        if (x < Dk) kb[x] = LaT<DT>::ld(((const E*)a.k)[b * a.ks[0] + t * a.ks[1] + hk * a.ks[2] + x]);
-        if (x < Dv) {
-            vb[x] = LaT<DT>::ld(((const E*)a.v)[b * a.vs[0] + t * a.vs[1] + hv * a.vs[2] + x]);
-            db[x] = LaT<DT>::ld(((const E*)a.dout)[b * a.ds[0] + t * a.ds[1] + h * a.ds[2] + x]);
-        }
-        __syncthreads();
-        if (x < Dk) {
-            const float w = expf(la_clampg(a.g[b * a.gs[0] + t * a.gs[1] + h * a.gs[2]]));
-            float s = 0.f;
-            for (int c = 0; c < Dv; ++c) {
-                const float y = S[x * Dv + c] * w + kb[x] * vb[c];
-                S[x * Dv + c] = y;
-                s += db[c] * y;
+    static __device__ __forceinline__ void tr(const char* t, int ks, int col0, int lane, typename LaOp<DT>::In& o) {
+        if constexpr (DT == 0) {
+            const char* q = t + (ks * 32 + (lane >> 4) * 4) * PITCH + (col0 + (lane & 15)) * 4;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o.x[e] = *(const float*)(q + (e < 4 ? e : 12 + e) * PITCH);
+        } else {
+            const char* q = t + (ks * 32 + (lane >> 4) * 4 + ((lane & 15) >> 2)) * PITCH + (col0 + 4 * (lane & 3)) * 2;
+#pragma unroll
+            for (int n = 0; n < NP; ++n) {
+                const la_u32x2 a = __builtin_bit_cast(la_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4bf16((la_lds_bf16x4*)(q + n * PLANE)));
+                const la_u32x2 b = __builtin_bit_cast(la_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4bf16((la_lds_bf16x4*)(q + n * PLANE + 16 * PITCH)));
+                o.p[n] = la_u32x4{a[0], a[1], b[0], b[1]};
             }
-            o[x] = s * a.scale;
         }
     }
-    __syncthreads();
-    for (int e = x; e < Dk * Dv; e += 128) last[so + e] = S[e];
-}
-
-__device__ double la_blocksum(double v, double* red) {
-    v = wave_sum_d(v);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    return red[0] + red[1];
-}
-
-// reverse pass: dk, dv per head, d decay per token, gradient of the first state
-template <int DT>
-__global__ __launch_bounds__(128) void la_bwd_kv_simple(LaArgs a, const float* dqh, const float* last, const float* dlast, float* dkh, float* dvh,
-                                                        float* dgt, float* dstate) {
-    typedef typename LaT<DT>::T E;
-    __shared__ float S[LA_DMAX * LA_DMAX];
-    __shared__ float qb[LA_DMAX], kb[LA_DMAX], vb[LA_DMAX], db[LA_DMAX];
-    __shared__ double red[2];
-    const int b = blockIdx.x / a.H, h = blockIdx.x % a.H, x = threadIdx.x, Dk = a.Dk, Dv = a.Dv;
-    const int hq = h / (a.H / a.Hq), hk = h / (a.H / a.Hk), hv = h / (a.H / a.Hv), n = la_len(a, b);
-    const long long so = (long long)blockIdx.x * Dk * Dv;
-    double cross = 0.0;
-    for (int e = x; e < Dk * Dv; e += 128) {
-        S[e] = dlast ? dlast[so + e] : 0.f;
-        cross += (double)S[e] * last[so + e];
+    static __device__ __forceinline__ void four(const char* t, int row, int col, float* x) {      // four neighbours of a row
+        const char* q = t + row * PITCH;
+        if constexpr (DT == 0) {
+            const float4 a = *(const float4*)(q + col * 4);
+            x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+        } else {
+            x[0] = x[1] = x[2] = x[3] = 0.f;
+#pragma unroll
+            for (int n = NP - 1; n >= 0; --n) {
+                const la_u32x2 a = *(const la_u32x2*)(q + n * PLANE + col * 2);
+                x[0] += __uint_as_float(a[0] << 16); x[1] += __uint_as_float(a[0] & 0xffff0000u);
+                x[2] += __uint_as_float(a[1] << 16); x[3] += __uint_as_float(a[1] & 0xffff0000u);
+            }
+        }
     }
-    cross = la_blocksum(cross, red);
-    for (int t = a.T - 1; t >= 0; --t) {
-        const long long row = ((long long)b * a.T + t) * a.H + h;
-        if (t >= n) {
-            if (x < Dk) dkh[row * Dk + x] = 0.f;
-            if (x < Dv) dvh[row * Dv + x] = 0.f;
-            if (x == 0) dgt[row] = 0.f;
+};
+
+// Global rows -> registers (load) -> LDS (store), so that the next chunk's rows are under way while this one is computed.  Rows from nv on
+// and columns from Dx on are zeros and not read.  vec: base, strides and Dx allow 16-byte loads; else element by element.
+template <int DT, int D, int NTH> struct LaLoad {
+    typedef typename LaT<DT>::T E;
+    static constexpr int EPC = DT == 0 ? 4 : 8, CPR = D / EPC, N = LA_C * CPR / NTH;
+    static_assert(LA_C * CPR % NTH == 0, "whole 16-byte pieces per thread");
+    static_assert(NTH % CPR == 0, "a thread's pieces share their columns");
+    la_u32x4 r[N];
+    // thread t owns columns EPC (t % CPR) .. of rows t / CPR + i NTH / CPR
+    __device__ __forceinline__ void load(const E* p, long long st, int nv, int Dx, int vec) {
+        const int row = threadIdx.x / CPR, c = (threadIdx.x % CPR) * EPC;
+        const E* q = p + row * st + c;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            r[i] = la_u32x4{0u, 0u, 0u, 0u};
+            if (row + i * (NTH / CPR) < nv && c < Dx) {
+                if (vec) r[i] = *(const la_u32x4*)q;
+                else {
+#pragma unroll
+                    for (int e = 0; e < EPC; ++e)
+                        if (c + e < Dx) {
+                            if constexpr (DT == 0) r[i][e] = __float_as_uint(q[e]);
+                            else r[i][e >> 1] |= (unsigned int)q[e] << (16 * (e & 1));
+                        }
+                }
+            }
+            q += st * (NTH / CPR);
+        }
+    }
+    __device__ __forceinline__ void store(char* t) const {
+        typedef LaTile<DT, D> TT;
+        char* q = t + threadIdx.x / CPR * TT::PITCH + (threadIdx.x % CPR) * EPC * (DT == 0 ? 4 : 2);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if constexpr (DT == 2) {
+                la_u32x4 hi, lo;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float a = v2a_lo_h2<true>(r[i][e]), b = v2a_hi_h2<true>(r[i][e]);
+                    hi[e] = v2a_pack_bf16x2(a, b);
+                    lo[e] = v2a_pack_bf16x2(a - __uint_as_float(hi[e] << 16), b - __uint_as_float(hi[e] & 0xffff0000u));
+                }
+                *(la_u32x4*)(q + i * (NTH / CPR) * TT::PITCH) = hi;
+                *(la_u32x4*)(q + i * (NTH / CPR) * TT::PITCH + TT::PLANE) = lo;
+            } else *(la_u32x4*)(q + i * (NTH / CPR) * TT::PITCH) = r[i];
+        }
+    }
+};
+
+// Running log2 decays of a chunk in every lane of one wave (lane = token): pair hi + lo, and the chunk's total
+struct LaGate {
+    float hi[LA_C], lo[LA_C];          // G_i
+    float wq[LA_C], wk[LA_C];          // exp(G_i), exp(G_64 - G_i)
+    float total;                       // exp(G_64)
+};
+__device__ __forceinline__ void la_gates(LaGate& s, float g, bool on, int lane) {
+    double x = on ? (double)la_clampg(g) * 1.4426950408889634 : 0.0;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const double y = __shfl_up(x, o, 64);
+        if (lane >= o) x += y;
+    }
+    const double tot = __shfl(x, 63, 64);
+    const float hi = (float)x;
+    s.hi[lane] = hi;
+    s.lo[lane] = (float)(x - (double)hi);
+    s.wq[lane] = __builtin_amdgcn_exp2f(hi);
+    s.wk[lane] = __builtin_amdgcn_exp2f((float)(tot - x));
+    if (lane == 63) s.total = __builtin_amdgcn_exp2f((float)tot);
+}
+
+// The six (16-row tile, 32-slot step) units of the lower triangle of a 64 x 64 score matrix, and the wave that computes each
+__device__ constexpr int la_unit_tile(int u) { return u == 0 ? 0 : u == 1 ? 1 : u < 4 ? 2 : 3; }
+__device__ constexpr int la_unit_step(int u) { return u == 3 || u == 5 ? 1 : 0; }
+__device__ constexpr int la_unit_wave(int u, int nw) { return nw == 1 ? 0 : nw == 2 ? u / 3 : nw == 4 ? (u < 2 ? 0 : u < 4 ? 1 : u - 2) : u; }
+template <int DT> constexpr int la_unit_bytes() { return 64 * 32; }      // two planes of 16 bytes a lane, or eight floats
+
+template <int DT> __device__ __forceinline__ void la_put(char* p, int u, int lane, const float* x) {
+    typename LaOp<DT>::C2 o;
+    la_split(x, o);
+    la_u32x4* q = (la_u32x4*)(p + u * la_unit_bytes<DT>()) + lane;
+    if constexpr (DT == 0) {
+        q[0] = la_u32x4{__float_as_uint(o.x[0]), __float_as_uint(o.x[1]), __float_as_uint(o.x[2]), __float_as_uint(o.x[3])};
+        q[64] = la_u32x4{__float_as_uint(o.x[4]), __float_as_uint(o.x[5]), __float_as_uint(o.x[6]), __float_as_uint(o.x[7])};
+    } else {
+        q[0] = o.p[0];
+        q[64] = o.p[1];
+    }
+}
+template <int DT> __device__ __forceinline__ void la_get(const char* p, int u, int lane, typename LaOp<DT>::C2& o) {
+    const la_u32x4* q = (const la_u32x4*)(p + u * la_unit_bytes<DT>()) + lane;
+    const la_u32x4 a = q[0], b = q[64];
+    if constexpr (DT == 0) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { o.x[e] = __uint_as_float(a[e]); o.x[4 + e] = __uint_as_float(b[e]); }
+    } else {
+        o.p[0] = a;
+        o.p[1] = b;
+    }
+}
+
+// exp(G_i - G_j) of the four slots 4 (lane / 16) .. of the 16 tokens from t0 against the one token `one`; FIRST: the slots are i (rows), else j
+template <bool SLOTS_I> __device__ __forceinline__ void la_weights(const LaGate& gt, int t0, int one, int lane, float* w) {
+    const float h1 = gt.hi[one], l1 = gt.lo[one];
+    const int s0 = t0 + (lane >> 4) * 4;
+    const float4 h = *(const float4*)&gt.hi[s0], l = *(const float4*)&gt.lo[s0];
+    const float hh[4] = {h.x, h.y, h.z, h.w}, ll[4] = {l.x, l.y, l.z, l.w};
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const float d = SLOTS_I ? (hh[r] - h1) + (ll[r] - l1) : (h1 - hh[r]) + (l1 - ll[r]);
+        const bool in = SLOTS_I ? s0 + r >= one : s0 + r <= one;
+        w[r] = in ? __builtin_amdgcn_exp2f(d) : 0.f;
+    }
+}
+
+template <int DT> __device__ __forceinline__ void la_store4(typename LaT<DT>::T* p, const f32x4& x, int room, bool vec) {
+    if (vec && room >= 4) {
+        if constexpr (DT == 0) *(f32x4*)p = x;
+        else *(la_u32x2*)p = la_u32x2{v2a_pack_h2<DT == 2>(x[0], x[1]), v2a_pack_h2<DT == 2>(x[2], x[3])};
+    } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (r < room) p[r] = LaT<DT>::st(x[r]);
+    }
+}
+
+struct LaScan {
+    const float* init;          // state before the first chunk in scan order (NULL: 0)
+    float* seg;                 // [B H][nseg][Dk][Dv]: local states of the segments (local) / states before them (otherwise, nseg > 1)
+    float* seg_decay;           // [B H][nseg]
+    float* chunk;               // state before each chunk in scan order, [B H][NC][Dk][Dv] (NULL: not kept)
+    float* last;                // state behind the last chunk (NULL)
+    void* out;
+    int NC, cps, nseg, ndv, local, rev, vx, vy, vq, vo;
+};
+
+// One workgroup walks the chunks of one segment of one (row, head) for NW * NT * 16 columns of the state, which stays in registers as
+// accumulators: wave w owns columns 16 NT w .. and all Dk rows.  OUT: the outputs too.  rev: the recurrence of the state's gradient, from the
+// last chunk to the first, E <- exp(G_64) E + scale sum_i exp(G_i) q_i dout_i^T (x = q, y = dout), else x = k, y = v.
+template <int DT, int DK, int NT, int NW, bool OUT>
+__global__ __launch_bounds__(64 * NW, 2) void la_scan(LaArgs a, LaScan p) {
+    typedef typename LaT<DT>::T E;
+    typedef LaTile<DT, DK> TX;
+    constexpr int DVT = 16 * NT * NW, NTH = 64 * NW;
+    typedef LaTile<DT, DVT> TY;
+    constexpr int QB = OUT ? TX::BYTES : 0, PB = OUT ? 6 * la_unit_bytes<DT>() : 0;
+    __shared__ __attribute__((aligned(16))) char sm[TX::BYTES + TY::BYTES + QB + PB];
+    __shared__ __attribute__((aligned(16))) LaGate gt;
+    char* sx = sm;
+    char* sy = sx + TX::BYTES;
+    char* sq = sy + TY::BYTES;
+    char* sp = sq + QB;
+    const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int blk = blockIdx.x;
+    const int dvt = blk % p.ndv;
+    blk /= p.ndv;
+    const int seg = blk % p.nseg, bh = blk / p.nseg, b = bh / a.H, h = bh % a.H;
+    const int len = la_len(a, b), Dk = a.Dk, Dv = a.Dv, dv0 = dvt * DVT + wid * NT * 16;
+    const int hq = h / (a.H / a.Hq), hk = h / (a.H / a.Hk), hv = h / (a.H / a.Hv);
+    const int yroom = Dv - dvt * DVT < DVT ? Dv - dvt * DVT : DVT;
+    const E* X = p.rev ? (const E*)a.q + b * a.qs[0] + hq * a.qs[2] : (const E*)a.k + b * a.ks[0] + hk * a.ks[2];
+    const E* Y = (p.rev ? (const E*)a.dout + b * a.ds[0] + h * a.ds[2] : (const E*)a.v + b * a.vs[0] + hv * a.vs[2]) + dvt * DVT;
+    const E* Q = (const E*)a.q + b * a.qs[0] + hq * a.qs[2];
+    const long long sxt = p.rev ? a.qs[1] : a.ks[1], syt = p.rev ? a.ds[1] : a.vs[1];
+    const float* g = a.g + b * a.gs[0] + h * a.gs[2];
+    const long long SS = (long long)Dk * Dv;
+
+    f32x4 S[DK / 16][NT];
+    const int d0 = (lane >> 4) * 4, c0 = dv0 + (lane & 15);      // of this lane's state values: rows d0 + 16 i + r, columns c0 + 16 n
+    {
+        const float* s0 = p.local ? nullptr : seg ? p.seg + ((long long)bh * p.nseg + seg) * SS : p.init ? p.init + bh * SS : nullptr;
+        const float* q = s0 + d0 * Dv + c0;
+#pragma unroll
+        for (int i = 0; i < DK / 16; ++i)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) S[i][n][r] = s0 && d0 + i * 16 + r < Dk && c0 + n * 16 < Dv ? q[(i * 16 + r) * Dv + n * 16] : 0.f;
+    }
+    auto put_state = [&](float* dst) {
+        float* q = dst + d0 * Dv + c0;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+            if (c0 + n * 16 < Dv)
+#pragma unroll
+                for (int i = 0; i < DK / 16; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (d0 + i * 16 + r < Dk) q[(i * 16 + r) * Dv + n * 16] = S[i][n][r];
+    };
+    LaLoad<DT, DK, NTH> rx, rq;
+    LaLoad<DT, DVT, NTH> ry;
+    float rg = 0.f;
+    auto valid = [&](int i) {
+        const int n = len - (p.rev ? p.NC - 1 - i : i) * LA_C;
+        return n < 0 ? 0 : n > LA_C ? LA_C : n;
+    };
+    const int iend = (seg + 1) * p.cps < p.NC ? (seg + 1) * p.cps : p.NC;
+    auto fetch = [&](int i) {
+        if (i >= iend) return;
+        const int nv = valid(i);
+        if (nv == 0) return;
+        const long long t0 = (long long)(p.rev ? p.NC - 1 - i : i) * LA_C;
+        rx.load(X + t0 * sxt, sxt, nv, Dk, p.vx);
+        ry.load(Y + t0 * syt, syt, nv, yroom, p.vy);
+        if constexpr (OUT) rq.load(Q + t0 * a.qs[1], a.qs[1], nv, Dk, p.vq);
+        if (wid == 0 && lane < nv) rg = g[(t0 + lane) * a.gs[1]];
+    };
+    float fac = 1.f;
+    fetch(seg * p.cps);
+    for (int i = seg * p.cps; i < iend; ++i) {
+        const int c = p.rev ? p.NC - 1 - i : i, nv = valid(i);
+        if (p.chunk && i > 0) put_state(p.chunk + ((long long)bh * p.NC + c) * SS);
+        E* out = (E*)p.out + (((long long)b * a.T + (long long)c * LA_C) * a.H + h) * Dv;
+        const int rows = a.T - c * LA_C < LA_C ? a.T - c * LA_C : LA_C;
+        const long long ot = (long long)a.H * Dv;
+        if (nv > 0) {
+            __syncthreads();
+            rx.store(sx);
+            ry.store(sy);
+            if constexpr (OUT) rq.store(sq);
+            if (wid == 0) la_gates(gt, rg, lane < nv, lane);
+            __syncthreads();
+        }
+        fetch(i + 1);
+        if (nv == 0) {                      // behind the row's end: the state stays, the outputs are 0
+            if constexpr (OUT)
+                for (int r = wid * 16 + (lane & 15); r < rows; r += 16 * NW)
+                    for (int d = dvt * DVT + (lane >> 4) * 4; d < dvt * DVT + DVT && d < Dv; d += 16)
+                        la_store4<DT>(out + r * ot + d, f32x4{0.f, 0.f, 0.f, 0.f}, Dv - d, p.vo);
             continue;
         }
-        __syncthreads();
-        if (x < Dk) {
-            qb[x] = LaT<DT>::ld(((const E*)a.q)[b * a.qs[0] + t * a.qs[1] + hq * a.qs[2] + x]);
-            kb[x] = LaT<DT>::ld(((const E*)a.k)[b * a.ks[0] + t * a.ks[1] + hk * a.ks[2] + x]);
-        }
-        if (x < Dv) {
-            vb[x] = LaT<DT>::ld(((const E*)a.v)[b * a.vs[0] + t * a.vs[1] + hv * a.vs[2] + x]);
-            db[x] = LaT<DT>::ld(((const E*)a.dout)[b * a.ds[0] + t * a.ds[1] + h * a.ds[2] + x]) * a.scale;
-        }
-        __syncthreads();
-        float dkx = 0.f, dvx = 0.f;
-        if (x < Dk)
-            for (int c = 0; c < Dv; ++c) {
-                const float y = S[x * Dv + c] + qb[x] * db[c];
-                S[x * Dv + c] = y;
-                dkx += y * vb[c];
+        f32x4 O[OUT ? NT : 1][4];
+        if constexpr (OUT) {
+#pragma unroll
+            for (int u = 0; u < 6; ++u)
+                if (la_unit_wave(u, NW) == wid && la_unit_tile(u) * 16 < nv) {
+                    const int it = la_unit_tile(u), js = la_unit_step(u) * 32;
+                    const bool two = js + 16 <= it * 16;
+                    f32x4 c0 = {0.f, 0.f, 0.f, 0.f}, c1 = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+                    for (int kk = 0; kk < DK / 32; ++kk) {
+                        typename LaOp<DT>::In qf, kf;
+                        TX::nat(sq, it * 16, kk, lane, qf);
+                        TX::nat(sx, js, kk, lane, kf);
+                        la_mma_in<DT>(c0, kf, qf);
+                        if (two) {
+                            TX::nat(sx, js + 16, kk, lane, kf);
+                            la_mma_in<DT>(c1, kf, qf);
+                        }
+                    }
+                    float w[8], x[8];
+                    la_weights<false>(gt, js, it * 16 + (lane & 15), lane, w);
+                    la_weights<false>(gt, js + 16, it * 16 + (lane & 15), lane, w + 4);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        x[r] = c0[r] * w[r] * a.scale;
+                        x[4 + r] = c1[r] * w[4 + r] * a.scale;
+                    }
+                    la_put<DT>(sp, u, lane, x);
+                }
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int it = 0; it < 4; ++it) O[n][it] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int kk = 0; kk < DK / 32; ++kk) {
+                typename LaOp<DT>::C2 sf[NT];
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    float x[8];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) { x[r] = S[2 * kk][n][r]; x[4 + r] = S[2 * kk + 1][n][r]; }
+                    la_split(x, sf[n]);
+                }
+#pragma unroll
+                for (int it = 0; it < 4; ++it) {
+                    typename LaOp<DT>::In qf;
+                    TX::nat(sq, it * 16, kk, lane, qf);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) la_mma(O[n][it], sf[n], qf);
+                }
+                __builtin_amdgcn_sched_barrier(0);      // else every operand read of the loop is hoisted and spilled
             }
-        __syncthreads();
-        if (x < Dv)
-            for (int c = 0; c < Dk; ++c) dvx += S[c * Dv + x] * kb[c];
-        double diff = 0.0;
-        if (x < Dk) {
-            dkh[row * Dk + x] = dkx;
-            diff = (double)qb[x] * dqh[row * Dk + x] - (double)kb[x] * dkx;
+#pragma unroll
+            for (int it = 0; it < 4; ++it) {
+                const float w = gt.wq[it * 16 + (lane & 15)] * a.scale;
+#pragma unroll
+                for (int n = 0; n < NT; ++n) O[n][it] *= w;
+            }
+            __syncthreads();
         }
-        if (x < Dv) dvh[row * Dv + x] = dvx;
-        cross += la_blocksum(diff, red);
-        if (x == 0) dgt[row] = (float)cross;
-        const float w = expf(la_clampg(a.g[b * a.gs[0] + t * a.gs[1] + h * a.gs[2]]));
-        for (int e = x; e < Dk * Dv; e += 128) S[e] *= w;
+        __builtin_amdgcn_sched_barrier(0);
+        const float tot = gt.total;
+#pragma unroll
+        for (int d = 0; d < DK / 16; ++d)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) S[d][n] *= tot;
+        fac *= tot;
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+            if (ks * 32 < nv) {
+                typename LaOp<DT>::In yf[NT];
+                typename LaOp<DT>::C3 yw[NT];
+                const float* wsrc = (p.rev ? gt.wq : gt.wk) + ks * 32 + (lane >> 4) * 4;
+                const float4 w0 = *(const float4*)wsrc, w1 = *(const float4*)(wsrc + 16);
+                const float sc = p.rev ? a.scale : 1.f;
+                const float w[8] = {w0.x * sc, w0.y * sc, w0.z * sc, w0.w * sc, w1.x * sc, w1.y * sc, w1.z * sc, w1.w * sc};
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    TY::tr(sy, ks, (wid * NT + n) * 16, lane, yf[n]);
+                    float x[8];
+                    la_join(yf[n], x);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[e] *= w[e];
+                    la_split(x, yw[n]);
+                }
+                if constexpr (OUT) {
+#pragma unroll
+                    for (int u = 0; u < 6; ++u)
+                        if (la_unit_step(u) == ks && la_unit_tile(u) * 16 < nv) {
+                            typename LaOp<DT>::C2 pf;
+                            la_get<DT>(sp, u, lane, pf);
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) la_mma(O[n][la_unit_tile(u)], yf[n], pf);
+                        }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+#pragma unroll
+                for (int d = 0; d < DK / 16; ++d) {
+                    typename LaOp<DT>::In xf;
+                    TX::tr(sx, ks, d * 16, lane, xf);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) la_mma(S[d][n], xf, yw[n]);
+                    if (d & 1) __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+        if constexpr (OUT) {
+#pragma unroll
+            for (int it = 0; it < 4; ++it) {
+                const int r = it * 16 + (lane & 15);
+                if (r < rows)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        const int d = dv0 + n * 16 + (lane >> 4) * 4;
+                        if (d < Dv) la_store4<DT>(out + r * ot + d, r < nv ? O[n][it] : f32x4{0.f, 0.f, 0.f, 0.f}, Dv - d, p.vo);
+                    }
+            }
+        }
+    }
+    if (p.local) {
+        put_state(p.seg + ((long long)bh * p.nseg + seg) * SS);
+        if (threadIdx.x == 0 && dvt == 0) p.seg_decay[(long long)bh * p.nseg + seg] = fac;
+    } else if (p.last && iend == p.NC) put_state(p.last + bh * SS);
+}
+
+// Local states of the segments -> states before them: S_0 = init, S_{s+1} = decay_s S_s + local_s, in place
+__global__ __launch_bounds__(256) void la_combine(float* seg, const float* seg_decay, const float* init, int nseg, long long SS) {
+    const long long bh = blockIdx.y, e = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (e >= SS) return;
+    float s = init ? init[bh * SS + e] : 0.f;
+    float* q = seg + bh * nseg * SS + e;
+    const float* f = seg_decay + bh * nseg;
+    for (int i = 0; i < nseg; ++i) {
+        const float x = i + 1 < nseg ? q[i * SS] : 0.f;
+        q[i * SS] = s;
+        s = s * f[i] + x;
+    }
+}
+
+struct LaBwd {
+    const float *s_chunk, *e_chunk;      // state before / gradient of the state behind each chunk, [B H][NC][Dk][Dv] (chunk 0 / NC - 1: the two below)
+    const float *s_first, *e_last;       // NULL: 0
+    void *dq, *dk, *dv;                  // in the inputs' type, or fp32 per head where heads are shared
+    float *dg, *dg_part;                 // per token, or the chunk's sum [NC][B H]
+    int NC, vq, vk, vv, vd, vst, fq, fk, fv;      // v: 16-byte loads allowed; f: fp32 per-head output
+};
+
+// One workgroup computes the gradients of one chunk of one (row, head):
+//   dq_i = s (exp(G_i) S do_i + sum_j W_ij (do_i . v_j) k_j)          R_i = q_i . (the first part)
+//   dk_j = exp(G_64 - G_j) E v_j + s sum_i W_ij (do_i . v_j) q_i      C_j = k_j . (the first part)
+//   dv_j = exp(G_64 - G_j) E^T k_j + s sum_i W_ij (q_i . k_j) do_i
+//   dg_t = exp(G_64) <S, E> + sum_{i >= t} (R_i + r_i - c_i) + sum_{j < t} C_j,   r_i = sum_{j < i} M_ij, c_j = sum_{i > j} M_ij,
+//          M_ij = s W_ij (q_i . k_j)(do_i . v_j): everything whose path crosses the decay of token t.
+// Wave w owns rows 16 w .. of dq^T, dk^T (and of S, E) and dv^T.  Scores are computed once, by units, and shared through LDS.
+template <int DT, int D>
+__global__ __launch_bounds__(4 * D) void la_bwd_chunk(LaArgs a, LaBwd p) {
+    typedef typename LaT<DT>::T E;
+    typedef LaTile<DT, D> TT;
+    constexpr int NW = D / 16, NTH = 64 * NW, KK = D / 32;
+    constexpr int UB = 6 * la_unit_bytes<DT>();
+    constexpr int NBUF = 4 * TT::BYTES + 3 * UB + 8192 <= 160 * 1024 ? 3 : 1;      // score buffers: all three at once where they fit
+    __shared__ __attribute__((aligned(16))) char sm[4 * TT::BYTES + NBUF * UB];
+    __shared__ __attribute__((aligned(16))) LaGate gt;
+    __shared__ float sr[NW][LA_C], sc[NW][LA_C], rm[4][LA_C], cm[2][LA_C], sz[NW];
+    char *sq = sm, *sk = sq + TT::BYTES, *sv = sk + TT::BYTES, *sd = sv + TT::BYTES, *s1 = sd + TT::BYTES;
+    char *s2 = s1 + (NBUF == 3 ? UB : 0), *s3 = s2 + (NBUF == 3 ? UB : 0);
+    const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int l16 = lane & 15, l4 = (lane >> 4) * 4;
+    const int c = blockIdx.x % p.NC, bh = blockIdx.x / p.NC, b = bh / a.H, h = bh % a.H;
+    const int Dk = a.Dk, Dv = a.Dv, w0 = wid * 16;
+    const int hq = h / (a.H / a.Hq), hk = h / (a.H / a.Hk), hv = h / (a.H / a.Hv);
+    const long long t0 = (long long)c * LA_C, SS = (long long)Dk * Dv;
+    const int rows = a.T - (int)t0 < LA_C ? a.T - (int)t0 : LA_C;
+    int nv = la_len(a, b) - (int)t0;
+    nv = nv < 0 ? 0 : nv > LA_C ? LA_C : nv;
+
+    // one row of four values of a gradient: shared heads keep fp32 per head (rows of H heads), others their own type
+    auto put = [&](void* base, int f32, int Hx, int hx, int Dx, int row, int d, const f32x4& x) {
+        if (d >= Dx || row >= rows) return;
+        if (f32) la_store4<0>((float*)base + (((long long)b * a.T + t0 + row) * a.H + h) * Dx + d, x, Dx - d, Dx % 4 == 0);
+        else la_store4<DT>((E*)base + (((long long)b * a.T + t0 + row) * Hx + hx) * Dx + d, x, Dx - d, Dx % 4 == 0);
+    };
+    if (nv == 0) {
+        const f32x4 z = {0.f, 0.f, 0.f, 0.f};
+        for (int r = l16; r < rows; r += 16) {
+            put(p.dq, p.fq, a.Hq, hq, Dk, r, w0 + l4, z);
+            put(p.dk, p.fk, a.Hk, hk, Dk, r, w0 + l4, z);
+            put(p.dv, p.fv, a.Hv, hv, Dv, r, w0 + l4, z);
+        }
+        if (wid == 0 && p.dg && lane < rows) p.dg[((long long)b * a.T + t0 + lane) * a.H + h] = 0.f;
+        if (threadIdx.x == 0 && p.dg_part) p.dg_part[(long long)c * a.B * a.H + bh] = 0.f;
+        return;
+    }
+    const E* Q = (const E*)a.q + b * a.qs[0] + t0 * a.qs[1] + hq * a.qs[2];
+    const E* K = (const E*)a.k + b * a.ks[0] + t0 * a.ks[1] + hk * a.ks[2];
+    const E* V = (const E*)a.v + b * a.vs[0] + t0 * a.vs[1] + hv * a.vs[2];
+    const E* G = (const E*)a.dout + b * a.ds[0] + t0 * a.ds[1] + h * a.ds[2];
+    const float* Sp = c == 0 ? (p.s_first ? p.s_first + bh * SS : nullptr) : p.s_chunk + ((long long)bh * p.NC + c) * SS;
+    const float* Ep = c == p.NC - 1 ? (p.e_last ? p.e_last + bh * SS : nullptr) : p.e_chunk + ((long long)bh * p.NC + c) * SS;
+    LaLoad<DT, D, NTH> rq, rk, rv, rd;
+    rq.load(Q, a.qs[1], nv, Dk, p.vq);
+    rk.load(K, a.ks[1], nv, Dk, p.vk);
+    rv.load(V, a.vs[1], nv, Dv, p.vv);
+    rd.load(G, a.ds[1], nv, Dv, p.vd);
+    const float rg = wid == 0 && lane < nv ? a.g[b * a.gs[0] + (t0 + lane) * a.gs[1] + h * a.gs[2]] : 0.f;
+    // rows w0 + l16 of S and E, in slot order along Dv
+    auto state_rows = [&](const float* st, float (&x)[KK][8]) {
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[kk][e] = 0.f;
+        if (!st || w0 + l16 >= Dk) return;
+        const float* q = st + (long long)(w0 + l16) * Dv;
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int d = kk * 32 + half * 16 + l4;
+                if (p.vst && d < Dv) *(float4*)&x[kk][half * 4] = *(const float4*)(q + d);
+                else
+                    for (int e = 0; e < 4; ++e)
+                        if (d + e < Dv) x[kk][half * 4 + e] = q[d + e];
+            }
+    };
+    float xs[KK][8], xe[KK][8];
+    state_rows(Sp, xs);
+    state_rows(Ep, xe);
+    rq.store(sq);
+    rk.store(sk);
+    rv.store(sv);
+    rd.store(sd);
+    if (wid == 0) la_gates(gt, rg, lane < nv, lane);
+    for (int e = threadIdx.x; e < 4 * LA_C; e += NTH) rm[0][e] = 0.f;
+    for (int e = threadIdx.x; e < 2 * LA_C; e += NTH) cm[0][e] = 0.f;
+    {
+        float z = 0.f;
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) z += xs[kk][e] * xe[kk][e];
+        z = wave_sum(z);
+        if (lane == 0) sz[wid] = z;
     }
     __syncthreads();
-    if (dstate) for (int e = x; e < Dk * Dv; e += 128) dstate[so + e] = S[e];
+
+    // W (do . v) with lane = i, slots = j: the operand of dq
+    auto unit1 = [&]() {
+#pragma unroll
+        for (int u = 0; u < 6; ++u) {
+            const int it = la_unit_tile(u), js = la_unit_step(u) * 32;
+            if ((NBUF == 3 && NW == 8 ? 6 + u / 3 : la_unit_wave(u, NW)) != wid || it * 16 >= nv) continue;
+            f32x4 c0 = {0.f, 0.f, 0.f, 0.f}, c1 = {0.f, 0.f, 0.f, 0.f};
+            const bool two = js + 16 <= it * 16;
+#pragma unroll
+            for (int kk = 0; kk < KK; ++kk)
+                if (kk * 32 < Dv) {
+                    typename LaOp<DT>::In df, vf;
+                    TT::nat(sd, it * 16, kk, lane, df);
+                    TT::nat(sv, js, kk, lane, vf);
+                    la_mma_in<DT>(c0, vf, df);
+                    if (two) {
+                        TT::nat(sv, js + 16, kk, lane, vf);
+                        la_mma_in<DT>(c1, vf, df);
+                    }
+                }
+            float w[8], x[8];
+            la_weights<false>(gt, js, it * 16 + l16, lane, w);
+            la_weights<false>(gt, js + 16, it * 16 + l16, lane, w + 4);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                x[r] = c0[r] * w[r] * a.scale;
+                x[4 + r] = c1[r] * w[4 + r] * a.scale;
+            }
+            la_put<DT>(s1, u, lane, x);
+        }
+    };
+    // W (x . y) with lane = j, slots = i: the operands of dk (x = do, y = v) and dv (x = q, y = k); unit u is tile 3 - tile(u), step 1 - step(u)
+    float raw[3][8];
+    auto unit23 = [&](const char* sx, const char* sy, char* dst, int Dx, bool third) {
+#pragma unroll
+        for (int u = 0; u < 6; ++u) {
+            const int jt = 3 - la_unit_tile(u), is = 32 - la_unit_step(u) * 32;
+            constexpr int per = NW == 8 ? 1 : NW == 4 ? 2 : 3;
+            const int at = u % per;
+            if (la_unit_wave(u, NW) != wid || jt * 16 >= nv || is >= nv) continue;
+            f32x4 c0 = {0.f, 0.f, 0.f, 0.f}, c1 = {0.f, 0.f, 0.f, 0.f};
+            const bool first = is + 16 > jt * 16;
+#pragma unroll
+            for (int kk = 0; kk < KK; ++kk)
+                if (kk * 32 < Dx) {
+                    typename LaOp<DT>::In xf, yf;
+                    TT::nat(sy, jt * 16, kk, lane, yf);
+                    if (first) {
+                        TT::nat(sx, is, kk, lane, xf);
+                        la_mma_in<DT>(c0, xf, yf);
+                    }
+                    TT::nat(sx, is + 16, kk, lane, xf);
+                    la_mma_in<DT>(c1, xf, yf);
+                }
+            float w[8], x[8];
+            const int j = jt * 16 + l16;
+            la_weights<true>(gt, is, j, lane, w);
+            la_weights<true>(gt, is + 16, j, lane, w + 4);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                x[r] = c0[r] * w[r] * a.scale;
+                x[4 + r] = c1[r] * w[4 + r] * a.scale;
+            }
+            la_put<DT>(dst, u, lane, x);
+            if (!third) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) { raw[at][r] = c0[r]; raw[at][4 + r] = c1[r]; }
+            } else {
+                float col = 0.f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int i = is + (e < 4 ? e : 12 + e) + l4;
+                    float m = i > j ? x[e] * raw[at][e] : 0.f;
+                    col += m;
+                    m += v2a_dpp<0xB1>(m);              // sum over the 16 lanes of a row group
+                    m += v2a_dpp<0x4E>(m);
+                    m += v2a_dpp<0x141>(m);
+                    m += v2a_dpp<0x140>(m);
+                    if (l16 == 0) rm[jt][i] = m;
+                }
+                col += __shfl_xor(col, 16, 64);
+                col += __shfl_xor(col, 32, 64);
+                if (lane < 16) cm[is >> 5][j] = col;
+            }
+        }
+    };
+    f32x4 acc[4];
+    auto clear = [&]() {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    };
+    // the part through the state: rows of `st` times the tokens' rows in `t`, weighted by w, and its product with the tokens' own rows in `own`
+    auto through_state = [&](const float (&x)[KK][8], const char* t, const float* w, float mul, const char* own, float* dst) {
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk)
+            if (kk * 32 < Dv) {
+                typename LaOp<DT>::C2 sf;
+                la_split(x[kk], sf);
+#pragma unroll
+                for (int tt = 0; tt < 4; ++tt) {
+                    typename LaOp<DT>::In tf;
+                    TT::nat(t, tt * 16, kk, lane, tf);
+                    la_mma(acc[tt], sf, tf);
+                }
+            }
+#pragma unroll
+        for (int tt = 0; tt < 4; ++tt) {
+            acc[tt] *= w[tt * 16 + l16] * mul;
+            float y[4];
+            TT::four(own, tt * 16 + l16, w0 + l4, y);
+            float s = (acc[tt][0] * y[0] + acc[tt][1] * y[1]) + (acc[tt][2] * y[2] + acc[tt][3] * y[3]);
+            s += __shfl_xor(s, 16, 64);
+            s += __shfl_xor(s, 32, 64);
+            if (lane < 16) dst[tt * 16 + lane] = s;
+        }
+    };
+    // the part within the chunk: columns w0 .. of the tokens in `t` times the shared scores
+    auto within = [&](const char* t, const char* units, bool mirrored) {
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+            if (ks * 32 < nv) {
+                typename LaOp<DT>::In tf;
+                TT::tr(t, ks, w0, lane, tf);
+#pragma unroll
+                for (int u = 0; u < 6; ++u) {
+                    const int tile = mirrored ? 3 - la_unit_tile(u) : la_unit_tile(u);
+                    if ((mirrored ? 1 - la_unit_step(u) : la_unit_step(u)) != ks || tile * 16 >= nv) continue;
+                    typename LaOp<DT>::C2 xf;
+                    la_get<DT>(units, u, lane, xf);
+                    la_mma(acc[tile], tf, xf);
+                }
+            }
+    };
+    auto emit = [&](void* base, int f32, int Hx, int hx, int Dx) {
+#pragma unroll
+        for (int tt = 0; tt < 4; ++tt) {
+            const int r = tt * 16 + l16;
+            put(base, f32, Hx, hx, Dx, r, w0 + l4, r < nv ? acc[tt] : f32x4{0.f, 0.f, 0.f, 0.f});
+        }
+    };
+    unit1();
+    if constexpr (NBUF == 3) {
+        unit23(sd, sv, s2, Dv, false);
+        unit23(sq, sk, s3, Dk, true);
+    }
+    __syncthreads();
+    clear();
+    through_state(xs, sd, gt.wq, a.scale, sq, sr[wid]);
+    within(sk, s1, false);
+    emit(p.dq, p.fq, a.Hq, hq, Dk);
+    if constexpr (NBUF == 1) {
+        __syncthreads();
+        unit23(sd, sv, s2, Dv, false);
+        __syncthreads();
+    }
+    clear();
+    through_state(xe, sv, gt.wk, 1.f, sk, sc[wid]);
+    within(sq, s2, true);
+    emit(p.dk, p.fk, a.Hk, hk, Dk);
+    if constexpr (NBUF == 1) {
+        __syncthreads();
+        unit23(sq, sk, s3, Dk, true);
+        __syncthreads();
+    }
+    clear();
+    if (Ep) {
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk)
+            if (kk * 32 < Dk) {
+                float x[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int d = kk * 32 + (e < 4 ? e : 12 + e) + l4;
+                    x[e] = d < Dk && w0 + l16 < Dv ? Ep[(long long)d * Dv + w0 + l16] : 0.f;
+                }
+                typename LaOp<DT>::C2 ef;
+                la_split(x, ef);
+#pragma unroll
+                for (int tt = 0; tt < 4; ++tt) {
+                    typename LaOp<DT>::In kf;
+                    TT::nat(sk, tt * 16, kk, lane, kf);
+                    la_mma(acc[tt], ef, kf);
+                }
+            }
+#pragma unroll
+        for (int tt = 0; tt < 4; ++tt) acc[tt] *= gt.wk[tt * 16 + l16];
+    }
+    within(sd, s3, true);
+    emit(p.dv, p.fv, a.Hv, hv, Dv);
+    __syncthreads();
+    if (wid == 0) {
+        double up = 0.0, down = 0.0, z = 0.0;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+            up += sr[w][lane];
+            down += sc[w][lane];
+            z += sz[w];
+        }
+        up += (double)((rm[0][lane] + rm[1][lane]) + (rm[2][lane] + rm[3][lane])) - (double)(cm[0][lane] + cm[1][lane]);
+        if (lane >= nv) up = down = 0.0;
+        const double own = down;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const double x = __shfl_down(up, o, 64), y = __shfl_up(down, o, 64);
+            if (lane + o < 64) up += x;
+            if (lane >= o) down += y;
+        }
+        const bool gone = __builtin_amdgcn_exp2f(la_clampg(rg) * LA_LOG2E) == 0.f;
+        double d = z * (double)gt.total + up + (down - own);
+        if (gone || lane >= nv) d = 0.0;
+        if (p.dg && lane < rows) p.dg[((long long)b * a.T + t0 + lane) * a.H + h] = (float)d;
+        if (p.dg_part) {
+            d = wave_sum_d(d);
+            if (lane == 0) p.dg_part[(long long)c * a.B * a.H + bh] = (float)d;
+        }
+    }
 }
 
 // gradients of shared heads: the heads of a group summed in order, rounded once
@@ -253,7 +948,7 @@ __global__ __launch_bounds__(256) void la_step_kernel(const void* q_, const void
 
 bool la_dims(int B, int T, int H, int Hq, int Hk, int Hv, int Dk, int Dv, int dtype) {
     return B >= 0 && T >= 0 && H > 0 && Hq > 0 && Hk > 0 && Hv > 0 && H % Hq == 0 && H % Hk == 0 && H % Hv == 0 && Dk > 0 && Dk <= LA_DMAX && Dv > 0 &&
-           Dv <= LA_DMAX && dtype >= 0 && dtype <= 2 && (long long)B * H < (1ll << 23);      // grid x block stays below 2^32 threads
+           Dv <= LA_DMAX && dtype >= 0 && dtype <= 2 && (long long)B * H * (T / 64 + 1) < (1ll << 23);      // grid x block stays below 2^32 threads
 }
 
 LaArgs la_args(const void* q, const void* k, const void* v, const float* g, const float* state, const int32_t* lens, const void* dout, const int64_t* st, int B,
@@ -274,13 +969,98 @@ size_t la_up(size_t n) { return (n + 255) & ~(size_t)255; }
         else { CALL(2); }            \
     } while (0)
 
+// How a call is cut: columns of the state per workgroup (dvt) and segments of the sequence.  One workgroup per CU and more keep the chip busy;
+// where (row, head) pairs and column tiles are fewer, the chunks are cut into segments of at least four, whose states come from a first pass.
+struct LaPlan {
+    int dvt, ndv, NC, cps, nseg;
+};
+LaPlan la_plan(int BH, int T, int Dv) {
+    LaPlan p;
+    p.dvt = Dv <= 32 ? 32 : Dv <= 64 ? 64 : 128;
+    p.ndv = cdiv(Dv, p.dvt);
+    p.NC = cdiv(T, LA_C);
+    p.nseg = 1;
+    p.cps = p.NC;
+    const long wg = (long)BH * p.ndv;
+    if (p.NC >= 8 && wg < 512) {
+        const int want = cdiv(512, wg);
+        p.cps = cdiv(p.NC, want);
+        if (p.cps < 4) p.cps = 4;
+        p.nseg = cdiv(p.NC, p.cps);
+    }
+    return p;
+}
+
+int la_vec(const void* p, const long long* st, int B, int T, int H, int D, int dtype) {
+    const long long es = dtype == 0 ? 4 : 2;
+    if (((uintptr_t)p & 15) || D * es % 16) return 0;
+    return !((B > 1 && st[0] * es % 16) || (T > 1 && st[1] * es % 16) || (H > 1 && st[2] * es % 16));
+}
+
+template <int DT, int DK, bool OUT> int la_scan_dv(const LaArgs& a, const LaScan& p, int dvt, hipStream_t s) {
+    const dim3 grid((unsigned)((long long)a.B * a.H * p.ndv * p.nseg));
+    if (dvt == 32) hipLaunchKernelGGL((la_scan<DT, DK, 1, 2, OUT>), grid, dim3(128), 0, s, a, p);
+    else if (dvt == 64) hipLaunchKernelGGL((la_scan<DT, DK, 1, 4, OUT>), grid, dim3(256), 0, s, a, p);
+    else hipLaunchKernelGGL((la_scan<DT, DK, 2, 4, OUT>), grid, dim3(256), 0, s, a, p);
+    V2A_CHECK_LAUNCH();
+    return V2A_OK;
+}
+template <int DT, bool OUT> int la_scan_dk(const LaArgs& a, const LaScan& p, int dvt, hipStream_t s) {
+    return a.Dk <= 32 ? la_scan_dv<DT, 32, OUT>(a, p, dvt, s) : a.Dk <= 64 ? la_scan_dv<DT, 64, OUT>(a, p, dvt, s) : la_scan_dv<DT, 128, OUT>(a, p, dvt, s);
+}
+template <bool OUT> int la_launch_scan(const LaArgs& a, const LaScan& p, int dvt, int dtype, hipStream_t s) {
+    return dtype == 0 ? la_scan_dk<0, OUT>(a, p, dvt, s) : dtype == 1 ? la_scan_dk<1, OUT>(a, p, dvt, s) : la_scan_dk<2, OUT>(a, p, dvt, s);
+}
+
+// A recurrence over the whole sequence: local states and their combination where there are segments, then the pass itself
+template <bool OUT> int la_recur(const LaArgs& a, LaScan p, const LaPlan& pl, int dtype, hipStream_t s) {
+    p.NC = pl.NC; p.cps = pl.cps; p.nseg = pl.nseg; p.ndv = pl.ndv;
+    const long long SS = (long long)a.Dk * a.Dv;
+    if (pl.nseg > 1) {
+        LaScan l = p;
+        l.local = 1; l.chunk = nullptr; l.last = nullptr;
+        const int rc = la_launch_scan<false>(a, l, pl.dvt, dtype, s);
+        if (rc != V2A_OK) return rc;
+        hipLaunchKernelGGL(la_combine, dim3(cdiv(SS, 256), (unsigned)(a.B * a.H)), dim3(256), 0, s, p.seg, p.seg_decay, p.init, pl.nseg, SS);
+        V2A_CHECK_LAUNCH();
+    }
+    return la_launch_scan<OUT>(a, p, pl.dvt, dtype, s);
+}
+
+struct LaFwdWs { size_t seg, decay, total; };
+LaFwdWs la_fwd_ws(const LaPlan& p, size_t BH, size_t SS) {
+    LaFwdWs w{};
+    if (p.nseg > 1) {
+        w.decay = la_up(BH * p.nseg * SS * 4);
+        w.total = w.decay + la_up(BH * p.nseg * 4);
+    }
+    return w;
+}
+struct LaBwdWs { size_t seg, decay, sch, ech, q, k, v, part, total; };
+LaBwdWs la_bwd_ws(const LaPlan& p, size_t B, size_t T, size_t H, int Hq, int Hk, int Hv, size_t Dk, size_t Dv, int per_token) {
+    LaBwdWs w{};
+    const size_t SS = Dk * Dv, BH = B * H, n = B * T * H;
+    size_t at = 0;
+    auto take = [&](size_t bytes) { const size_t o = at; at += la_up(bytes); return o; };
+    w.seg = take(p.nseg > 1 ? BH * p.nseg * SS * 4 : 0);
+    w.decay = take(p.nseg > 1 ? BH * p.nseg * 4 : 0);
+    w.sch = take(p.NC > 1 ? BH * p.NC * SS * 4 : 0);
+    w.ech = take(p.NC > 1 ? BH * p.NC * SS * 4 : 0);
+    w.q = take((size_t)Hq < H ? n * Dk * 4 : 0);
+    w.k = take((size_t)Hk < H ? n * Dk * 4 : 0);
+    w.v = take((size_t)Hv < H ? n * Dv * 4 : 0);
+    w.part = take(per_token ? 0 : BH * p.NC * 4);
+    w.total = at;
+    return w;
+}
+
 }  // namespace
 
 extern "C" {
 
 size_t v2a_linattn_fwd_workspace_bytes(int B, int T, int H, int Dk, int Dv, int dtype) {
-    (void)B; (void)T; (void)H; (void)Dk; (void)Dv; (void)dtype;
-    return 0;
+    if (!la_dims(B, T, H, H, H, H, Dk, Dv, dtype) || B == 0) return 0;
+    return la_fwd_ws(la_plan(B * H, T, Dv), (size_t)B * H, (size_t)Dk * Dv).total;
 }
 
 int v2a_linattn_fwd(const void* q, const void* k, const void* v, const float* g, const float* state, const int32_t* lens, void* out, float* state_out,
@@ -289,18 +1069,26 @@ int v2a_linattn_fwd(const void* q, const void* k, const void* v, const float* g,
     if (!strides || !la_dims(B, T, H, Hq, Hk, Hv, Dk, Dv, dtype)) return V2A_ERR_ARG;
     if (B == 0 || (T == 0 && !state_out)) return V2A_OK;
     if (T > 0 && (!q || !k || !v || !g || !out)) return V2A_ERR_ARG;
+    const LaPlan pl = la_plan(B * H, T, Dv);
+    const LaFwdWs w = la_fwd_ws(pl, (size_t)B * H, (size_t)Dk * Dv);
+    if (ws_bytes < w.total || (w.total && !ws)) return V2A_ERR_WORKSPACE;
     const LaArgs a = la_args(q, k, v, g, state, lens, nullptr, strides, B, T, H, Hq, Hk, Hv, Dk, Dv, scale);
-#define CALL(DT) hipLaunchKernelGGL((la_fwd_simple<DT>), dim3(B * H), dim3(128), 0, s, a, out, state_out)
-    LA_BY_TYPE(dtype, CALL);
-#undef CALL
-    V2A_CHECK_LAUNCH();
-    return V2A_OK;
+    LaScan p{};
+    p.init = state;
+    p.seg = (float*)((char*)ws + w.seg);
+    p.seg_decay = (float*)((char*)ws + w.decay);
+    p.last = state_out;
+    p.out = out;
+    p.vx = la_vec(k, a.ks, B, T, Hk, Dk, dtype);
+    p.vy = la_vec(v, a.vs, B, T, Hv, Dv, dtype);
+    p.vq = la_vec(q, a.qs, B, T, Hq, Dk, dtype);
+    p.vo = Dv % 4 == 0 && ((uintptr_t)out & 15) == 0;
+    return la_recur<true>(a, p, pl, dtype, s);
 }
 
 size_t v2a_linattn_bwd_workspace_bytes(int B, int T, int H, int Hq, int Hk, int Hv, int Dk, int Dv, int dtype, int per_token_decay) {
     if (!la_dims(B, T, H, Hq, Hk, Hv, Dk, Dv, dtype)) return 0;
-    const size_t n = (size_t)B * T * H;
-    return 2 * la_up(n * Dk * 4) + la_up(n * Dv * 4) + la_up((size_t)B * H * Dk * Dv * 4) + la_up(n * 4);
+    return la_bwd_ws(la_plan(B * H, T, Dv), B, T, H, Hq, Hk, Hv, Dk, Dv, per_token_decay).total;
 }
 
 int v2a_linattn_bwd(const void* q, const void* k, const void* v, const float* g, const float* state, const int32_t* lens, const void* dout,
@@ -308,32 +1096,60 @@ int v2a_linattn_bwd(const void* q, const void* k, const void* v, const float* g,
                     int Hv, int Dk, int Dv, int dtype, int per_token_decay, float scale, void* ws, size_t ws_bytes, hipStream_t s) {
     if (!strides || !la_dims(B, T, H, Hq, Hk, Hv, Dk, Dv, dtype)) return V2A_ERR_ARG;
     if (B > 0 && T > 0 && (!q || !k || !v || !g || !dout || !dq || !dk || !dv)) return V2A_ERR_ARG;
-    if (ws_bytes < v2a_linattn_bwd_workspace_bytes(B, T, H, Hq, Hk, Hv, Dk, Dv, dtype, per_token_decay) || (ws_bytes && !ws)) return V2A_ERR_WORKSPACE;
+    const LaPlan pl = la_plan(B * H, T, Dv);
+    const LaBwdWs w = la_bwd_ws(pl, B, T, H, Hq, Hk, Hv, Dk, Dv, per_token_decay);
+    if (ws_bytes < w.total || (w.total && !ws)) return V2A_ERR_WORKSPACE;
     const LaArgs a = la_args(q, k, v, g, state, lens, dout, strides, B, T, H, Hq, Hk, Hv, Dk, Dv, scale);
-    const size_t n = (size_t)B * T * H;
-    char* p = (char*)ws;
-    float* dqh = (float*)p; p += la_up(n * Dk * 4);
-    float* dkh = (float*)p; p += la_up(n * Dk * 4);
-    float* dvh = (float*)p; p += la_up(n * Dv * 4);
-    float* last = (float*)p; p += la_up((size_t)B * H * Dk * Dv * 4);
-    float* dgt = per_token_decay && dg ? dg : (float*)p;
+    auto at = [&](size_t o) { return (float*)((char*)ws + o); };
+    int rc = V2A_OK;
     if (B > 0) {
-#define CALL(DT)                                                                                        \
-    hipLaunchKernelGGL((la_bwd_q_simple<DT>), dim3(B * H), dim3(128), 0, s, a, dqh, last);              \
-    hipLaunchKernelGGL((la_bwd_kv_simple<DT>), dim3(B * H), dim3(128), 0, s, a, dqh, last, dstate_out, dkh, dvh, dgt, dstate)
-        LA_BY_TYPE(dtype, CALL);
+        LaScan p{};
+        p.seg = at(w.seg);
+        p.seg_decay = at(w.decay);
+        const int vq = la_vec(q, a.qs, B, T, Hq, Dk, dtype), vk = la_vec(k, a.ks, B, T, Hk, Dk, dtype), vv = la_vec(v, a.vs, B, T, Hv, Dv, dtype);
+        const int vd = la_vec(dout, a.ds, B, T, H, Dv, dtype);
+        if (pl.NC > 1) {
+            LaScan f = p;
+            f.init = state; f.chunk = at(w.sch); f.vx = vk; f.vy = vv;
+            rc = la_recur<false>(a, f, pl, dtype, s);
+            if (rc != V2A_OK) return rc;
+        }
+        if (pl.NC > 1 || dstate) {
+            LaScan r = p;
+            r.init = dstate_out; r.chunk = pl.NC > 1 ? at(w.ech) : nullptr; r.last = dstate; r.rev = 1; r.vx = vq; r.vy = vd;
+            rc = la_recur<false>(a, r, pl, dtype, s);
+            if (rc != V2A_OK) return rc;
+        }
+        if (T > 0) {
+            LaBwd d{};
+            d.s_chunk = at(w.sch); d.e_chunk = at(w.ech); d.s_first = state; d.e_last = dstate_out;
+            d.fq = Hq < H; d.fk = Hk < H; d.fv = Hv < H;
+            d.dq = d.fq ? (void*)at(w.q) : dq;
+            d.dk = d.fk ? (void*)at(w.k) : dk;
+            d.dv = d.fv ? (void*)at(w.v) : dv;
+            d.dg = per_token_decay ? dg : nullptr;
+            d.dg_part = per_token_decay || !dg ? nullptr : at(w.part);
+            d.NC = pl.NC; d.vq = vq; d.vk = vk; d.vv = vv; d.vd = vd;
+            d.vst = Dv % 4 == 0 && (((uintptr_t)state | (uintptr_t)dstate_out) & 15) == 0;
+            const dim3 grid((unsigned)((long long)B * H * pl.NC));
+            const int Dm = Dk > Dv ? Dk : Dv;
+#define CALL(DT)                                                                                                        \
+    if (Dm <= 32) hipLaunchKernelGGL((la_bwd_chunk<DT, 32>), grid, dim3(128), 0, s, a, d);                              \
+    else if (Dm <= 64) hipLaunchKernelGGL((la_bwd_chunk<DT, 64>), grid, dim3(256), 0, s, a, d);                         \
+    else hipLaunchKernelGGL((la_bwd_chunk<DT, 128>), grid, dim3(512), 0, s, a, d)
+            LA_BY_TYPE(dtype, CALL);
 #undef CALL
-        const long long rows = (long long)B * T;
-        if (rows > 0) {
-#define CALL(DT)                                                                                                                   \
-    hipLaunchKernelGGL((la_share<DT>), dim3(1024), dim3(256), 0, s, dqh, dq, rows, Hq, H / Hq, Dk);                                \
-    hipLaunchKernelGGL((la_share<DT>), dim3(1024), dim3(256), 0, s, dkh, dk, rows, Hk, H / Hk, Dk);                                \
-    hipLaunchKernelGGL((la_share<DT>), dim3(1024), dim3(256), 0, s, dvh, dv, rows, Hv, H / Hv, Dv)
+            V2A_CHECK_LAUNCH();
+            const long long rows = (long long)B * T;
+#define CALL(DT)                                                                                                                               \
+    if (d.fq) hipLaunchKernelGGL((la_share<DT>), dim3(1024), dim3(256), 0, s, at(w.q), dq, rows, Hq, H / Hq, Dk);                              \
+    if (d.fk) hipLaunchKernelGGL((la_share<DT>), dim3(1024), dim3(256), 0, s, at(w.k), dk, rows, Hk, H / Hk, Dk);                              \
+    if (d.fv) hipLaunchKernelGGL((la_share<DT>), dim3(1024), dim3(256), 0, s, at(w.v), dv, rows, Hv, H / Hv, Dv)
             LA_BY_TYPE(dtype, CALL);
 #undef CALL
         }
     }
-    if (dg && !per_token_decay) hipLaunchKernelGGL(la_dg_heads, dim3(H), dim3(256), 0, s, dgt, dg, (long long)B * T, H);
+    if (dg && !per_token_decay) hipLaunchKernelGGL(la_dg_heads, dim3(H), dim3(256), 0, s, at(w.part), dg, (long long)B * pl.NC, H);
     V2A_CHECK_LAUNCH();
     return V2A_OK;
 }
