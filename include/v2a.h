@@ -242,7 +242,7 @@ int v2a_linattn_step(const void* q, const void* k, const void* v, const float* g
  * ld_table / ld_pos elements; out, dout, dtable, dpos contiguous; dtype 0 fp32 / 1 bf16 / 2 fp16, sums in fp32, rounded once. */
 int v2a_embed_fwd(const void* ids, int ids64, const void* table, const void* pos, void* out, long long N, long long T, long long V, int D, long long ld_table,
                   long long ld_pos, int dtype, float scale, v2a_stream_t s);
-size_t v2a_embed_bwd_workspace_bytes(long long N, long long V, int D);
+size_t v2a_embed_bwd_workspace_bytes(long long N, long long V, int D, int dtype);
 int v2a_embed_bwd(const void* ids, int ids64, const void* dout, void* dtable, void* dpos, long long N, long long T, long long V, int D, long long pos_rows, int dtype,
                   float scale, void* ws, size_t ws_bytes, v2a_stream_t s);
 /* video-model training (GoalGaussianDiffusion.forward / p_losses, flowdiffusion/flowdiffusion/goal_diffusion.py:674-724):

@@ -1,81 +1,476 @@
-// Token embedding: out[i] = scale * table[id_i] + pos[i mod T], and its gradient: dtable[r] = scale * sum of dout over the tokens r in order,
-// dpos[t] = sum over the sequences.  Ids outside [0, V) are empty: a zero row, no gradient.
+// Token embedding: out[i] = scale * table[id_i] + pos[i mod T], and its gradient: dtable[r] = scale * sum of dout over the tokens r,
+// dpos[t] = sum over the sequences.  Ids outside [0, V) are empty: a zero row, no gradient.  Memory-bound: one read and one write per value.
+//
+// The gradient has no atomics and one order of summation: the tokens are sorted by id (stable, so equal ids stay in token order), a row's
+// tokens are then neighbours, and fixed pieces of the sorted list are summed independently.
+//   launch 1   sort (or the histogram of its first digit) in the first workgroups, dpos and the zero fill of dtable in the others: the
+//              fill and dpos need no order and hide behind the latency-bound sort
+//   (launches  further steps of the sort: two per digit where there are more than EM_SMALL tokens)
+//   next       every piece of the list: rows that lie inside a piece are written, rows that cross a border leave fp32 partial sums
+//   last       rows that cross borders: their partial sums, in piece order
 #include "common.h"
 
 namespace {
 
-template <int DT> __device__ __forceinline__ float em_ld(const void* p, long long i) {
-    if constexpr (DT == 0) return ((const float*)p)[i];
-    else return v2a_h2f<DT == 2>(((const unsigned short*)p)[i]);
-}
-template <int DT> __device__ __forceinline__ void em_st(void* p, long long i, float x) {
-    if constexpr (DT == 0) ((float*)p)[i] = x;
-    else ((unsigned short*)p)[i] = v2a_f2h<DT == 2>(x);
-}
-__device__ __forceinline__ long long em_id(const void* ids, int wide, long long i) { return wide ? ((const long long*)ids)[i] : (long long)((const int*)ids)[i]; }
+constexpr int EM_SORT_T = 1024, EM_WAVES = EM_SORT_T / 64, EM_KPT = 4, EM_SMALL = EM_SORT_T * EM_KPT, EM_BINS = 1024, EM_TILES = 64;
 
-template <int DT>
-__global__ __launch_bounds__(256) void embed_fwd_kernel(const void* ids, int wide, const void* table, const void* pos, void* out, long long N, long long T, long long V, int D,
-                                                        long long ldt, long long ldp, float scale) {
-    for (long long i = blockIdx.x; i < N; i += gridDim.x) {
-        const long long id = em_id(ids, wide, i);
-        for (int c = threadIdx.x; c < D; c += 256) {
-            float y = 0.f;
-            if (id >= 0 && id < V) {
-                y = em_ld<DT>(table, id * ldt + c) * scale;
-                if (pos) y += em_ld<DT>(pos, (i % T) * ldp + c);
+template <int DT> struct EmT { typedef unsigned short T; static constexpr int EPC = 8; };
+template <> struct EmT<0> { typedef float T; static constexpr int EPC = 4; };
+template <int DT> __device__ __forceinline__ float em_f(typename EmT<DT>::T x) {
+    if constexpr (DT == 0) return x;
+    else return v2a_h2f<DT == 2>(x);
+}
+template <int DT> __device__ __forceinline__ typename EmT<DT>::T em_r(float x) {
+    if constexpr (DT == 0) return x;
+    else return v2a_f2h<DT == 2>(x);
+}
+// W values from p[0 .. W): 16 bytes, or one value
+template <int DT, int W> __device__ __forceinline__ void em_ld(const typename EmT<DT>::T* p, float* x) {
+    if constexpr (W == 1) x[0] = em_f<DT>(*p);
+    else if constexpr (DT == 0) {
+        const float4 v = *(const float4*)p;
+        x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+    } else v2a_unpack_h8<DT == 2>(*(const uint4*)p, x);
+}
+template <int DT, int W> __device__ __forceinline__ void em_st(typename EmT<DT>::T* p, const float* x) {
+    if constexpr (W == 1) *p = em_r<DT>(x[0]);
+    else if constexpr (DT == 0) *(float4*)p = make_float4(x[0], x[1], x[2], x[3]);
+    else *(uint4*)p = make_uint4(v2a_pack_h2<DT == 2>(x[0], x[1]), v2a_pack_h2<DT == 2>(x[2], x[3]), v2a_pack_h2<DT == 2>(x[4], x[5]), v2a_pack_h2<DT == 2>(x[6], x[7]));
+}
+// id of token i, or V for an empty place
+__device__ __forceinline__ unsigned em_key(const void* ids, int wide, unsigned i, unsigned V) {
+    if (wide) {
+        const long long id = ((const long long*)ids)[i];
+        return id >= 0 && id < (long long)V ? (unsigned)id : V;
+    }
+    const int id = ((const int*)ids)[i];
+    return id >= 0 && (unsigned)id < V ? (unsigned)id : V;
+}
+
+struct EmShape {
+    unsigned N, T, V;
+    int D, lpr, ncol;      // lanes that share a row (power of two, at most 64), column blocks of lpr pieces
+};
+
+// A group of lpr lanes takes a row; each lane has RPT rows under way at once
+template <int DT, int W>
+__global__ __launch_bounds__(256) void embed_fwd_kernel(const void* ids, int wide, const void* table_, const void* pos_, void* out_, EmShape e, long long ldt,
+                                                        long long ldp, float scale) {
+    typedef typename EmT<DT>::T E;
+    constexpr int RPT = 4;
+    const E *table = (const E*)table_, *pos = (const E*)pos_;
+    E* out = (E*)out_;
+    const unsigned l = threadIdx.x & (e.lpr - 1), groups = gridDim.x * 256 / e.lpr, gid = (blockIdx.x * 256 + threadIdx.x) / e.lpr;
+    for (unsigned long long r0 = gid; r0 < e.N; r0 += (unsigned long long)groups * RPT) {
+        unsigned key[RPT];
+#pragma unroll
+        for (int j = 0; j < RPT; ++j) {
+            const unsigned long long r = r0 + (unsigned long long)j * groups;
+            key[j] = r < e.N ? em_key(ids, wide, (unsigned)r, e.V) : e.V;
+        }
+        for (int c = l * W; c < e.D; c += e.lpr * W) {
+            float x[RPT][W];
+#pragma unroll
+            for (int j = 0; j < RPT; ++j)
+                if (key[j] < e.V) em_ld<DT, W>(table + key[j] * ldt + c, x[j]);
+#pragma unroll
+            for (int j = 0; j < RPT; ++j) {
+                const unsigned long long r = r0 + (unsigned long long)j * groups;
+                if (r >= e.N) break;
+                float p[W];
+#pragma unroll
+                for (int w = 0; w < W; ++w) {
+                    p[w] = 0.f;
+                    x[j][w] = key[j] < e.V ? x[j][w] * scale : 0.f;
+                }
+                if (pos && key[j] < e.V) em_ld<DT, W>(pos + ((unsigned)r % e.T) * ldp + c, p);
+                if (pos)
+#pragma unroll
+                    for (int w = 0; w < W; ++w) x[j][w] += p[w];
+                em_st<DT, W>(out + r * e.D + c, x[j]);
             }
-            em_st<DT>(out, i * D + c, y);
         }
     }
 }
 
-template <int DT>
-__global__ __launch_bounds__(256) void embed_bwd_simple(const void* ids, int wide, const void* dout, void* dtable, long long N, long long V, int D,
-                                                        float scale) {
-    __shared__ int hit[256];
-    for (long long r = blockIdx.x; r < V; r += gridDim.x)
-    for (int c0 = 0; c0 < D; c0 += 256) {
-        const int c = c0 + threadIdx.x;
-        float s = 0.f;
-        for (long long i0 = 0; i0 < N; i0 += 256) {
-            const long long i = i0 + threadIdx.x;
-            const int m = i < N && em_id(ids, wide, i) == r;
-            if (!__syncthreads_or(m)) continue;
-            hit[threadIdx.x] = m;
-            __syncthreads();
-            for (int j = 0; j < 256; ++j)
-                if (hit[j] && c < D) s += em_ld<DT>(dout, (i0 + j) * D + c);
-            __syncthreads();
+// ---------------------------------------------------------------------------------------------------------------------- sort
+struct EmSort {
+    const void* ids;
+    int wide, bits, passes;                 // digits of `bits` bits, low first
+    unsigned N, V, tile, ntiles;            // tokens per workgroup of the many-workgroup form
+    unsigned *key, *pos, *key2, *pos2;      // ping and pong
+    unsigned* hist;                         // [ntiles][2^bits]
+};
+
+// Stable rank of each of this wave's 64 * EM_KPT keys (key j of lane l is number 64 j + l) among the wave's equal digits, which also counts
+// them: lanes with the digit's bits all equal find each other by ballots.
+__device__ __forceinline__ void em_wave_rank(const unsigned (&dig)[EM_KPT], const bool (&on)[EM_KPT], int bits, unsigned short* count, int lane, unsigned (&rank)[EM_KPT]) {
+#pragma unroll
+    for (int j = 0; j < EM_KPT; ++j) {
+        unsigned long long same = __ballot(on[j]);
+        for (int b = 0; b < bits; ++b) {
+            const unsigned long long m = __ballot((dig[j] >> b) & 1);
+            same &= (dig[j] >> b) & 1 ? m : ~m;
         }
-        if (c < D) em_st<DT>(dtable, r * D + c, s * scale);
+        const unsigned below = __popcll(same & ((1ull << lane) - 1));
+        const unsigned start = on[j] ? count[dig[j]] : 0u;
+        rank[j] = start + below;
+        __builtin_amdgcn_wave_barrier();
+        if (on[j] && below == 0) count[dig[j]] = (unsigned short)(start + __popcll(same));
+        __builtin_amdgcn_wave_barrier();
     }
 }
 
-template <int DT>
-__global__ __launch_bounds__(256) void embed_dpos_kernel(const void* ids, int wide, const void* dout, void* dpos, long long Bn, long long T, long long V, int D, long long P) {
-    for (long long t = blockIdx.x; t < P; t += gridDim.x)
-    for (int c = threadIdx.x; c < D; c += 256) {
-        float s = 0.f;
-        if (t < T)
-            for (long long b = 0; b < Bn; ++b) {
-                const long long id = em_id(ids, wide, b * T + t);
-                if (id >= 0 && id < V) s += em_ld<DT>(dout, (b * T + t) * D + c);
+// exclusive scan over the workgroup's 1024 threads
+__device__ __forceinline__ unsigned em_scan(unsigned v, unsigned* tmp) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    unsigned x = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const unsigned y = __shfl_up(x, o, 64);
+        if (lane >= o) x += y;
+    }
+    if (lane == 63) tmp[w] = x;
+    __syncthreads();
+    unsigned before = 0;
+    for (int i = 0; i < w; ++i) before += tmp[i];
+    __syncthreads();
+    return before + x - v;
+}
+
+struct EmSortLds {
+    unsigned short count[EM_WAVES][EM_BINS];
+    unsigned base[EM_BINS], tmp[EM_WAVES];
+};
+
+// up to EM_SMALL tokens: one workgroup, all digits, through LDS
+__device__ void em_sort_small(const EmSort& s, EmSortLds& L, unsigned (*xch)[EM_SMALL]) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, bins = 1 << s.bits;
+    unsigned key[EM_KPT], pos[EM_KPT];
+    bool on[EM_KPT];
+#pragma unroll
+    for (int j = 0; j < EM_KPT; ++j) {
+        const unsigned i = w * 64 * EM_KPT + j * 64 + lane;
+        on[j] = i < s.N;
+        pos[j] = i;
+        key[j] = on[j] ? em_key(s.ids, s.wide, i, s.V) : 0u;
+    }
+    for (int p = 0; p < s.passes; ++p) {
+        for (int i = threadIdx.x; i < EM_WAVES * EM_BINS / 2; i += EM_SORT_T) ((unsigned*)L.count)[i] = 0u;
+        __syncthreads();
+        unsigned dig[EM_KPT], rank[EM_KPT];
+#pragma unroll
+        for (int j = 0; j < EM_KPT; ++j) dig[j] = (key[j] >> (p * s.bits)) & (bins - 1);
+        em_wave_rank(dig, on, s.bits, L.count[w], lane, rank);
+        __syncthreads();
+        unsigned total = 0;
+        if (threadIdx.x < bins)
+            for (int i = 0; i < EM_WAVES; ++i) {
+                const unsigned n = L.count[i][threadIdx.x];
+                L.count[i][threadIdx.x] = (unsigned short)total;
+                total += n;
             }
-        em_st<DT>(dpos, t * D + c, s);
+        L.base[threadIdx.x] = em_scan(total, L.tmp);
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < EM_KPT; ++j)
+            if (on[j]) {
+                const unsigned d = L.base[dig[j]] + L.count[w][dig[j]] + rank[j];
+                xch[0][d] = key[j];
+                xch[1][d] = pos[j];
+            }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < EM_KPT; ++j) {
+            const unsigned i = w * 64 * EM_KPT + j * 64 + lane;
+            if (on[j]) {
+                key[j] = xch[0][i];
+                pos[j] = xch[1][i];
+            }
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int j = 0; j < EM_KPT; ++j) {
+        const unsigned i = w * 64 * EM_KPT + j * 64 + lane;
+        if (on[j]) {
+            s.key[i] = key[j];
+            s.pos[i] = pos[j];
+        }
     }
 }
 
-#define EM_BY_TYPE(dtype, CALL)        \
-    do {                               \
-        if ((dtype) == 0) { CALL(0); } \
-        else if ((dtype) == 1) { CALL(1); } \
-        else { CALL(2); }              \
-    } while (0)
+// how many tokens of workgroup `t`'s tile have each digit of pass p
+__device__ void em_hist(const EmSort& s, int p, unsigned t, unsigned* count) {
+    const int bins = 1 << s.bits;
+    for (int i = threadIdx.x; i < bins; i += EM_SORT_T) count[i] = 0u;
+    __syncthreads();
+    const unsigned a = t * s.tile, b = s.N - a < s.tile ? s.N : a + s.tile;
+    for (unsigned i = a + threadIdx.x; i < b; i += EM_SORT_T) {
+        const unsigned k = p == 0 ? em_key(s.ids, s.wide, i, s.V) : s.key[i];
+        atomicAdd(&count[(k >> (p * s.bits)) & (bins - 1)], 1u);
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < bins; i += EM_SORT_T) s.hist[(size_t)t * bins + i] = count[i];
+}
+__global__ __launch_bounds__(EM_SORT_T) void embed_hist_kernel(EmSort s, int p) {
+    __shared__ unsigned count[EM_BINS];
+    em_hist(s, p, blockIdx.x, count);
+}
+// the tokens of a tile to their places of pass p; a workgroup adds up the at most EM_TILES histograms itself
+__global__ __launch_bounds__(EM_SORT_T) void embed_scatter_kernel(EmSort s, int p) {
+    __shared__ EmSortLds L;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, bins = 1 << s.bits;
+    unsigned before = 0, total = 0;
+    if (threadIdx.x < bins)
+        for (unsigned t = 0; t < s.ntiles; ++t) {
+            const unsigned n = s.hist[(size_t)t * bins + threadIdx.x];
+            if (t < blockIdx.x) before += n;
+            total += n;
+        }
+    const unsigned start = em_scan(total, L.tmp) + before;
+    L.base[threadIdx.x] = start;
+    const unsigned a = blockIdx.x * s.tile, end = s.N - a < s.tile ? s.N : a + s.tile;
+    for (unsigned a0 = a; a0 < end; a0 += EM_SMALL) {
+        for (int i = threadIdx.x; i < EM_WAVES * EM_BINS / 2; i += EM_SORT_T) ((unsigned*)L.count)[i] = 0u;
+        unsigned key[EM_KPT], pos[EM_KPT], dig[EM_KPT], rank[EM_KPT];
+        bool on[EM_KPT];
+#pragma unroll
+        for (int j = 0; j < EM_KPT; ++j) {
+            const unsigned i = a0 + w * 64 * EM_KPT + j * 64 + lane;
+            on[j] = i < end;
+            key[j] = !on[j] ? 0u : p == 0 ? em_key(s.ids, s.wide, i, s.V) : s.key[i];
+            pos[j] = !on[j] ? 0u : p == 0 ? i : s.pos[i];
+            dig[j] = (key[j] >> (p * s.bits)) & (bins - 1);
+        }
+        __syncthreads();
+        em_wave_rank(dig, on, s.bits, L.count[w], lane, rank);
+        __syncthreads();
+        unsigned n = 0;
+        if (threadIdx.x < bins)
+            for (int i = 0; i < EM_WAVES; ++i) {
+                const unsigned c = L.count[i][threadIdx.x];
+                L.count[i][threadIdx.x] = (unsigned short)n;
+                n += c;
+            }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < EM_KPT; ++j)
+            if (on[j]) {
+                const unsigned d = L.base[dig[j]] + L.count[w][dig[j]] + rank[j];
+                s.key2[d] = key[j];
+                s.pos2[d] = pos[j];
+            }
+        __syncthreads();
+        if (threadIdx.x < bins) L.base[threadIdx.x] += n;
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------- gradient
+struct EmGrad {
+    const void* dout;
+    void *dtable, *dpos;
+    unsigned P, nsort, nfill;      // rows of dpos; workgroups of launch 1 that sort / fill (those between the two compute dpos)
+    float scale;
+};
+
+// Launch 1.  dpos: one workgroup per (position, column block); wave w adds sequences w, w + 16, .., the waves' sums are added in order.
+template <int DT, int W>
+__global__ __launch_bounds__(EM_SORT_T) void embed_first_kernel(EmSort s, EmGrad g, EmShape e) {
+    typedef typename EmT<DT>::T E;
+    __shared__ union {
+        struct { EmSortLds l; unsigned xch[2][EM_SMALL]; } sort;
+        unsigned count[EM_BINS];
+        float part[EM_WAVES][64 * W];
+    } sm;
+    if (blockIdx.x < g.nsort) {
+        if (s.N <= (unsigned)EM_SMALL) em_sort_small(s, sm.sort.l, sm.sort.xch);
+        else em_hist(s, 0, blockIdx.x, sm.count);
+        return;
+    }
+    const unsigned blk = blockIdx.x - g.nsort, ndpos = gridDim.x - g.nsort - g.nfill;
+    if (blk >= ndpos) {
+        const size_t n = (size_t)e.V * e.D;
+        E* q = (E*)g.dtable;
+        const size_t step = (size_t)g.nfill * EM_SORT_T, at = (size_t)(blk - ndpos) * EM_SORT_T + threadIdx.x;
+        if (((uintptr_t)q & 15) == 0) {
+            const size_t nv = n / EmT<DT>::EPC;
+            for (size_t i = at; i < nv; i += step) ((uint4*)q)[i] = make_uint4(0u, 0u, 0u, 0u);
+            for (size_t i = nv * EmT<DT>::EPC + at; i < n; i += step) q[i] = 0;
+        } else
+            for (size_t i = at; i < n; i += step) q[i] = 0;
+        return;
+    }
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const unsigned nc = (e.D + 64 * W - 1) / (64 * W), Bn = e.N / e.T;
+    for (unsigned long long u = blk; u < (unsigned long long)g.P * nc; u += ndpos) {
+        const unsigned t = (unsigned)(u / nc);
+        const int c = (int)(u % nc) * 64 * W + lane * W;
+        float acc[W];
+#pragma unroll
+        for (int i = 0; i < W; ++i) acc[i] = 0.f;
+        if (t < e.T && c < e.D)
+#pragma unroll 4
+            for (unsigned b = w; b < Bn; b += EM_WAVES) {
+                const unsigned r = b * e.T + t;
+                if (em_key(s.ids, s.wide, r, e.V) < e.V) {
+                    float x[W];
+                    em_ld<DT, W>((const E*)g.dout + (size_t)r * e.D + c, x);
+#pragma unroll
+                    for (int i = 0; i < W; ++i) acc[i] += x[i];
+                }
+            }
+#pragma unroll
+        for (int i = 0; i < W; ++i) sm.part[w][i * 64 + lane] = acc[i];
+        __syncthreads();
+        if (w == 0 && c < e.D) {
+            for (int j = 1; j < EM_WAVES; ++j)
+#pragma unroll
+                for (int i = 0; i < W; ++i) acc[i] += sm.part[j][i * 64 + lane];
+            em_st<DT, W>((E*)g.dpos + (size_t)t * e.D + c, acc);
+        }
+        __syncthreads();
+    }
+}
+
+// Pieces of `ts` neighbours of the sorted list, one per group of lpr lanes.  part [pieces][2][Dp]: 0 = a row that began before the piece
+// (through to its end or past the piece), 1 = a row that begins inside and goes on behind it.
+template <int DT, int W>
+__global__ __launch_bounds__(256) void embed_pieces_kernel(const unsigned* key, const unsigned* pos, EmGrad g, EmShape e, float* part, int Dp, unsigned ts) {
+    typedef typename EmT<DT>::T E;
+    constexpr int AHEAD = 8;
+    const unsigned l = threadIdx.x & (e.lpr - 1);
+    const unsigned long long gid = ((unsigned long long)blockIdx.x * 256 + threadIdx.x) / e.lpr;
+    const unsigned long long t = gid / e.ncol, a64 = t * ts;
+    if (a64 >= e.N) return;
+    const int c = ((int)(gid % e.ncol) * e.lpr + l) * W;
+    if (c >= e.D) return;
+    const unsigned a = (unsigned)a64, b = e.N - a < ts ? e.N : a + ts;
+    unsigned cur = key[a];
+    bool before = a > 0 && key[a - 1] == cur;
+    float acc[W];
+#pragma unroll
+    for (int i = 0; i < W; ++i) acc[i] = 0.f;
+    auto partial = [&](int which) {
+        float* q = part + (t * 2 + which) * Dp + c;
+        if constexpr (W == 1) q[0] = acc[0];
+        else
+#pragma unroll
+            for (int i = 0; i < W; i += 4) *(float4*)(q + i) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
+    };
+    auto whole = [&]() {
+        float x[W];
+#pragma unroll
+        for (int i = 0; i < W; ++i) x[i] = acc[i] * g.scale;
+        em_st<DT, W>((E*)g.dtable + (size_t)cur * e.D + c, x);
+    };
+    for (unsigned i0 = a; i0 < b && cur < e.V; i0 += AHEAD) {
+        unsigned k[AHEAD];
+        float x[AHEAD][W];
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+            k[j] = i0 + j < b ? key[i0 + j] : e.V;
+            if (k[j] < e.V) em_ld<DT, W>((const E*)g.dout + (size_t)pos[i0 + j] * e.D + c, x[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+            if (i0 + j >= b) break;
+            if (k[j] != cur) {
+                if (before) partial(0);
+                else if (cur < e.V) whole();
+                before = false;
+                cur = k[j];
+#pragma unroll
+                for (int i = 0; i < W; ++i) acc[i] = 0.f;
+            }
+            if (k[j] < e.V)
+#pragma unroll
+                for (int i = 0; i < W; ++i) acc[i] += x[j][i];
+        }
+    }
+    if (cur >= e.V) return;
+    if (before) partial(0);
+    else if (b < e.N && key[b] == cur) partial(1);
+    else whole();
+}
+
+// Rows that cross pieces: the piece in which one begins adds its part 1 and the parts 0 of the pieces behind it; wave w takes pieces w, w + 8, ..
+template <int DT>
+__global__ __launch_bounds__(512) void embed_join_kernel(const unsigned* key, EmGrad g, EmShape e, const float* part, int Dp, unsigned ts) {
+    typedef typename EmT<DT>::T E;
+    __shared__ float sum[8][256];
+    const unsigned t = blockIdx.x, a = t * ts;
+    const unsigned long long b = (unsigned long long)a + ts;
+    if (b >= e.N) return;
+    const unsigned cur = key[b - 1];
+    if (cur >= e.V || key[b] != cur || (key[a] == cur && a > 0 && key[a - 1] == cur)) return;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const unsigned np = (e.N - 1) / ts + 1;
+    for (int c0 = 0; c0 < e.D; c0 += 256) {
+        const int c = c0 + lane * 4;
+        float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (c < e.D) {
+            if (w == 0) s = *(const float4*)(part + ((size_t)t * 2 + 1) * Dp + c);
+#pragma unroll 4
+            for (unsigned i = t + 1 + w; i < np; i += 8) {
+                if (key[(size_t)i * ts] != cur) break;
+                const float4 x = *(const float4*)(part + (size_t)i * 2 * Dp + c);
+                s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
+            }
+            *(float4*)&sum[w][lane * 4] = s;
+        }
+        __syncthreads();
+        for (int d = threadIdx.x; d < 256 && c0 + d < e.D; d += 512) {
+            float y = sum[0][d];
+#pragma unroll
+            for (int i = 1; i < 8; ++i) y += sum[i][d];
+            ((E*)g.dtable)[(size_t)cur * e.D + c0 + d] = em_r<DT>(y * g.scale);
+        }
+        __syncthreads();
+    }
+}
 
 bool em_dims(long long N, long long T, long long V, int D, int dtype) {
     return N >= 0 && N < (1ll << 31) && T > 0 && N % T == 0 && V > 0 && V < (1ll << 31) - 1 && D > 0 && dtype >= 0 && dtype <= 2;
 }
+EmShape em_shape(long long N, long long T, long long V, int D, int W) {
+    EmShape e;
+    e.N = (unsigned)N; e.T = (unsigned)(T < (1ll << 31) ? T : (1ll << 31)); e.V = (unsigned)V; e.D = D;
+    const int pieces = cdiv(D, W);
+    e.lpr = 1;
+    while (e.lpr < pieces && e.lpr < 64) e.lpr *= 2;
+    e.ncol = cdiv(pieces, e.lpr);
+    return e;
+}
+// pieces of 8 .. 64 tokens: long ones leave fewer partial sums, but a few thousand lane groups are needed to keep the memory busy
+unsigned em_piece(long long N, int D, int dtype) {
+    const long long ncol = cdiv(D, dtype == 0 ? 256 : 512);
+    unsigned ts = 8;
+    while (ts < 64 && N * ncol / (ts * 2) >= 4096) ts *= 2;
+    return ts;
+}
+struct EmWs { size_t key, pos, key2, pos2, hist, part, total; int Dp; unsigned ts; };
+EmWs em_ws(long long N, int D, int dtype) {
+    EmWs w;
+    size_t at = 0;
+    auto take = [&](size_t n) { const size_t o = at; at += (n + 255) & ~(size_t)255; return o; };
+    w.ts = em_piece(N, D, dtype);
+    w.Dp = (D + 7) & ~7;
+    w.key = take(N * 4); w.pos = take(N * 4);
+    w.key2 = take(N > EM_SMALL ? N * 4 : 0); w.pos2 = take(N > EM_SMALL ? N * 4 : 0);
+    w.hist = take(N > EM_SMALL ? (size_t)EM_TILES * EM_BINS * 4 : 0);
+    w.part = take((size_t)cdiv(N, w.ts) * 2 * w.Dp * 4);
+    w.total = at;
+    return w;
+}
+bool em_al(const void* p, long long ld, int dtype) { return ((uintptr_t)p & 15) == 0 && ld * (dtype == 0 ? 4 : 2) % 16 == 0; }
+
+#define EM_BY_TYPE(dtype, vec, CALL)                          \
+    do {                                                      \
+        if ((dtype) == 0) { if (vec) { CALL(0, 4); } else { CALL(0, 1); } } \
+        else if ((dtype) == 1) { if (vec) { CALL(1, 8); } else { CALL(1, 1); } } \
+        else { if (vec) { CALL(2, 8); } else { CALL(2, 1); } } \
+    } while (0)
 
 }  // namespace
 
@@ -86,25 +481,78 @@ int v2a_embed_fwd(const void* ids, int ids64, const void* table, const void* pos
     if (!em_dims(N, T, V, D, dtype) || ld_table < 0 || ld_pos < 0) return V2A_ERR_ARG;
     if (N == 0) return V2A_OK;
     if (!ids || !table || !out) return V2A_ERR_ARG;
-#define CALL(DT) hipLaunchKernelGGL((embed_fwd_kernel<DT>), dim3((unsigned)(N < 65536 ? N : 65536)), dim3(256), 0, s, ids, ids64, table, pos, out, N, T, V, D, ld_table, ld_pos, scale)
-    EM_BY_TYPE(dtype, CALL);
+    const bool vec = em_al(table, V > 1 ? ld_table : 0, dtype) && em_al(out, D, dtype) && (!pos || em_al(pos, T > 1 ? ld_pos : 0, dtype));
+    const EmShape e = em_shape(N, T, V, D, vec ? (dtype == 0 ? 4 : 8) : 1);
+    long long blocks = (N * e.lpr + 1023) / 1024;
+    if (blocks > 8192) blocks = 8192;
+    if (blocks < 256) blocks = (N * e.lpr + 255) / 256;      // few rows: one each
+#define CALL(DT, W) hipLaunchKernelGGL((embed_fwd_kernel<DT, W>), dim3((unsigned)blocks), dim3(256), 0, s, ids, ids64, table, pos, out, e, ld_table, ld_pos, scale)
+    EM_BY_TYPE(dtype, vec, CALL);
 #undef CALL
     V2A_CHECK_LAUNCH();
     return V2A_OK;
 }
 
-size_t v2a_embed_bwd_workspace_bytes(long long N, long long V, int D) { return 0; }
+size_t v2a_embed_bwd_workspace_bytes(long long N, long long V, int D, int dtype) {
+    if (!em_dims(N, 1, V, D, dtype) || N == 0) return 0;
+    return em_ws(N, D, dtype).total;
+}
 
 int v2a_embed_bwd(const void* ids, int ids64, const void* dout, void* dtable, void* dpos, long long N, long long T, long long V, int D, long long pos_rows, int dtype,
                   float scale, void* ws, size_t ws_bytes, hipStream_t s) {
-    if (!em_dims(N, T, V, D, dtype) || !dtable || (dpos && pos_rows < T)) return V2A_ERR_ARG;
+    if (!em_dims(N, T, V, D, dtype) || !dtable || (dpos && (pos_rows < T || pos_rows >= (1ll << 31)) && N > 0)) return V2A_ERR_ARG;
     if (N > 0 && (!ids || !dout)) return V2A_ERR_ARG;
-#define CALL(DT)                                                                                                                                  \
-    hipLaunchKernelGGL((embed_bwd_simple<DT>), dim3((unsigned)(V < 65536 ? V : 65536)), dim3(256), 0, s, ids, ids64, dout, dtable, N, V, D, scale);                          \
-    if (dpos && pos_rows) hipLaunchKernelGGL((embed_dpos_kernel<DT>), dim3((unsigned)(pos_rows < 65536 ? pos_rows : 65536)), dim3(256), 0, s, ids, ids64, dout, dpos, N / T, T, V, D, pos_rows)
-    EM_BY_TYPE(dtype, CALL);
+    const EmWs w = em_ws(N, D, dtype);
+    if (N > 0 && (ws_bytes < w.total || !ws)) return V2A_ERR_WORKSPACE;
+    char* base = (char*)ws;
+    const bool vec = em_al(dout, D, dtype) && em_al(dtable, D, dtype) && em_al(dpos, D, dtype);
+    const EmShape e = em_shape(N, T, V, D, vec ? (dtype == 0 ? 4 : 8) : 1);
+    EmSort q{};
+    q.ids = ids; q.wide = ids64; q.N = (unsigned)N; q.V = (unsigned)V;
+    int bits = 1;
+    while ((V >> bits) > 0) ++bits;               // keys 0 .. V
+    q.passes = cdiv(bits, 10);
+    q.bits = cdiv(bits, q.passes);
+    q.key = (unsigned*)(base + w.key); q.pos = (unsigned*)(base + w.pos);
+    q.key2 = (unsigned*)(base + w.key2); q.pos2 = (unsigned*)(base + w.pos2);
+    q.hist = (unsigned*)(base + w.hist);
+    q.tile = EM_SMALL;
+    while (cdiv(N, q.tile) > EM_TILES) q.tile *= 2;
+    q.ntiles = cdiv(N, q.tile);
+    EmGrad g{};
+    g.dout = dout; g.dtable = dtable; g.dpos = dpos; g.scale = scale;
+    g.P = dpos ? (unsigned)pos_rows : 0u;
+    g.nsort = N == 0 ? 0 : N <= EM_SMALL ? 1 : q.ntiles;
+    const int W = vec ? (dtype == 0 ? 4 : 8) : 1;
+    const long long units = (long long)g.P * cdiv(D, 64 * W), ndpos = units < 4096 ? units : 4096;
+    const long long fill = ((long long)V * D * (dtype == 0 ? 4 : 2) + 65535) / 65536;
+    g.nfill = (unsigned)(fill < 1024 ? fill : 1024);
+#define CALL(DT, W) hipLaunchKernelGGL((embed_first_kernel<DT, W>), dim3(g.nsort + (unsigned)ndpos + g.nfill), dim3(EM_SORT_T), 0, s, q, g, e)
+    EM_BY_TYPE(dtype, vec, CALL);
 #undef CALL
     V2A_CHECK_LAUNCH();
+    if (N == 0) return V2A_OK;
+    if (N > EM_SMALL) {
+        for (int p = 0; p < q.passes; ++p) {
+            if (p > 0) hipLaunchKernelGGL(embed_hist_kernel, dim3(q.ntiles), dim3(EM_SORT_T), 0, s, q, p);
+            hipLaunchKernelGGL(embed_scatter_kernel, dim3(q.ntiles), dim3(EM_SORT_T), 0, s, q, p);
+            unsigned* t = q.key; q.key = q.key2; q.key2 = t;
+            t = q.pos; q.pos = q.pos2; q.pos2 = t;
+        }
+        V2A_CHECK_LAUNCH();
+    }
+    const unsigned pieces = (unsigned)cdiv(N, w.ts);
+    const long long lanes = (long long)pieces * e.ncol * e.lpr;
+#define CALL(DT, W) hipLaunchKernelGGL((embed_pieces_kernel<DT, W>), dim3((unsigned)((lanes + 255) / 256)), dim3(256), 0, s, q.key, q.pos, g, e, (float*)(base + w.part), w.Dp, w.ts)
+    EM_BY_TYPE(dtype, vec, CALL);
+#undef CALL
+    V2A_CHECK_LAUNCH();
+    if (pieces > 1) {
+#define CALL(DT, W) hipLaunchKernelGGL((embed_join_kernel<DT>), dim3(pieces - 1), dim3(512), 0, s, q.key, g, e, (const float*)(base + w.part), w.Dp, w.ts)
+        EM_BY_TYPE(dtype, false, CALL);
+#undef CALL
+        V2A_CHECK_LAUNCH();
+    }
     return V2A_OK;
 }
 

@@ -889,58 +889,92 @@ __global__ __launch_bounds__(256) void la_dg_heads(const float* dgt, float* dg, 
 }
 
 // ---------------------------------------------------------------------------------------------------------------------- single tokens
-// One workgroup per (row, head).  Rows that name the same slot are taken by the first of them, in row order, as successive tokens.
-template <int DT>
+// One workgroup per (row, head): reads and writes the Dk x Dv state once, which is all of the traffic that counts.  lv lanes of 16 bytes cover
+// a state row, the other lanes take further rows, eight of them under way per lane.  Rows that name the same slot are taken by the first of
+// them, in row order, as successive tokens.
+template <int DT, int W>
 __global__ __launch_bounds__(256) void la_step_kernel(const void* q_, const void* k_, const void* v_, const float* g, float* state, const int* slots,
                                                       void* out_, long long qb_, long long qh_, long long kb_, long long kh_, long long vb_, long long vh_,
-                                                      long long gb_, long long gh_, int B, int N, int H, int Hq, int Hk, int Hv, int Dk, int Dv, float scale) {
+                                                      long long gb_, long long gh_, int B, int N, int H, int Hq, int Hk, int Hv, int Dk, int Dv, int lv, float scale) {
     typedef typename LaT<DT>::T E;
+    constexpr int AHEAD = 8;
     __shared__ float qs[LA_DMAX], ks[LA_DMAX];
-    __shared__ float red[256];
+    __shared__ float red[4][LA_DMAX];
+    __shared__ int nexts[256];
     const int x = threadIdx.x, h = blockIdx.x % H;
-    int b = blockIdx.x / H;
-    int slot = b;
+    int b = blockIdx.x / H, slot = b;
     E* out = (E*)out_;
+    bool more = false;
     if (slots) {
         slot = slots[b];
+        int low = 0, high = 0;
+        for (int j = x; j < B; j += 256) {
+            const bool same = slots[j] == slot;
+            low |= same && j < b;
+            high |= same && j > b;
+        }
         if (slot < 0 || slot >= N) {
-            for (int c = x; c < Dv; c += 256) out[((long long)b * H + h) * Dv + c] = LaT<DT>::st(0.f);
+            if (x < Dv) out[((long long)b * H + h) * Dv + x] = LaT<DT>::st(0.f);
             return;
         }
-        int low = 0;
-        for (int j = x; j < b; j += 256) low |= slots[j] == slot;
         if (__syncthreads_or(low)) return;
+        more = __syncthreads_or(high);
     }
     float* S = state + ((long long)slot * H + h) * Dk * Dv;
-    while (b < B) {
+    const int c = (x & (lv - 1)) * W, r0 = x / lv, rg = 256 / lv, lane = x & 63;
+    for (;;) {
         const E* q = (const E*)q_ + b * qb_ + (h / (H / Hq)) * qh_;
         const E* k = (const E*)k_ + b * kb_ + (h / (H / Hk)) * kh_;
         const E* v = (const E*)v_ + b * vb_ + (h / (H / Hv)) * vh_;
-        const float w = expf(la_clampg(g[b * gb_ + h * gh_]));
-        __syncthreads();
+        const float w = __builtin_amdgcn_exp2f(la_clampg(g[b * gb_ + h * gh_]) * 1.44269504088896340736f);
         if (x < Dk) { qs[x] = LaT<DT>::ld(q[x]) * scale; ks[x] = LaT<DT>::ld(k[x]); }
+        float vv[W], o[W];
+#pragma unroll
+        for (int i = 0; i < W; ++i) { vv[i] = c + i < Dv ? LaT<DT>::ld(v[c + i]) : 0.f; o[i] = 0.f; }
         __syncthreads();
-        const int c = x & 127, r0 = x >> 7;
-        float o = 0.f;
-        if (c < Dv) {
-            const float vv = LaT<DT>::ld(v[c]);
-            for (int r = r0; r < Dk; r += 2) {
-                const float y = S[(long long)r * Dv + c] * w + ks[r] * vv;
-                S[(long long)r * Dv + c] = y;
-                o += qs[r] * y;
+        for (int r1 = r0; r1 < Dk; r1 += AHEAD * rg) {
+            float y[AHEAD][W];
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j) {
+                const int r = r1 + j * rg;
+                if (r < Dk && c < Dv) {
+                    if constexpr (W == 4) *(f32x4*)y[j] = *(const f32x4*)(S + r * Dv + c);
+                    else y[j][0] = S[r * Dv + c];
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j) {
+                const int r = r1 + j * rg;
+                if (r < Dk && c < Dv) {
+                    const float kr = ks[r], qr = qs[r];
+#pragma unroll
+                    for (int i = 0; i < W; ++i) {
+                        y[j][i] = y[j][i] * w + kr * vv[i];
+                        o[i] += qr * y[j][i];
+                    }
+                    if constexpr (W == 4) *(f32x4*)(S + r * Dv + c) = *(const f32x4*)y[j];
+                    else S[r * Dv + c] = y[j][0];
+                }
             }
         }
-        red[x] = o;
+#pragma unroll
+        for (int i = 0; i < W; ++i)
+            for (int m = lv; m < 64; m *= 2) o[i] += __shfl_xor(o[i], m, 64);
+        if (W == 4) {
+            if (lane < lv && c < Dv) *(f32x4*)&red[x >> 6][c] = f32x4{o[0], o[W > 1 ? 1 : 0], o[W > 2 ? 2 : 0], o[W > 3 ? 3 : 0]};
+        } else if (lv >= 64) {              // one value a lane, 128 lanes a row: waves 0 and 2 hold columns 0 .. 63, 1 and 3 the others
+            if (c < Dv) red[(x >> 6) & 2][c] = o[0], red[((x >> 6) & 2) + 1][c] = 0.f;
+        } else if (lane < lv && c < Dv) red[x >> 6][c] = o[0];
         __syncthreads();
-        if (x < Dv) out[((long long)b * H + h) * Dv + x] = LaT<DT>::st(red[x] + red[x + 128]);
-        if (!slots) return;
+        if (x < Dv) out[((long long)b * H + h) * Dv + x] = LaT<DT>::st((red[0][x] + red[1][x]) + (red[2][x] + red[3][x]));
+        if (!more) return;
         int next = 0x7fffffff;
         for (int j = b + 1 + x; j < B; j += 256)
             if (slots[j] == slot) { next = j; break; }
-        if (!__syncthreads_or(next != 0x7fffffff)) return;
-        ((int*)red)[x] = next;
+        nexts[x] = next;
         __syncthreads();
-        for (int j = 0; j < 256; ++j) next = min(next, ((int*)red)[j]);
+        for (int j = 0; j < 256; ++j) next = min(next, nexts[j]);
+        if (next == 0x7fffffff) return;
         b = next;
         __syncthreads();
     }
@@ -1160,11 +1194,18 @@ int v2a_linattn_step(const void* q, const void* k, const void* v, const float* g
     if (B == 0) return V2A_OK;
     if (!q || !k || !v || !g || !state || !out) return V2A_ERR_ARG;
     const int64_t* t = strides;
-#define CALL(DT)                                                                                                                                        \
-    hipLaunchKernelGGL((la_step_kernel<DT>), dim3(B * H), dim3(256), 0, s, q, k, v, g, state, slots, out, (long long)t[0], (long long)t[1],              \
-                       (long long)t[2], (long long)t[3], (long long)t[4], (long long)t[5], (long long)t[6], (long long)t[7], B, N, H, Hq, Hk, Hv, Dk, Dv, scale)
+    const bool vec = Dv % 4 == 0 && ((uintptr_t)state & 15) == 0;
+    int lv = 1;
+    while (lv * (vec ? 4 : 1) < Dv) lv *= 2;
+#define STEP(DT, W)                                                                                                                                     \
+    hipLaunchKernelGGL((la_step_kernel<DT, W>), dim3(B * H), dim3(256), 0, s, q, k, v, g, state, slots, out, (long long)t[0], (long long)t[1],           \
+                       (long long)t[2], (long long)t[3], (long long)t[4], (long long)t[5], (long long)t[6], (long long)t[7], B, N, H, Hq, Hk, Hv, Dk, Dv, lv, scale)
+#define CALL(DT)              \
+    if (vec) { STEP(DT, 4); } \
+    else STEP(DT, 1)
     LA_BY_TYPE(dtype, CALL);
 #undef CALL
+#undef STEP
     V2A_CHECK_LAUNCH();
     return V2A_OK;
 }

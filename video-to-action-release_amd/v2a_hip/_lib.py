@@ -113,7 +113,7 @@ SIGNATURES = {
     "v2a_linattn_bwd": (I, [P] * 14 + [I] * 10 + [F, P, SZ, P]),
     "v2a_linattn_step": (I, [P] * 8 + [I] * 9 + [F, P]),
     "v2a_embed_fwd": (I, [P, I, P, P, P, LL, LL, LL, I, LL, LL, I, F, P]),
-    "v2a_embed_bwd_workspace_bytes": (SZ, [LL, LL, I]),
+    "v2a_embed_bwd_workspace_bytes": (SZ, [LL, LL, I, I]),
     "v2a_embed_bwd": (I, [P, I, P, P, P, LL, LL, LL, I, LL, I, F, P, SZ, P]),
     "v2a_video_qsample": (I, [P, P, P, P, P, P, I, SZ, I, P]),
     "v2a_video_loss_workspace_bytes": (SZ, [I]),

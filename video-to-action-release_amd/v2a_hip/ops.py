@@ -1701,7 +1701,7 @@ def embed_bwd(ids, dout, vocab, scale=1.0, pos_rows=None):
     D = dout.shape[-1]
     dtable = torch.empty((vocab, D), dtype=dout.dtype, device=dout.device)
     dpos = None if pos_rows is None else torch.empty((pos_rows, D), dtype=dout.dtype, device=dout.device)
-    nb = lib.v2a_embed_bwd_workspace_bytes(N, vocab, D)
+    nb = lib.v2a_embed_bwd_workspace_bytes(N, vocab, D, _SEQ_DT[dout.dtype])
     ws = torch.empty(nb, dtype=torch.uint8, device=dout.device) if nb else None
     check(lib.v2a_embed_bwd(ids.data_ptr(), wide, dout.data_ptr(), dtable.data_ptr(), _p(dpos), N, max(T, 1), vocab, D, pos_rows or 0, _SEQ_DT[dout.dtype],
                             float(scale), _p(ws), nb, _stream()), "embed_bwd")
