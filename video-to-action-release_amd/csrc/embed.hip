@@ -138,6 +138,19 @@ __device__ __forceinline__ unsigned em_scan(unsigned v, unsigned* tmp) {
     return before + x - v;
 }
 
+// this thread's digit: counts of the waves -> counts of the waves before each; returns their sum
+__device__ __forceinline__ unsigned em_waves_scan(unsigned short (*count)[EM_BINS]) {
+    unsigned c[EM_WAVES], n = 0;
+#pragma unroll
+    for (int i = 0; i < EM_WAVES; ++i) c[i] = count[i][threadIdx.x];
+#pragma unroll
+    for (int i = 0; i < EM_WAVES; ++i) {
+        count[i][threadIdx.x] = (unsigned short)n;
+        n += c[i];
+    }
+    return n;
+}
+
 struct EmSortLds {
     unsigned short count[EM_WAVES][EM_BINS];
     unsigned base[EM_BINS], tmp[EM_WAVES];
@@ -165,11 +178,7 @@ __device__ void em_sort_small(const EmSort& s, EmSortLds& L, unsigned (*xch)[EM_
         __syncthreads();
         unsigned total = 0;
         if (threadIdx.x < bins)
-            for (int i = 0; i < EM_WAVES; ++i) {
-                const unsigned n = L.count[i][threadIdx.x];
-                L.count[i][threadIdx.x] = (unsigned short)total;
-                total += n;
-            }
+            total = em_waves_scan(L.count);
         L.base[threadIdx.x] = em_scan(total, L.tmp);
         __syncthreads();
 #pragma unroll
@@ -200,7 +209,8 @@ __device__ void em_sort_small(const EmSort& s, EmSortLds& L, unsigned (*xch)[EM_
     }
 }
 
-// how many tokens of workgroup `t`'s tile have each digit of pass p
+// How many tokens of workgroup `t`'s tile have each digit of pass p.  (Counted by the scatter of the digit before, with atomics on the tile
+// that a token goes to, it would save a launch of 5 us, but a token that fills half the list takes 50 us at one address.)
 __device__ void em_hist(const EmSort& s, int p, unsigned t, unsigned* count) {
     const int bins = 1 << s.bits;
     for (int i = threadIdx.x; i < bins; i += EM_SORT_T) count[i] = 0u;
@@ -223,6 +233,7 @@ __global__ __launch_bounds__(EM_SORT_T) void embed_scatter_kernel(EmSort s, int 
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, bins = 1 << s.bits;
     unsigned before = 0, total = 0;
     if (threadIdx.x < bins)
+#pragma unroll 8
         for (unsigned t = 0; t < s.ntiles; ++t) {
             const unsigned n = s.hist[(size_t)t * bins + threadIdx.x];
             if (t < blockIdx.x) before += n;
@@ -248,11 +259,7 @@ __global__ __launch_bounds__(EM_SORT_T) void embed_scatter_kernel(EmSort s, int 
         __syncthreads();
         unsigned n = 0;
         if (threadIdx.x < bins)
-            for (int i = 0; i < EM_WAVES; ++i) {
-                const unsigned c = L.count[i][threadIdx.x];
-                L.count[i][threadIdx.x] = (unsigned short)n;
-                n += c;
-            }
+            n = em_waves_scan(L.count);
         __syncthreads();
 #pragma unroll
         for (int j = 0; j < EM_KPT; ++j)
@@ -364,26 +371,37 @@ __global__ __launch_bounds__(256) void embed_pieces_kernel(const unsigned* key, 
         for (int i = 0; i < W; ++i) x[i] = acc[i] * g.scale;
         em_st<DT, W>((E*)g.dtable + (size_t)cur * e.D + c, x);
     };
+    unsigned k[AHEAD], r[AHEAD];
+    auto fetch = [&](unsigned i0) {          // pieces begin at multiples of eight, and the lists have room to the next one
+        const uint4 k0 = *(const uint4*)(key + i0), k1 = *(const uint4*)(key + i0 + 4), r0 = *(const uint4*)(pos + i0), r1 = *(const uint4*)(pos + i0 + 4);
+        k[0] = k0.x; k[1] = k0.y; k[2] = k0.z; k[3] = k0.w; k[4] = k1.x; k[5] = k1.y; k[6] = k1.z; k[7] = k1.w;
+        r[0] = r0.x; r[1] = r0.y; r[2] = r0.z; r[3] = r0.w; r[4] = r1.x; r[5] = r1.y; r[6] = r1.z; r[7] = r1.w;
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j)
+            if (i0 + j >= b) k[j] = e.V;
+    };
+    fetch(a);
     for (unsigned i0 = a; i0 < b && cur < e.V; i0 += AHEAD) {
-        unsigned k[AHEAD];
         float x[AHEAD][W];
+        unsigned kk[AHEAD];
 #pragma unroll
         for (int j = 0; j < AHEAD; ++j) {
-            k[j] = i0 + j < b ? key[i0 + j] : e.V;
-            if (k[j] < e.V) em_ld<DT, W>((const E*)g.dout + (size_t)pos[i0 + j] * e.D + c, x[j]);
+            kk[j] = k[j];
+            if (kk[j] < e.V) em_ld<DT, W>((const E*)g.dout + (size_t)r[j] * e.D + c, x[j]);
         }
+        if (i0 + AHEAD < b) fetch(i0 + AHEAD);
 #pragma unroll
         for (int j = 0; j < AHEAD; ++j) {
             if (i0 + j >= b) break;
-            if (k[j] != cur) {
+            if (kk[j] != cur) {
                 if (before) partial(0);
                 else if (cur < e.V) whole();
                 before = false;
-                cur = k[j];
+                cur = kk[j];
 #pragma unroll
                 for (int i = 0; i < W; ++i) acc[i] = 0.f;
             }
-            if (k[j] < e.V)
+            if (kk[j] < e.V)
 #pragma unroll
                 for (int i = 0; i < W; ++i) acc[i] += x[j][i];
         }
@@ -394,36 +412,55 @@ __global__ __launch_bounds__(256) void embed_pieces_kernel(const unsigned* key, 
     else whole();
 }
 
-// Rows that cross pieces: the piece in which one begins adds its part 1 and the parts 0 of the pieces behind it; wave w takes pieces w, w + 8, ..
+// Rows that cross pieces: the piece in which one begins adds its part 1 and the parts 0 of the pieces behind it, wave w those of w, w + 16, ..
+// One workgroup per (16 pieces, 256 columns), most of which have nothing to do; a run's end is found first, 64 borders at a time, so that the
+// sum has known bounds and eight loads under way.
+constexpr int EM_JOIN = 16;
 template <int DT>
-__global__ __launch_bounds__(512) void embed_join_kernel(const unsigned* key, EmGrad g, EmShape e, const float* part, int Dp, unsigned ts) {
+__global__ __launch_bounds__(1024) void embed_join_kernel(const unsigned* key, EmGrad g, EmShape e, const float* part, int Dp, unsigned ts) {
     typedef typename EmT<DT>::T E;
-    __shared__ float sum[8][256];
-    const unsigned t = blockIdx.x, a = t * ts;
-    const unsigned long long b = (unsigned long long)a + ts;
-    if (b >= e.N) return;
-    const unsigned cur = key[b - 1];
-    if (cur >= e.V || key[b] != cur || (key[a] == cur && a > 0 && key[a - 1] == cur)) return;
+    constexpr int NWV = 16;
+    __shared__ float sum[NWV][256];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const unsigned np = (e.N - 1) / ts + 1;
-    for (int c0 = 0; c0 < e.D; c0 += 256) {
-        const int c = c0 + lane * 4;
+    const unsigned long long mine = (unsigned long long)blockIdx.x * EM_JOIN + lane, b = (mine + 1) * ts;
+    bool owns = false;
+    unsigned id = 0;
+    if (lane < EM_JOIN && b < e.N) {
+        const size_t a = mine * ts;
+        id = key[b - 1];
+        owns = id < e.V && key[b] == id && !(key[a] == id && a > 0 && key[a - 1] == id);
+    }
+    for (unsigned long long todo = __ballot(owns); todo; todo &= todo - 1) {
+        const int at = __ffsll((unsigned long long)todo) - 1;
+        const unsigned t = blockIdx.x * EM_JOIN + at, cur = __shfl(id, at, 64);
+        unsigned lo = t + 2, hi = np;          // the first piece from t + 2 on that begins with another id lies in [lo, hi]
+        while (lo < hi) {
+            const unsigned step = (hi - lo + 63) / 64, i = lo + lane * step;
+            const unsigned n = __popcll(__ballot(i < hi && key[(size_t)i * ts] == cur));      // sorted: a prefix of the probes
+            if (n == 0) { hi = lo; break; }
+            const unsigned top = lo + n * step;
+            lo = lo + (n - 1) * step + 1;
+            hi = top < hi ? top : hi;
+        }
+        const unsigned end = hi;
+        const int c0 = blockIdx.y * 256, c = c0 + lane * 4;
         float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
         if (c < e.D) {
             if (w == 0) s = *(const float4*)(part + ((size_t)t * 2 + 1) * Dp + c);
-#pragma unroll 4
-            for (unsigned i = t + 1 + w; i < np; i += 8) {
-                if (key[(size_t)i * ts] != cur) break;
+#pragma unroll 8
+            for (unsigned i = t + 1 + w; i < end; i += NWV) {
                 const float4 x = *(const float4*)(part + (size_t)i * 2 * Dp + c);
                 s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
             }
             *(float4*)&sum[w][lane * 4] = s;
         }
         __syncthreads();
-        for (int d = threadIdx.x; d < 256 && c0 + d < e.D; d += 512) {
+        const int d = threadIdx.x;
+        if (d < 256 && c0 + d < e.D) {
             float y = sum[0][d];
 #pragma unroll
-            for (int i = 1; i < 8; ++i) y += sum[i][d];
+            for (int i = 1; i < NWV; ++i) y += sum[i][d];
             ((E*)g.dtable)[(size_t)cur * e.D + c0 + d] = em_r<DT>(y * g.scale);
         }
         __syncthreads();
@@ -439,6 +476,8 @@ EmShape em_shape(long long N, long long T, long long V, int D, int W) {
     const int pieces = cdiv(D, W);
     e.lpr = 1;
     while (e.lpr < pieces && e.lpr < 64) e.lpr *= 2;
+    // 64 lanes would idle in the last block of a row of, say, 96 pieces: half of them where that covers fewer places
+    while (e.lpr > 16 && cdiv(pieces, e.lpr / 2) * (e.lpr / 2) < cdiv(pieces, e.lpr) * e.lpr) e.lpr /= 2;
     e.ncol = cdiv(pieces, e.lpr);
     return e;
 }
@@ -456,8 +495,9 @@ EmWs em_ws(long long N, int D, int dtype) {
     auto take = [&](size_t n) { const size_t o = at; at += (n + 255) & ~(size_t)255; return o; };
     w.ts = em_piece(N, D, dtype);
     w.Dp = (D + 7) & ~7;
-    w.key = take(N * 4); w.pos = take(N * 4);
-    w.key2 = take(N > EM_SMALL ? N * 4 : 0); w.pos2 = take(N > EM_SMALL ? N * 4 : 0);
+    const size_t n4 = (size_t)(N + 7) / 8 * 8 * 4;
+    w.key = take(n4); w.pos = take(n4);
+    w.key2 = take(N > EM_SMALL ? n4 : 0); w.pos2 = take(N > EM_SMALL ? n4 : 0);
     w.hist = take(N > EM_SMALL ? (size_t)EM_TILES * EM_BINS * 4 : 0);
     w.part = take((size_t)cdiv(N, w.ts) * 2 * w.Dp * 4);
     w.total = at;
@@ -548,7 +588,7 @@ int v2a_embed_bwd(const void* ids, int ids64, const void* dout, void* dtable, vo
 #undef CALL
     V2A_CHECK_LAUNCH();
     if (pieces > 1) {
-#define CALL(DT, W) hipLaunchKernelGGL((embed_join_kernel<DT>), dim3(pieces - 1), dim3(512), 0, s, q.key, g, e, (const float*)(base + w.part), w.Dp, w.ts)
+#define CALL(DT, W) hipLaunchKernelGGL((embed_join_kernel<DT>), dim3(cdiv(pieces - 1, EM_JOIN), cdiv(D, 256)), dim3(1024), 0, s, q.key, g, e, (const float*)(base + w.part), w.Dp, w.ts)
         EM_BY_TYPE(dtype, false, CALL);
 #undef CALL
         V2A_CHECK_LAUNCH();

@@ -400,6 +400,8 @@ __global__ __launch_bounds__(64 * NW, 2) void la_scan(LaArgs a, LaScan p) {
                         la_store4<DT>(out + r * ot + d, f32x4{0.f, 0.f, 0.f, 0.f}, Dv - d, p.vo);
             continue;
         }
+        const bool live = i > seg * p.cps || seg || p.init;               // the state is not 0
+        const bool keep = !OUT || i + 1 < iend || p.last;                 // somebody reads it
         f32x4 O[OUT ? NT : 1][4];
         if constexpr (OUT) {
 #pragma unroll
@@ -433,6 +435,7 @@ __global__ __launch_bounds__(64 * NW, 2) void la_scan(LaArgs a, LaScan p) {
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int it = 0; it < 4; ++it) O[n][it] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (live)
 #pragma unroll
             for (int kk = 0; kk < DK / 32; ++kk) {
                 typename LaOp<DT>::C2 sf[NT];
@@ -444,12 +447,13 @@ __global__ __launch_bounds__(64 * NW, 2) void la_scan(LaArgs a, LaScan p) {
                     la_split(x, sf[n]);
                 }
 #pragma unroll
-                for (int it = 0; it < 4; ++it) {
-                    typename LaOp<DT>::In qf;
-                    TX::nat(sq, it * 16, kk, lane, qf);
+                for (int it = 0; it < 4; ++it)
+                    if (it * 16 < nv) {
+                        typename LaOp<DT>::In qf;
+                        TX::nat(sq, it * 16, kk, lane, qf);
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) la_mma(O[n][it], sf[n], qf);
-                }
+                        for (int n = 0; n < NT; ++n) la_mma(O[n][it], sf[n], qf);
+                    }
                 __builtin_amdgcn_sched_barrier(0);      // else every operand read of the loop is hoisted and spilled
             }
 #pragma unroll
@@ -496,6 +500,7 @@ __global__ __launch_bounds__(64 * NW, 2) void la_scan(LaArgs a, LaScan p) {
                         }
                     __builtin_amdgcn_sched_barrier(0);
                 }
+                if (keep)
 #pragma unroll
                 for (int d = 0; d < DK / 16; ++d) {
                     typename LaOp<DT>::In xf;
@@ -531,10 +536,16 @@ __global__ __launch_bounds__(256) void la_combine(float* seg, const float* seg_d
     float s = init ? init[bh * SS + e] : 0.f;
     float* q = seg + bh * nseg * SS + e;
     const float* f = seg_decay + bh * nseg;
-    for (int i = 0; i < nseg; ++i) {
-        const float x = i + 1 < nseg ? q[i * SS] : 0.f;
-        q[i * SS] = s;
-        s = s * f[i] + x;
+    for (int i0 = 0; i0 < nseg; i0 += 8) {
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = i0 + j + 1 < nseg ? q[(i0 + j) * SS] : 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (i0 + j < nseg) {
+                q[(i0 + j) * SS] = s;
+                s = s * f[i0 + j] + x[j];
+            }
     }
 }
 
@@ -1035,7 +1046,8 @@ template <int DT, int DK, bool OUT> int la_scan_dv(const LaArgs& a, const LaScan
     const dim3 grid((unsigned)((long long)a.B * a.H * p.ndv * p.nseg));
     if (dvt == 32) hipLaunchKernelGGL((la_scan<DT, DK, 1, 2, OUT>), grid, dim3(128), 0, s, a, p);
     else if (dvt == 64) hipLaunchKernelGGL((la_scan<DT, DK, 1, 4, OUT>), grid, dim3(256), 0, s, a, p);
-    else hipLaunchKernelGGL((la_scan<DT, DK, 2, 4, OUT>), grid, dim3(256), 0, s, a, p);
+    else if constexpr (DK == 32) hipLaunchKernelGGL((la_scan<DT, DK, 2, 4, OUT>), grid, dim3(256), 0, s, a, p);
+    else hipLaunchKernelGGL((la_scan<DT, DK, 1, 8, OUT>), grid, dim3(512), 0, s, a, p);
     V2A_CHECK_LAUNCH();
     return V2A_OK;
 }
