@@ -32,10 +32,10 @@ __device__ __forceinline__ float la_clampg(float g) { return g < LA_GMIN ? LA_GM
 // A chunk is 64 tokens.  With G_i = g_1 + .. + g_i inside it, W_ij = exp(G_i - G_j) for j <= i and S the state before it,
 //     o_i = scale (exp(G_i) S^T q_i + sum_j W_ij (q_i . k_j) v_j),      S' = exp(G_64) S + sum_j exp(G_64 - G_j) k_j v_j^T,
 // all of it matrix products.  They run on 16 x 16 x 32 MFMA tiles whose 32-long reduction index is numbered so that no operand is ever
-// shuffled: slot e of lane group lane / 16 is element 4 (lane / 16) + e for e < 4 and 16 + 4 (lane / 16) + e - 4 above.  With that
-// numbering two stacked 16 x 16 accumulators ARE the next product's operand (rows of one index, lane % 16 the other): the pair scores and
-// the state go from accumulator to operand in registers, and a transposing LDS read (ds_read_b64_tr_b16) of a row-major tile gives the
-// operand of the transposed tile.
+// shuffled; lane group g = lane / 16 holds eight slots of it.  Over tokens, slots 0 .. 3 are tokens 4 g .. of the first 16 and slots 4 .. 7
+// those of the second 16: two stacked 16 x 16 score accumulators ARE the operand of the product with v, and two transposing LDS reads
+// (ds_read_b64_tr_b16) of a row-major tile give the operand of the transposed tile.  Over a head's width the slots are eight neighbours
+// 8 g ..: one 16-byte read of a row; the state's rows are dealt to its accumulators so that two of them are such an operand as well.
 // Number formats: bf16 inputs are one exact 8-bit plane, fp16 inputs two (8 + 3 bits, exact); factors computed in fp32 (scores, states)
 // are fed as two planes (off by at most 2^-17 of the value), decay-weighted values of the state update as three (exact fp32), because the
 // state is an fp32 result and lives long.  Sums are fp32.  fp32 inputs use the fp32 MFMA (16 x 16 x 4) in the same slot order.
@@ -123,26 +123,23 @@ template <int DT, int D> struct LaTile {
     static constexpr int PLANE = LA_C * PITCH;
     static constexpr int BYTES = PLANE * NP;
     static __device__ __forceinline__ void nat(const char* t, int row0, int kk, int lane, typename LaOp<DT>::In& o) {
-        const char* q = t + (row0 + (lane & 15)) * PITCH;
+        const char* q = t + (row0 + (lane & 15)) * PITCH + (kk * 32 + (lane >> 4) * 8) * (DT == 0 ? 4 : 2);
         if constexpr (DT == 0) {
-            const float4 a = *(const float4*)(q + (kk * 32 + (lane >> 4) * 4) * 4), b = *(const float4*)(q + (kk * 32 + 16 + (lane >> 4) * 4) * 4);
+            const float4 a = *(const float4*)q, b = *(const float4*)(q + 16);
             o.x[0] = a.x; o.x[1] = a.y; o.x[2] = a.z; o.x[3] = a.w; o.x[4] = b.x; o.x[5] = b.y; o.x[6] = b.z; o.x[7] = b.w;
         } else {
 #pragma unroll
-            for (int n = 0; n < NP; ++n) {
-                const la_u32x2 a = *(const la_u32x2*)(q + n * PLANE + (kk * 32 + (lane >> 4) * 4) * 2);
-                const la_u32x2 b = *(const la_u32x2*)(q + n * PLANE + (kk * 32 + 16 + (lane >> 4) * 4) * 2);
-                o.p[n] = la_u32x4{a[0], a[1], b[0], b[1]};
-            }
+            for (int n = 0; n < NP; ++n) o.p[n] = *(const la_u32x4*)(q + n * PLANE);
         }
     }
-    static __device__ __forceinline__ void tr(const char* t, int ks, int col0, int lane, typename LaOp<DT>::In& o) {
+    // lane % 16 = column col0 + CS (lane % 16 / 4) + lane % 4: 16 neighbours (CS 4), or every other four of 32 (CS 8)
+    template <int CS> static __device__ __forceinline__ void tr(const char* t, int ks, int col0, int lane, typename LaOp<DT>::In& o) {
         if constexpr (DT == 0) {
-            const char* q = t + (ks * 32 + (lane >> 4) * 4) * PITCH + (col0 + (lane & 15)) * 4;
+            const char* q = t + (ks * 32 + (lane >> 4) * 4) * PITCH + (col0 + CS * ((lane & 15) >> 2) + (lane & 3)) * 4;
 #pragma unroll
             for (int e = 0; e < 8; ++e) o.x[e] = *(const float*)(q + (e < 4 ? e : 12 + e) * PITCH);
         } else {
-            const char* q = t + (ks * 32 + (lane >> 4) * 4 + ((lane & 15) >> 2)) * PITCH + (col0 + 4 * (lane & 3)) * 2;
+            const char* q = t + (ks * 32 + (lane >> 4) * 4 + ((lane & 15) >> 2)) * PITCH + (col0 + CS * (lane & 3)) * 2;
 #pragma unroll
             for (int n = 0; n < NP; ++n) {
                 const la_u32x2 a = __builtin_bit_cast(la_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4bf16((la_lds_bf16x4*)(q + n * PLANE)));
@@ -217,20 +214,35 @@ template <int DT, int D, int NTH> struct LaLoad {
     }
 };
 
-// Running log2 decays of a chunk in every lane of one wave (lane = token): pair hi + lo, and the chunk's total
+// Running log2 decays of a chunk, computed by one wave (lane = token): pair hi + lo, and the chunk's total
 struct LaGate {
     float hi[LA_C], lo[LA_C];          // G_i
     float wq[LA_C], wk[LA_C];          // exp(G_i), exp(G_64 - G_i)
     float total;                       // exp(G_64)
+    float pad[3];
 };
+// x of the lane `shr` lanes below within the 16-lane row, 0 where there is none
+template <int CTRL> __device__ __forceinline__ double la_row_shr(double x) {
+    const la_u32x2 u = __builtin_bit_cast(la_u32x2, x);
+    return __builtin_bit_cast(double, la_u32x2{(unsigned)__builtin_amdgcn_update_dpp(0, (int)u[0], CTRL, 0xf, 0xf, true),
+                                               (unsigned)__builtin_amdgcn_update_dpp(0, (int)u[1], CTRL, 0xf, 0xf, true)});
+}
+__device__ __forceinline__ double la_lane(double x, int l) {
+    const la_u32x2 u = __builtin_bit_cast(la_u32x2, x);
+    return __builtin_bit_cast(double, la_u32x2{(unsigned)__builtin_amdgcn_readlane((int)u[0], l), (unsigned)__builtin_amdgcn_readlane((int)u[1], l)});
+}
+// inclusive sum over the 64 lanes: inside the rows by DPP, over the rows by readlane (twelve ds_bpermute round trips otherwise: 1000 cycles)
+__device__ __forceinline__ double la_running(double x, int lane) {
+    x += la_row_shr<0x111>(x);
+    x += la_row_shr<0x112>(x);
+    x += la_row_shr<0x114>(x);
+    x += la_row_shr<0x118>(x);
+    const double r0 = la_lane(x, 15), r1 = la_lane(x, 31), r2 = la_lane(x, 47);
+    return x + (lane < 16 ? 0.0 : lane < 32 ? r0 : lane < 48 ? r0 + r1 : r0 + r1 + r2);
+}
 __device__ __forceinline__ void la_gates(LaGate& s, float g, bool on, int lane) {
-    double x = on ? (double)la_clampg(g) * 1.4426950408889634 : 0.0;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const double y = __shfl_up(x, o, 64);
-        if (lane >= o) x += y;
-    }
-    const double tot = __shfl(x, 63, 64);
+    const double x = la_running(on ? (double)la_clampg(g) * 1.4426950408889634 : 0.0, lane);
+    const double tot = la_lane(x, 63);
     const float hi = (float)x;
     s.hi[lane] = hi;
     s.lo[lane] = (float)(x - (double)hi);
@@ -243,6 +255,7 @@ __device__ __forceinline__ void la_gates(LaGate& s, float g, bool on, int lane) 
 __device__ constexpr int la_unit_tile(int u) { return u == 0 ? 0 : u == 1 ? 1 : u < 4 ? 2 : 3; }
 __device__ constexpr int la_unit_step(int u) { return u == 3 || u == 5 ? 1 : 0; }
 __device__ constexpr int la_unit_wave(int u, int nw) { return nw == 1 ? 0 : nw == 2 ? u / 3 : nw == 4 ? (u < 2 ? 0 : u < 4 ? 1 : u - 2) : u; }
+__device__ __forceinline__ int la_unit(int tile, int step) { return step == 0 ? (tile < 3 ? tile : 4) : tile == 2 ? 3 : 5; }
 template <int DT> constexpr int la_unit_bytes() { return 64 * 32; }      // two planes of 16 bytes a lane, or eight floats
 
 template <int DT> __device__ __forceinline__ void la_put(char* p, int u, int lane, const float* x) {
@@ -301,21 +314,29 @@ struct LaScan {
     float* chunk;               // state before each chunk in scan order, [B H][NC][Dk][Dv] (NULL: not kept)
     float* last;                // state behind the last chunk (NULL)
     void* out;
-    int NC, cps, nseg, ndv, local, rev, vx, vy, vq, vo;
+    int NC, cps, nseg, ndv, local, rev, vx, vy, vq, vo, vst;
 };
 
 // One workgroup walks the chunks of one segment of one (row, head) for NW * NT * 16 columns of the state, which stays in registers as
 // accumulators: wave w owns columns 16 NT w .. and all Dk rows.  OUT: the outputs too.  rev: the recurrence of the state's gradient, from the
 // last chunk to the first, E <- exp(G_64) E + scale sum_i exp(G_i) q_i dout_i^T (x = q, y = dout), else x = k, y = v.
+template <int DT, int DK, int NT, int NW, bool OUT> constexpr int la_scan_lds() {
+    return LaTile<DT, DK>::BYTES * (OUT ? 2 : 1) + LaTile<DT, 16 * NT * NW>::BYTES + (OUT ? 6 * la_unit_bytes<DT>() : 0);
+}
+// waves per SIMD that the LDS allows, two at most: the register bound of the launch
+template <int DT, int DK, int NT, int NW, bool OUT> constexpr int la_scan_waves() {
+    const int n = 160 * 1024 / (la_scan_lds<DT, DK, NT, NW, OUT>() + 2304) * NW / 4;
+    return n < 1 ? 1 : n > 2 ? 2 : n;
+}
 template <int DT, int DK, int NT, int NW, bool OUT>
-__global__ __launch_bounds__(64 * NW, 2) void la_scan(LaArgs a, LaScan p) {
+__global__ __launch_bounds__(64 * NW, (la_scan_waves<DT, DK, NT, NW, OUT>())) void la_scan(LaArgs a, LaScan p) {
     typedef typename LaT<DT>::T E;
     typedef LaTile<DT, DK> TX;
     constexpr int DVT = 16 * NT * NW, NTH = 64 * NW;
     typedef LaTile<DT, DVT> TY;
-    constexpr int QB = OUT ? TX::BYTES : 0, PB = OUT ? 6 * la_unit_bytes<DT>() : 0;
-    __shared__ __attribute__((aligned(16))) char sm[TX::BYTES + TY::BYTES + QB + PB];
-    __shared__ __attribute__((aligned(16))) LaGate gt;
+    constexpr int QB = OUT ? TX::BYTES : 0;
+    __shared__ __attribute__((aligned(16))) char sm[la_scan_lds<DT, DK, NT, NW, OUT>()];
+    __shared__ __attribute__((aligned(16))) LaGate gts[2];
     char* sx = sm;
     char* sy = sx + TX::BYTES;
     char* sq = sy + TY::BYTES;
@@ -335,90 +356,163 @@ __global__ __launch_bounds__(64 * NW, 2) void la_scan(LaArgs a, LaScan p) {
     const float* g = a.g + b * a.gs[0] + h * a.gs[2];
     const long long SS = (long long)Dk * Dv;
 
+    // This lane's state values.  OUT: S[i][n][r] is row 32 (i / 2) + 8 (lane / 16) + 4 (i % 2) + r, column c0 + 4 n (two tiles a wave: every
+    // other four of 32 columns, so that a lane's outputs are eight neighbours) -- the operand of the product with q.  Else the transposed
+    // tile, row 16 i + lane % 16, columns c0 + 16 n + r: four neighbours for the states that go to memory.
     f32x4 S[DK / 16][NT];
-    const int d0 = (lane >> 4) * 4, c0 = dv0 + (lane & 15);      // of this lane's state values: rows d0 + 16 i + r, columns c0 + 16 n
-    {
-        const float* s0 = p.local ? nullptr : seg ? p.seg + ((long long)bh * p.nseg + seg) * SS : p.init ? p.init + bh * SS : nullptr;
-        const float* q = s0 + d0 * Dv + c0;
+    constexpr int CS = OUT && NT == 2 ? 8 : 4, NC0 = CS == 8 ? 4 : 16;
+    const int d0 = OUT ? (lane >> 4) * 8 : lane & 15, c0 = OUT ? dv0 + CS * ((lane & 15) >> 2) + (lane & 3) : dv0 + (lane >> 4) * 4;
+    // OUT exchanges the state through LDS, half of the rows at a time (in whole 32-row blocks), so that memory sees whole rows
+    constexpr int NH = DK == 32 ? 1 : 2, HR = DK / NH, PER = HR * DVT / 4 / NTH;
+    static_assert(!OUT || HR * DVT * 4 <= la_scan_lds<DT, DK, NT, NW, OUT>(), "half a state fits");
+    auto get_state = [&](const float* s0) __attribute__((always_inline)) {
+        if constexpr (OUT) {
 #pragma unroll
-        for (int i = 0; i < DK / 16; ++i)
+            for (int half = 0; half < NH; ++half) {
+                f32x4 t[PER];
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
+                for (int e = 0; e < PER; ++e) {
+                    const int at = (e * NTH + threadIdx.x) * 4, d = half * HR + at / DVT, c = dvt * DVT + at % DVT;
+                    t[e] = f32x4{0.f, 0.f, 0.f, 0.f};
+                    if (d < Dk && c < Dv) {
+                        const float* q = s0 + d * Dv + c;
+                        if (p.vst) t[e] = *(const f32x4*)q;
+                        else
 #pragma unroll
-                for (int r = 0; r < 4; ++r) S[i][n][r] = s0 && d0 + i * 16 + r < Dk && c0 + n * 16 < Dv ? q[(i * 16 + r) * Dv + n * 16] : 0.f;
-    }
-    auto put_state = [&](float* dst) {
-        float* q = dst + d0 * Dv + c0;
+                            for (int r = 0; r < 4; ++r) t[e][r] = c + r < Dv ? q[r] : 0.f;
+                    }
+                }
+                __syncthreads();
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-            if (c0 + n * 16 < Dv)
+                for (int e = 0; e < PER; ++e) ((f32x4*)sm)[e * NTH + threadIdx.x] = t[e];
+                __syncthreads();
 #pragma unroll
-                for (int i = 0; i < DK / 16; ++i)
+                for (int i = half * (HR / 16); i < (half + 1) * (HR / 16); ++i)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (d0 + i * 16 + r < Dk) q[(i * 16 + r) * Dv + n * 16] = S[i][n][r];
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            S[i][n][r] = ((const float*)sm)[(d0 + i / 2 * 32 + i % 2 * 4 + r - half * HR) * DVT + c0 - dvt * DVT + n * NC0];
+            }
+        } else
+#pragma unroll
+            for (int i = 0; i < DK / 16; ++i)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const int d = d0 + i * 16, c = c0 + n * NC0;
+                    const float* q = s0 + d * Dv + c;
+                    if (d < Dk && c < Dv) {
+                        if (p.vst) S[i][n] = *(const f32x4*)q;
+                        else
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) S[i][n][r] = c + r < Dv ? q[r] : 0.f;
+                    }
+                }
     };
+    auto put_state = [&](float* dst) __attribute__((always_inline)) {
+        if constexpr (OUT) {
+#pragma unroll
+            for (int half = 0; half < NH; ++half) {
+                __syncthreads();
+#pragma unroll
+                for (int i = half * (HR / 16); i < (half + 1) * (HR / 16); ++i)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            ((float*)sm)[(d0 + i / 2 * 32 + i % 2 * 4 + r - half * HR) * DVT + c0 - dvt * DVT + n * NC0] = S[i][n][r];
+                __syncthreads();
+#pragma unroll
+                for (int e = 0; e < PER; ++e) {
+                    const int at = (e * NTH + threadIdx.x) * 4, d = half * HR + at / DVT, c = dvt * DVT + at % DVT;
+                    if (d < Dk && c < Dv) la_store4<0>(dst + d * Dv + c, ((const f32x4*)sm)[e * NTH + threadIdx.x], Dv - c, p.vst);
+                }
+            }
+        } else
+#pragma unroll
+            for (int i = 0; i < DK / 16; ++i)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const int d = d0 + i * 16, c = c0 + n * NC0;
+                    if (d < Dk && c < Dv) la_store4<0>(dst + d * Dv + c, S[i][n], Dv - c, p.vst);
+                }
+    };
+#pragma unroll
+    for (int i = 0; i < DK / 16; ++i)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) S[i][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (const float* s0 = p.local ? nullptr : seg ? p.seg + ((long long)bh * p.nseg + seg) * SS : p.init ? p.init + bh * SS : nullptr) get_state(s0);
     LaLoad<DT, DK, NTH> rx, rq;
     LaLoad<DT, DVT, NTH> ry;
     float rg = 0.f;
+    const int ibeg = seg * p.cps, iend = (seg + 1) * p.cps < p.NC ? (seg + 1) * p.cps : p.NC;
+    // chunks with tokens: the first ones of the sequence.  The others leave the state as it is and are walked apart from the main loop, so
+    // that the accumulators have one definition in it (a second path through the loop doubled their registers).
+    const int nvc = (len + LA_C - 1) / LA_C, vlo = p.rev ? p.NC - nvc : 0, vhi = p.rev ? p.NC : nvc;
+    const int vbeg = vlo > ibeg ? (vlo < iend ? vlo : iend) : ibeg, vend = vhi < iend ? (vhi > vbeg ? vhi : vbeg) : iend;
+    auto chunk_of = [&](int i) { return p.rev ? p.NC - 1 - i : i; };
     auto valid = [&](int i) {
-        const int n = len - (p.rev ? p.NC - 1 - i : i) * LA_C;
-        return n < 0 ? 0 : n > LA_C ? LA_C : n;
+        const int n = len - chunk_of(i) * LA_C;
+        return n > LA_C ? LA_C : n;
     };
-    const int iend = (seg + 1) * p.cps < p.NC ? (seg + 1) * p.cps : p.NC;
-    auto fetch = [&](int i) {
-        if (i >= iend) return;
-        const int nv = valid(i);
-        if (nv == 0) return;
-        const long long t0 = (long long)(p.rev ? p.NC - 1 - i : i) * LA_C;
-        rx.load(X + t0 * sxt, sxt, nv, Dk, p.vx);
-        ry.load(Y + t0 * syt, syt, nv, yroom, p.vy);
-        if constexpr (OUT) rq.load(Q + t0 * a.qs[1], a.qs[1], nv, Dk, p.vq);
-        if (wid == 0 && lane < nv) rg = g[(t0 + lane) * a.gs[1]];
+    // The next chunk's rows are requested behind the score barrier: the work behind it is as long as the loads take, and their registers are
+    // free before it.  Its decays are summed by the last wave meanwhile (gts[i & 1] belongs to chunk i), from values requested a chunk earlier.
+    auto first = [&](int i) { return (long long)chunk_of(i) * LA_C; };
+    auto fetch_x = [&](int i) { if (i < vend) rx.load(X + first(i) * sxt, sxt, valid(i), Dk, p.vx); };
+    auto fetch_y = [&](int i) { if (i < vend) ry.load(Y + first(i) * syt, syt, valid(i), yroom, p.vy); };
+    auto fetch_q = [&](int i) { if constexpr (OUT) if (i < vend) rq.load(Q + first(i) * a.qs[1], a.qs[1], valid(i), Dk, p.vq); };
+    auto fetch_g = [&](int i) { if (wid == NW - 1 && i < vend && lane < valid(i)) rg = g[(first(i) + lane) * a.gs[1]]; };
+    auto gates = [&](int i) { if (wid == NW - 1 && i < vend) la_gates(gts[i & 1], rg, lane < valid(i), lane); };
+    auto skip = [&](int i) __attribute__((always_inline)) {               // a chunk without tokens
+        const int c = chunk_of(i);
+        if constexpr (OUT) {
+            E* out = (E*)p.out + (((long long)b * a.T + (long long)c * LA_C) * a.H + h) * Dv;
+            const int rows = a.T - c * LA_C < LA_C ? a.T - c * LA_C : LA_C;
+            for (int r = wid * 16 + (lane & 15); r < rows; r += 16 * NW)
+                for (int d = dvt * DVT + (lane >> 4) * 4; d < dvt * DVT + DVT && d < Dv; d += 16)
+                    la_store4<DT>(out + (long long)r * a.H * Dv + d, f32x4{0.f, 0.f, 0.f, 0.f}, Dv - d, p.vo);
+        } else if (p.chunk && i > 0) put_state(p.chunk + ((long long)bh * p.NC + c) * SS);
     };
     float fac = 1.f;
-    fetch(seg * p.cps);
-    for (int i = seg * p.cps; i < iend; ++i) {
-        const int c = p.rev ? p.NC - 1 - i : i, nv = valid(i);
-        if (p.chunk && i > 0) put_state(p.chunk + ((long long)bh * p.NC + c) * SS);
+    fetch_g(vbeg);
+    fetch_x(vbeg);
+    fetch_y(vbeg);
+    fetch_q(vbeg);
+    for (int i = ibeg; i < vbeg; ++i) skip(i);
+    gates(vbeg);
+    fetch_g(vbeg + 1);
+    for (int i = vbeg; i < vend; ++i) {
+        const int c = chunk_of(i), nv = valid(i);
+        if (!OUT && p.chunk && i > 0) put_state(p.chunk + ((long long)bh * p.NC + c) * SS);
         E* out = (E*)p.out + (((long long)b * a.T + (long long)c * LA_C) * a.H + h) * Dv;
         const int rows = a.T - c * LA_C < LA_C ? a.T - c * LA_C : LA_C;
         const long long ot = (long long)a.H * Dv;
-        if (nv > 0) {
-            __syncthreads();
-            rx.store(sx);
-            ry.store(sy);
-            if constexpr (OUT) rq.store(sq);
-            if (wid == 0) la_gates(gt, rg, lane < nv, lane);
-            __syncthreads();
-        }
-        fetch(i + 1);
-        if (nv == 0) {                      // behind the row's end: the state stays, the outputs are 0
-            if constexpr (OUT)
-                for (int r = wid * 16 + (lane & 15); r < rows; r += 16 * NW)
-                    for (int d = dvt * DVT + (lane >> 4) * 4; d < dvt * DVT + DVT && d < Dv; d += 16)
-                        la_store4<DT>(out + r * ot + d, f32x4{0.f, 0.f, 0.f, 0.f}, Dv - d, p.vo);
-            continue;
-        }
-        const bool live = i > seg * p.cps || seg || p.init;               // the state is not 0
-        const bool keep = !OUT || i + 1 < iend || p.last;                 // somebody reads it
-        f32x4 O[OUT ? NT : 1][4];
+        __syncthreads();
+        rx.store(sx);
+        ry.store(sy);
+        if constexpr (OUT) rq.store(sq);
+        __syncthreads();
+        const LaGate& gt = gts[i & 1];
+        const bool live = i > vbeg || seg || p.init;                      // the state is not 0
+        const bool keep = !OUT || i + 1 < vend || p.last;                 // somebody reads it
+        const int nks = nv > 32 ? 2 : 1;
         if constexpr (OUT) {
+            f32x4 O[NT][4];
 #pragma unroll
             for (int u = 0; u < 6; ++u)
                 if (la_unit_wave(u, NW) == wid && la_unit_tile(u) * 16 < nv) {
                     const int it = la_unit_tile(u), js = la_unit_step(u) * 32;
                     const bool two = js + 16 <= it * 16;
-                    f32x4 c0 = {0.f, 0.f, 0.f, 0.f}, c1 = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 1
+                    f32x4 s0 = {0.f, 0.f, 0.f, 0.f}, s1 = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 2
                     for (int kk = 0; kk < DK / 32; ++kk) {
                         typename LaOp<DT>::In qf, kf;
                         TX::nat(sq, it * 16, kk, lane, qf);
                         TX::nat(sx, js, kk, lane, kf);
-                        la_mma_in<DT>(c0, kf, qf);
+                        la_mma_in<DT>(s0, kf, qf);
                         if (two) {
                             TX::nat(sx, js + 16, kk, lane, kf);
-                            la_mma_in<DT>(c1, kf, qf);
+                            la_mma_in<DT>(s1, kf, qf);
                         }
                     }
                     float w[8], x[8];
@@ -426,8 +520,8 @@ __global__ __launch_bounds__(64 * NW, 2) void la_scan(LaArgs a, LaScan p) {
                     la_weights<false>(gt, js + 16, it * 16 + (lane & 15), lane, w + 4);
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        x[r] = c0[r] * w[r] * a.scale;
-                        x[4 + r] = c1[r] * w[4 + r] * a.scale;
+                        x[r] = s0[r] * w[r] * a.scale;
+                        x[4 + r] = s1[r] * w[4 + r] * a.scale;
                     }
                     la_put<DT>(sp, u, lane, x);
                 }
@@ -435,94 +529,119 @@ __global__ __launch_bounds__(64 * NW, 2) void la_scan(LaArgs a, LaScan p) {
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int it = 0; it < 4; ++it) O[n][it] = f32x4{0.f, 0.f, 0.f, 0.f};
-            if (live)
+            if (live) {
 #pragma unroll
-            for (int kk = 0; kk < DK / 32; ++kk) {
-                typename LaOp<DT>::C2 sf[NT];
+                for (int kk = 0; kk < DK / 32; ++kk) {
+                    typename LaOp<DT>::C2 sf[NT];
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    float x[8];
+                    for (int n = 0; n < NT; ++n) {
+                        float x[8];
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) { x[r] = S[2 * kk][n][r]; x[4 + r] = S[2 * kk + 1][n][r]; }
-                    la_split(x, sf[n]);
-                }
+                        for (int r = 0; r < 4; ++r) { x[r] = S[2 * kk][n][r]; x[4 + r] = S[2 * kk + 1][n][r]; }
+                        la_split(x, sf[n]);
+                    }
 #pragma unroll
-                for (int it = 0; it < 4; ++it)
-                    if (it * 16 < nv) {
+                    for (int it = 0; it < 4; ++it) {
                         typename LaOp<DT>::In qf;
                         TX::nat(sq, it * 16, kk, lane, qf);
 #pragma unroll
                         for (int n = 0; n < NT; ++n) la_mma(O[n][it], sf[n], qf);
                     }
-                __builtin_amdgcn_sched_barrier(0);      // else every operand read of the loop is hoisted and spilled
+                    __builtin_amdgcn_sched_barrier(0);      // else the splits of the whole state are done at once and spill
+                }
+#pragma unroll
+                for (int it = 0; it < 4; ++it) {
+                    const float w = gt.wq[it * 16 + (lane & 15)] * a.scale;
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) O[n][it] *= w;
+                }
             }
+            gates(i + 1);
+            fetch_g(i + 2);
+            __syncthreads();
+            fetch_x(i + 1);
+            fetch_y(i + 1);
+            fetch_q(i + 1);
+#pragma unroll 1
+            for (int ks = 0; ks < nks; ++ks) {
+                typename LaOp<DT>::In yf[NT];
+#pragma unroll
+                for (int n = 0; n < NT; ++n) TY::template tr<CS>(sy, ks, wid * NT * 16 + n * NC0, lane, yf[n]);
+#pragma unroll
+                for (int it = 0; it < 4; ++it)
+                    if ((it >= 2 || ks == 0) && it * 16 < nv) {
+                        typename LaOp<DT>::C2 pf;
+                        la_get<DT>(sp, la_unit(it, ks), lane, pf);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) la_mma(O[n][it], yf[n], pf);
+                    }
+            }
+            // lane: 4 NT neighbouring columns of token it * 16 + lane % 16
 #pragma unroll
             for (int it = 0; it < 4; ++it) {
-                const float w = gt.wq[it * 16 + (lane & 15)] * a.scale;
+                const int r = it * 16 + (lane & 15), d = dv0 + (lane >> 4) * 4 * NT;
+                if (r < rows && d < Dv) {
+                    if (r >= nv)
 #pragma unroll
-                for (int n = 0; n < NT; ++n) O[n][it] *= w;
+                        for (int n = 0; n < NT; ++n) O[n][it] = f32x4{0.f, 0.f, 0.f, 0.f};
+                    E* q = out + r * ot + d;
+                    if constexpr (NT == 2 && DT != 0) {
+                        if (p.vo && d + 8 <= Dv) {
+                            *(la_u32x4*)q = la_u32x4{v2a_pack_h2<DT == 2>(O[0][it][0], O[0][it][1]), v2a_pack_h2<DT == 2>(O[0][it][2], O[0][it][3]),
+                                                     v2a_pack_h2<DT == 2>(O[1][it][0], O[1][it][1]), v2a_pack_h2<DT == 2>(O[1][it][2], O[1][it][3])};
+                            continue;
+                        }
+                    }
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+                        if (d + n * 4 < Dv) la_store4<DT>(q + n * 4, O[n][it], Dv - d - n * 4, p.vo);
+                }
             }
-            __syncthreads();
+        } else {
+            fetch_x(i + 1);
+            fetch_y(i + 1);
+            gates(i + 1);
+            fetch_g(i + 2);
         }
-        __builtin_amdgcn_sched_barrier(0);
         const float tot = gt.total;
+        fac *= tot;
 #pragma unroll
         for (int d = 0; d < DK / 16; ++d)
 #pragma unroll
             for (int n = 0; n < NT; ++n) S[d][n] *= tot;
-        fac *= tot;
+        const int nku = keep ? nks : 0;
+#pragma unroll 1
+        for (int ks = 0; ks < nku; ++ks) {
+            typename LaOp<DT>::C3 yw[NT];
+            const float* wsrc = (p.rev ? gt.wq : gt.wk) + ks * 32 + (lane >> 4) * 4;
+            const float4 w0 = *(const float4*)wsrc, w1 = *(const float4*)(wsrc + 16);
+            const float sc = p.rev ? a.scale : 1.f;
+            const float w[8] = {w0.x * sc, w0.y * sc, w0.z * sc, w0.w * sc, w1.x * sc, w1.y * sc, w1.z * sc, w1.w * sc};
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
-            if (ks * 32 < nv) {
-                typename LaOp<DT>::In yf[NT];
-                typename LaOp<DT>::C3 yw[NT];
-                const float* wsrc = (p.rev ? gt.wq : gt.wk) + ks * 32 + (lane >> 4) * 4;
-                const float4 w0 = *(const float4*)wsrc, w1 = *(const float4*)(wsrc + 16);
-                const float sc = p.rev ? a.scale : 1.f;
-                const float w[8] = {w0.x * sc, w0.y * sc, w0.z * sc, w0.w * sc, w1.x * sc, w1.y * sc, w1.z * sc, w1.w * sc};
+            for (int n = 0; n < NT; ++n) {
+                typename LaOp<DT>::In yf;
+                TY::template tr<CS>(sy, ks, wid * NT * 16 + n * NC0, lane, yf);
+                float x[8];
+                la_join(yf, x);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] *= w[e];
+                la_split(x, yw[n]);
+            }
+#pragma unroll
+            for (int d = 0; d < DK / 16; ++d) {
+                typename LaOp<DT>::In xf;
+                if constexpr (OUT) TX::template tr<8>(sx, ks, d / 2 * 32 + d % 2 * 4, lane, xf);
+                else TX::template tr<4>(sx, ks, d * 16, lane, xf);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    TY::tr(sy, ks, (wid * NT + n) * 16, lane, yf[n]);
-                    float x[8];
-                    la_join(yf[n], x);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) x[e] *= w[e];
-                    la_split(x, yw[n]);
+                    if constexpr (OUT) la_mma(S[d][n], xf, yw[n]);
+                    else la_mma(S[d][n], yw[n], xf);
                 }
-                if constexpr (OUT) {
-#pragma unroll
-                    for (int u = 0; u < 6; ++u)
-                        if (la_unit_step(u) == ks && la_unit_tile(u) * 16 < nv) {
-                            typename LaOp<DT>::C2 pf;
-                            la_get<DT>(sp, u, lane, pf);
-#pragma unroll
-                            for (int n = 0; n < NT; ++n) la_mma(O[n][la_unit_tile(u)], yf[n], pf);
-                        }
-                    __builtin_amdgcn_sched_barrier(0);
-                }
-                if (keep)
-#pragma unroll
-                for (int d = 0; d < DK / 16; ++d) {
-                    typename LaOp<DT>::In xf;
-                    TX::tr(sx, ks, d * 16, lane, xf);
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) la_mma(S[d][n], xf, yw[n]);
-                    if (d & 1) __builtin_amdgcn_sched_barrier(0);
-                }
-            }
-        if constexpr (OUT) {
-#pragma unroll
-            for (int it = 0; it < 4; ++it) {
-                const int r = it * 16 + (lane & 15);
-                if (r < rows)
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        const int d = dv0 + n * 16 + (lane >> 4) * 4;
-                        if (d < Dv) la_store4<DT>(out + r * ot + d, r < nv ? O[n][it] : f32x4{0.f, 0.f, 0.f, 0.f}, Dv - d, p.vo);
-                    }
+                if (d & 1) __builtin_amdgcn_sched_barrier(0);
             }
         }
     }
+    for (int i = vend; i < iend; ++i) skip(i);
     if (p.local) {
         put_state(p.seg + ((long long)bh * p.nseg + seg) * SS);
         if (threadIdx.x == 0 && dvt == 0) p.seg_decay[(long long)bh * p.nseg + seg] = fac;
@@ -627,7 +746,7 @@ __global__ __launch_bounds__(4 * D) void la_bwd_chunk(LaArgs a, LaBwd p) {
         for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-                const int d = kk * 32 + half * 16 + l4;
+                const int d = kk * 32 + l4 * 2 + half * 4;
                 if (p.vst && d < Dv) *(float4*)&x[kk][half * 4] = *(const float4*)(q + d);
                 else
                     for (int e = 0; e < 4; ++e)
@@ -777,7 +896,7 @@ __global__ __launch_bounds__(4 * D) void la_bwd_chunk(LaArgs a, LaBwd p) {
         for (int ks = 0; ks < 2; ++ks)
             if (ks * 32 < nv) {
                 typename LaOp<DT>::In tf;
-                TT::tr(t, ks, w0, lane, tf);
+                TT::template tr<4>(t, ks, w0, lane, tf);
 #pragma unroll
                 for (int u = 0; u < 6; ++u) {
                     const int tile = mirrored ? 3 - la_unit_tile(u) : la_unit_tile(u);
@@ -827,7 +946,7 @@ __global__ __launch_bounds__(4 * D) void la_bwd_chunk(LaArgs a, LaBwd p) {
                 float x[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const int d = kk * 32 + (e < 4 ? e : 12 + e) + l4;
+                    const int d = kk * 32 + l4 * 2 + e;
                     x[e] = d < Dk && w0 + l16 < Dv ? Ep[(long long)d * Dv + w0 + l16] : 0.f;
                 }
                 typename LaOp<DT>::C2 ef;
@@ -1046,7 +1165,7 @@ template <int DT, int DK, bool OUT> int la_scan_dv(const LaArgs& a, const LaScan
     const dim3 grid((unsigned)((long long)a.B * a.H * p.ndv * p.nseg));
     if (dvt == 32) hipLaunchKernelGGL((la_scan<DT, DK, 1, 2, OUT>), grid, dim3(128), 0, s, a, p);
     else if (dvt == 64) hipLaunchKernelGGL((la_scan<DT, DK, 1, 4, OUT>), grid, dim3(256), 0, s, a, p);
-    else if constexpr (DK == 32) hipLaunchKernelGGL((la_scan<DT, DK, 2, 4, OUT>), grid, dim3(256), 0, s, a, p);
+    else if constexpr (DK == 32 || (OUT && DT == 1)) hipLaunchKernelGGL((la_scan<DT, DK, 2, 4, OUT>), grid, dim3(256), 0, s, a, p);
     else hipLaunchKernelGGL((la_scan<DT, DK, 1, 8, OUT>), grid, dim3(512), 0, s, a, p);
     V2A_CHECK_LAUNCH();
     return V2A_OK;
@@ -1060,6 +1179,7 @@ template <bool OUT> int la_launch_scan(const LaArgs& a, const LaScan& p, int dvt
 
 // A recurrence over the whole sequence: local states and their combination where there are segments, then the pass itself
 template <bool OUT> int la_recur(const LaArgs& a, LaScan p, const LaPlan& pl, int dtype, hipStream_t s) {
+    p.vst = a.Dv % 4 == 0 && (((uintptr_t)p.init | (uintptr_t)p.last) & 15) == 0;      // the workspace is aligned
     p.NC = pl.NC; p.cps = pl.cps; p.nseg = pl.nseg; p.ndv = pl.ndv;
     const long long SS = (long long)a.Dk * a.Dv;
     if (pl.nseg > 1) {
@@ -1128,7 +1248,7 @@ int v2a_linattn_fwd(const void* q, const void* k, const void* v, const float* g,
     p.vx = la_vec(k, a.ks, B, T, Hk, Dk, dtype);
     p.vy = la_vec(v, a.vs, B, T, Hv, Dv, dtype);
     p.vq = la_vec(q, a.qs, B, T, Hq, Dk, dtype);
-    p.vo = Dv % 4 == 0 && ((uintptr_t)out & 15) == 0;
+    p.vo = Dv % (dtype == 0 ? 4 : 8) == 0 && ((uintptr_t)out & 15) == 0;
     return la_recur<true>(a, p, pl, dtype, s);
 }
 
