@@ -669,122 +669,195 @@ __global__ __launch_bounds__(256) void la_combine(float* seg, const float* seg_d
 }
 
 struct LaBwd {
-    const float *s_chunk, *e_chunk;      // state before / gradient of the state behind each chunk, [B H][NC][Dk][Dv] (chunk 0 / NC - 1: the two below)
-    const float *s_first, *e_last;       // NULL: 0
+    const float* s_chunk;                // state before each chunk, [B H][NC][Dk][Dv] (chunk 0: s_first)
+    const float *s_first, *e_last;       // before the sequence / gradient of the state behind it; NULL: 0
+    const float* e_seg;                  // gradient of the state behind each segment, [B H][nseg][Dk][Dv], segments from the end (the last one: e_last)
+    float* e_first;                      // gradient of the state before the sequence; NULL: not wanted
     void *dq, *dk, *dv;                  // in the inputs' type, or fp32 per head where heads are shared
     float *dg, *dg_part;                 // per token, or the chunk's sum [NC][B H]
-    int NC, vq, vk, vv, vd, vst, fq, fk, fv;      // v: 16-byte loads allowed; f: fp32 per-head output
+    int NC, cps, nseg, vq, vk, vv, vd, vst, fq, fk, fv;      // v: 16-byte accesses allowed; f: fp32 per-head output
 };
 
-// One workgroup computes the gradients of one chunk of one (row, head):
+// One workgroup walks the chunks of one segment of one (row, head) from the last to the first, with the gradient E of the state behind the
+// chunk in accumulators:
 //   dq_i = s (exp(G_i) S do_i + sum_j W_ij (do_i . v_j) k_j)          R_i = q_i . (the first part)
 //   dk_j = exp(G_64 - G_j) E v_j + s sum_i W_ij (do_i . v_j) q_i      C_j = k_j . (the first part)
 //   dv_j = exp(G_64 - G_j) E^T k_j + s sum_i W_ij (q_i . k_j) do_i
 //   dg_t = exp(G_64) <S, E> + sum_{i >= t} (R_i + r_i - c_i) + sum_{j < t} C_j,   r_i = sum_{j < i} M_ij, c_j = sum_{i > j} M_ij,
-//          M_ij = s W_ij (q_i . k_j)(do_i . v_j): everything whose path crosses the decay of token t.
-// Wave w owns rows 16 w .. of dq^T, dk^T (and of S, E) and dv^T.  Scores are computed once, by units, and shared through LDS.
+//          M_ij = s W_ij (q_i . k_j)(do_i . v_j): everything whose path crosses the decay of token t,
+//   E <- exp(G_64) E + s sum_i exp(G_i) q_i do_i^T.
+// dg is summed from these parts, not from <q, dq> - <k, dk> over the sequence, whose difference of long sums would lose what it is after.
+// Wave w owns rows 16 w .. of S, E, dq^T, dk^T and columns 16 w .. of dv^T; as dk contracts E over its columns and dv over its rows, E is
+// kept twice, by rows and by columns, which costs 48 more MFMA per wave and chunk but no exchange.  Scores are computed once, by units, and
+// shared through LDS; the next chunk's rows are on their way meanwhile.
 template <int DT, int D>
-__global__ __launch_bounds__(4 * D) void la_bwd_chunk(LaArgs a, LaBwd p) {
+__global__ __launch_bounds__(4 * D) void la_bwd_chunks(LaArgs a, LaBwd p) {
     typedef typename LaT<DT>::T E;
     typedef LaTile<DT, D> TT;
     constexpr int NW = D / 16, NTH = 64 * NW, KK = D / 32;
     constexpr int UB = 6 * la_unit_bytes<DT>();
-    constexpr int NBUF = 4 * TT::BYTES + 3 * UB + 8192 <= 160 * 1024 ? 3 : 1;      // score buffers: all three at once where they fit
+    constexpr int NBUF = 4 * TT::BYTES + 3 * UB + 10240 <= 160 * 1024 ? 3 : 1;      // score buffers: all three at once where they fit
     __shared__ __attribute__((aligned(16))) char sm[4 * TT::BYTES + NBUF * UB];
-    __shared__ __attribute__((aligned(16))) LaGate gt;
+    __shared__ __attribute__((aligned(16))) LaGate gts[2];
     __shared__ float sr[NW][LA_C], sc[NW][LA_C], rm[4][LA_C], cm[2][LA_C], sz[NW];
     char *sq = sm, *sk = sq + TT::BYTES, *sv = sk + TT::BYTES, *sd = sv + TT::BYTES, *s1 = sd + TT::BYTES;
     char *s2 = s1 + (NBUF == 3 ? UB : 0), *s3 = s2 + (NBUF == 3 ? UB : 0);
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l16 = lane & 15, l4 = (lane >> 4) * 4;
-    const int c = blockIdx.x % p.NC, bh = blockIdx.x / p.NC, b = bh / a.H, h = bh % a.H;
+    const int seg = blockIdx.x % p.nseg, bh = blockIdx.x / p.nseg, b = bh / a.H, h = bh % a.H;
     const int Dk = a.Dk, Dv = a.Dv, w0 = wid * 16;
     const int hq = h / (a.H / a.Hq), hk = h / (a.H / a.Hk), hv = h / (a.H / a.Hv);
-    const long long t0 = (long long)c * LA_C, SS = (long long)Dk * Dv;
-    const int rows = a.T - (int)t0 < LA_C ? a.T - (int)t0 : LA_C;
-    int nv = la_len(a, b) - (int)t0;
-    nv = nv < 0 ? 0 : nv > LA_C ? LA_C : nv;
+    const long long SS = (long long)Dk * Dv;
+    const int len = la_len(a, b);
+    const E* Q = (const E*)a.q + b * a.qs[0] + hq * a.qs[2];
+    const E* K = (const E*)a.k + b * a.ks[0] + hk * a.ks[2];
+    const E* V = (const E*)a.v + b * a.vs[0] + hv * a.vs[2];
+    const E* G = (const E*)a.dout + b * a.ds[0] + h * a.ds[2];
+    const float* g = a.g + b * a.gs[0] + h * a.gs[2];
 
     // one row of four values of a gradient: shared heads keep fp32 per head (rows of H heads), others their own type
-    auto put = [&](void* base, int f32, int Hx, int hx, int Dx, int row, int d, const f32x4& x) {
-        if (d >= Dx || row >= rows) return;
-        if (f32) la_store4<0>((float*)base + (((long long)b * a.T + t0 + row) * a.H + h) * Dx + d, x, Dx - d, Dx % 4 == 0);
-        else la_store4<DT>((E*)base + (((long long)b * a.T + t0 + row) * Hx + hx) * Dx + d, x, Dx - d, Dx % 4 == 0);
+    auto put = [&](void* base, int f32, int Hx, int hx, int Dx, int c, int row, int d, const f32x4& x) __attribute__((always_inline)) {
+        const long long t = (long long)c * LA_C + row;
+        if (d >= Dx || t >= a.T) return;
+        if (f32) la_store4<0>((float*)base + (((long long)b * a.T + t) * a.H + h) * Dx + d, x, Dx - d, Dx % 4 == 0);
+        else la_store4<DT>((E*)base + (((long long)b * a.T + t) * Hx + hx) * Dx + d, x, Dx - d, Dx % 4 == 0);
     };
-    if (nv == 0) {
+    // this segment's chunks chi, chi - 1, .. clo; those from nvc on have no tokens
+    const int chi = p.NC - 1 - seg * p.cps, clo = chi - p.cps + 1 > 0 ? chi - p.cps + 1 : 0;
+    const int nvc = (len + LA_C - 1) / LA_C, cfirst = chi < nvc ? chi : nvc - 1;
+    for (int c = chi; c > cfirst && c >= clo; --c) {
         const f32x4 z = {0.f, 0.f, 0.f, 0.f};
-        for (int r = l16; r < rows; r += 16) {
-            put(p.dq, p.fq, a.Hq, hq, Dk, r, w0 + l4, z);
-            put(p.dk, p.fk, a.Hk, hk, Dk, r, w0 + l4, z);
-            put(p.dv, p.fv, a.Hv, hv, Dv, r, w0 + l4, z);
+        for (int r = l16; r < LA_C; r += 16) {
+            put(p.dq, p.fq, a.Hq, hq, Dk, c, r, w0 + l4, z);
+            put(p.dk, p.fk, a.Hk, hk, Dk, c, r, w0 + l4, z);
+            put(p.dv, p.fv, a.Hv, hv, Dv, c, r, w0 + l4, z);
         }
-        if (wid == 0 && p.dg && lane < rows) p.dg[((long long)b * a.T + t0 + lane) * a.H + h] = 0.f;
+        if (wid == 0 && p.dg && c * LA_C + lane < a.T) p.dg[((long long)b * a.T + (long long)c * LA_C + lane) * a.H + h] = 0.f;
         if (threadIdx.x == 0 && p.dg_part) p.dg_part[(long long)c * a.B * a.H + bh] = 0.f;
-        return;
     }
-    const E* Q = (const E*)a.q + b * a.qs[0] + t0 * a.qs[1] + hq * a.qs[2];
-    const E* K = (const E*)a.k + b * a.ks[0] + t0 * a.ks[1] + hk * a.ks[2];
-    const E* V = (const E*)a.v + b * a.vs[0] + t0 * a.vs[1] + hv * a.vs[2];
-    const E* G = (const E*)a.dout + b * a.ds[0] + t0 * a.ds[1] + h * a.ds[2];
-    const float* Sp = c == 0 ? (p.s_first ? p.s_first + bh * SS : nullptr) : p.s_chunk + ((long long)bh * p.NC + c) * SS;
-    const float* Ep = c == p.NC - 1 ? (p.e_last ? p.e_last + bh * SS : nullptr) : p.e_chunk + ((long long)bh * p.NC + c) * SS;
-    LaLoad<DT, D, NTH> rq, rk, rv, rd;
-    rq.load(Q, a.qs[1], nv, Dk, p.vq);
-    rk.load(K, a.ks[1], nv, Dk, p.vk);
-    rv.load(V, a.vs[1], nv, Dv, p.vv);
-    rd.load(G, a.ds[1], nv, Dv, p.vd);
-    const float rg = wid == 0 && lane < nv ? a.g[b * a.gs[0] + (t0 + lane) * a.gs[1] + h * a.gs[2]] : 0.f;
-    // rows w0 + l16 of S and E, in slot order along Dv
-    auto state_rows = [&](const float* st, float (&x)[KK][8]) {
+
+    // E by rows: e1[kk][half][r] is row w0 + l16, column 32 kk + 8 (lane / 16) + 4 half + r; by columns: e2, row and column exchanged
+    f32x4 e1[KK][2], e2[KK][2];
 #pragma unroll
-        for (int kk = 0; kk < KK; ++kk)
+    for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[kk][e] = 0.f;
-        if (!st || w0 + l16 >= Dk) return;
-        const float* q = st + (long long)(w0 + l16) * Dv;
+        for (int half = 0; half < 2; ++half) e1[kk][half] = e2[kk][half] = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto state_rows = [&](const float* st, f32x4 (&x)[KK][2]) __attribute__((always_inline)) {      // zeros where there is no value
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
                 const int d = kk * 32 + l4 * 2 + half * 4;
-                if (p.vst && d < Dv) *(float4*)&x[kk][half * 4] = *(const float4*)(q + d);
-                else
-                    for (int e = 0; e < 4; ++e)
-                        if (d + e < Dv) x[kk][half * 4 + e] = q[d + e];
+                x[kk][half] = f32x4{0.f, 0.f, 0.f, 0.f};
+                if (st && w0 + l16 < Dk && d < Dv) {
+                    const float* q = st + (w0 + l16) * Dv + d;
+                    if (p.vst) x[kk][half] = *(const f32x4*)q;
+                    else
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) x[kk][half][r] = d + r < Dv ? q[r] : 0.f;
+                }
             }
     };
-    float xs[KK][8], xe[KK][8];
-    state_rows(Sp, xs);
-    state_rows(Ep, xe);
-    rq.store(sq);
-    rk.store(sk);
-    rv.store(sv);
-    rd.store(sd);
-    if (wid == 0) la_gates(gt, rg, lane < nv, lane);
-    for (int e = threadIdx.x; e < 4 * LA_C; e += NTH) rm[0][e] = 0.f;
-    for (int e = threadIdx.x; e < 2 * LA_C; e += NTH) cm[0][e] = 0.f;
-    {
-        float z = 0.f;
+    const float* ep = seg ? p.e_seg + ((long long)bh * p.nseg + seg) * SS : p.e_last ? p.e_last + bh * SS : nullptr;
+    bool have_e = ep != nullptr;
+    if (ep) {
+        state_rows(ep, e1);
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) z += xs[kk][e] * xe[kk][e];
-        z = wave_sum(z);
-        if (lane == 0) sz[wid] = z;
-    }
-    __syncthreads();
-
-    // W (do . v) with lane = i, slots = j: the operand of dq
-    auto unit1 = [&]() {
+            for (int half = 0; half < 2; ++half)
 #pragma unroll
-        for (int u = 0; u < 6; ++u) {
-            const int it = la_unit_tile(u), js = la_unit_step(u) * 32;
-            if ((NBUF == 3 && NW == 8 ? 6 + u / 3 : la_unit_wave(u, NW)) != wid || it * 16 >= nv) continue;
-            f32x4 c0 = {0.f, 0.f, 0.f, 0.f}, c1 = {0.f, 0.f, 0.f, 0.f};
-            const bool two = js + 16 <= it * 16;
+                for (int r = 0; r < 4; ++r) {
+                    const int d = kk * 32 + l4 * 2 + half * 4 + r, c = w0 + l16;
+                    const float x = ep[(d < Dk ? d : 0) * Dv + (c < Dv ? c : 0)];
+                    e2[kk][half][r] = d < Dk && c < Dv ? x : 0.f;
+                }
+    }
+    LaLoad<DT, D, NTH> rq, rk, rv, rd;
+    float rg = 0.f, rgn = 0.f;      // this chunk's and the next one's decays, in the first / last wave
+    auto valid = [&](int c) { return len - c * LA_C < LA_C ? len - c * LA_C : LA_C; };
+    auto fetch = [&](int c) __attribute__((always_inline)) {
+        if (c < clo) return;
+        const long long t0 = (long long)c * LA_C;
+        const int nv = valid(c);
+        rq.load(Q + t0 * a.qs[1], a.qs[1], nv, Dk, p.vq);
+        rk.load(K + t0 * a.ks[1], a.ks[1], nv, Dk, p.vk);
+        rv.load(V + t0 * a.vs[1], a.vs[1], nv, Dv, p.vv);
+        rd.load(G + t0 * a.ds[1], a.ds[1], nv, Dv, p.vd);
+    };
+    auto fetch_g = [&](int c) { if (wid == NW - 1 && c >= clo && lane < valid(c)) rgn = g[((long long)c * LA_C + lane) * a.gs[1]]; };
+    auto gates = [&](int c) { if (wid == NW - 1 && c >= clo) la_gates(gts[c & 1], rgn, lane < valid(c), lane); };
+    auto state_of = [&](int c) { return c == 0 ? (p.s_first ? p.s_first + bh * SS : nullptr) : p.s_chunk + ((long long)bh * p.NC + c) * SS; };
+    f32x4 xs[KK][2];
+    if (cfirst >= clo) {
+        fetch_g(cfirst);
+        fetch(cfirst);
+        state_rows(state_of(cfirst), xs);
+        gates(cfirst);
+        fetch_g(cfirst - 1);
+    }
+    f32x4 acc[4];
+    float raw[3][8];
+    // d decay of the chunk whose parts are in LDS (first wave, lane = token)
+    auto decays = [&](int c) __attribute__((always_inline)) {
+        const int nv = valid(c);
+        double up = 0.0, down = 0.0, z = 0.0;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+            up += sr[w][lane];
+            down += sc[w][lane];
+            z += sz[w];
+        }
+        // parts that no unit of the lower triangle wrote are left out
+#pragma unroll
+        for (int jt = 0; jt < 4; ++jt)
+            if (lane >= jt * 16) up += rm[jt][lane];
+        if (lane < 32) up -= cm[0][lane];
+        if (nv > 32) up -= cm[1][lane];
+        if (lane >= nv) up = down = 0.0;
+        const double down_to = la_running(down, lane) - down, all = la_running(up, lane), up_from = la_lane(all, 63) - all + up;
+        const float gg = lane < nv ? g[((long long)c * LA_C + lane) * a.gs[1]] : 0.f;
+        const bool gone = __builtin_amdgcn_exp2f(la_clampg(gg) * LA_LOG2E) == 0.f;
+        double d = z * (double)gts[c & 1].total + up_from + down_to;
+        if (gone || lane >= nv) d = 0.0;
+        const long long t = (long long)c * LA_C + lane;
+        if (p.dg && t < a.T) p.dg[((long long)b * a.T + t) * a.H + h] = (float)d;
+        if (p.dg_part) {
+            d = wave_sum_d(d);
+            if (lane == 0) p.dg_part[(long long)c * a.B * a.H + bh] = (float)d;
+        }
+    };
+    for (int c = cfirst; c >= clo; --c) {
+        const int nv = valid(c);
+        const LaGate& gt = gts[c & 1];
+        __syncthreads();
+        rq.store(sq);
+        rk.store(sk);
+        rv.store(sv);
+        rd.store(sd);
+        if (wid == 0 && c < cfirst) decays(c + 1);
+        __syncthreads();
+        {
+            float z = 0.f;
 #pragma unroll
             for (int kk = 0; kk < KK; ++kk)
-                if (kk * 32 < Dv) {
+#pragma unroll
+                for (int half = 0; half < 2; ++half)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) z += xs[kk][half][r] * e1[kk][half][r];
+            z = wave_sum(z);
+            if (lane == 0) sz[wid] = z;
+        }
+        // W (do . v) with lane = i, slots = j: the operand of dq
+        auto unit1 = [&]() __attribute__((always_inline)) {
+#pragma unroll
+            for (int u = 0; u < 6; ++u) {
+                const int it = la_unit_tile(u), js = la_unit_step(u) * 32;
+                if ((NBUF == 3 && NW == 8 ? 6 + u / 3 : la_unit_wave(u, NW)) != wid || it * 16 >= nv) continue;
+                f32x4 c0 = {0.f, 0.f, 0.f, 0.f}, c1 = {0.f, 0.f, 0.f, 0.f};
+                const bool two = js + 16 <= it * 16;
+#pragma unroll 2
+                for (int kk = 0; kk < KK; ++kk) {
                     typename LaOp<DT>::In df, vf;
                     TT::nat(sd, it * 16, kk, lane, df);
                     TT::nat(sv, js, kk, lane, vf);
@@ -794,31 +867,29 @@ __global__ __launch_bounds__(4 * D) void la_bwd_chunk(LaArgs a, LaBwd p) {
                         la_mma_in<DT>(c1, vf, df);
                     }
                 }
-            float w[8], x[8];
-            la_weights<false>(gt, js, it * 16 + l16, lane, w);
-            la_weights<false>(gt, js + 16, it * 16 + l16, lane, w + 4);
+                float w[8], x[8];
+                la_weights<false>(gt, js, it * 16 + l16, lane, w);
+                la_weights<false>(gt, js + 16, it * 16 + l16, lane, w + 4);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                x[r] = c0[r] * w[r] * a.scale;
-                x[4 + r] = c1[r] * w[4 + r] * a.scale;
+                for (int r = 0; r < 4; ++r) {
+                    x[r] = c0[r] * w[r] * a.scale;
+                    x[4 + r] = c1[r] * w[4 + r] * a.scale;
+                }
+                la_put<DT>(s1, u, lane, x);
             }
-            la_put<DT>(s1, u, lane, x);
-        }
-    };
-    // W (x . y) with lane = j, slots = i: the operands of dk (x = do, y = v) and dv (x = q, y = k); unit u is tile 3 - tile(u), step 1 - step(u)
-    float raw[3][8];
-    auto unit23 = [&](const char* sx, const char* sy, char* dst, int Dx, bool third) {
+        };
+        // W (x . y) with lane = j, slots = i: the operands of dk (x = do, y = v) and dv (x = q, y = k); unit u is tile 3 - tile(u), step 1 - step(u)
+        auto unit23 = [&](const char* sx, const char* sy, char* dst, bool third) __attribute__((always_inline)) {
 #pragma unroll
-        for (int u = 0; u < 6; ++u) {
-            const int jt = 3 - la_unit_tile(u), is = 32 - la_unit_step(u) * 32;
-            constexpr int per = NW == 8 ? 1 : NW == 4 ? 2 : 3;
-            const int at = u % per;
-            if (la_unit_wave(u, NW) != wid || jt * 16 >= nv || is >= nv) continue;
-            f32x4 c0 = {0.f, 0.f, 0.f, 0.f}, c1 = {0.f, 0.f, 0.f, 0.f};
-            const bool first = is + 16 > jt * 16;
-#pragma unroll
-            for (int kk = 0; kk < KK; ++kk)
-                if (kk * 32 < Dx) {
+            for (int u = 0; u < 6; ++u) {
+                const int jt = 3 - la_unit_tile(u), is = 32 - la_unit_step(u) * 32;
+                constexpr int per = NW == 8 ? 1 : NW == 4 ? 2 : 3;
+                const int at = u % per;
+                if (la_unit_wave(u, NW) != wid || jt * 16 >= nv || is >= nv) continue;
+                f32x4 c0 = {0.f, 0.f, 0.f, 0.f}, c1 = {0.f, 0.f, 0.f, 0.f};
+                const bool first = is + 16 > jt * 16;
+#pragma unroll 2
+                for (int kk = 0; kk < KK; ++kk) {
                     typename LaOp<DT>::In xf, yf;
                     TT::nat(sy, jt * 16, kk, lane, yf);
                     if (first) {
@@ -828,168 +899,184 @@ __global__ __launch_bounds__(4 * D) void la_bwd_chunk(LaArgs a, LaBwd p) {
                     TT::nat(sx, is + 16, kk, lane, xf);
                     la_mma_in<DT>(c1, xf, yf);
                 }
-            float w[8], x[8];
-            const int j = jt * 16 + l16;
-            la_weights<true>(gt, is, j, lane, w);
-            la_weights<true>(gt, is + 16, j, lane, w + 4);
+                float w[8], x[8];
+                const int j = jt * 16 + l16;
+                la_weights<true>(gt, is, j, lane, w);
+                la_weights<true>(gt, is + 16, j, lane, w + 4);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                x[r] = c0[r] * w[r] * a.scale;
-                x[4 + r] = c1[r] * w[4 + r] * a.scale;
-            }
-            la_put<DT>(dst, u, lane, x);
-            if (!third) {
-#pragma unroll
-                for (int r = 0; r < 4; ++r) { raw[at][r] = c0[r]; raw[at][4 + r] = c1[r]; }
-            } else {
-                float col = 0.f;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int i = is + (e < 4 ? e : 12 + e) + l4;
-                    float m = i > j ? x[e] * raw[at][e] : 0.f;
-                    col += m;
-                    m += v2a_dpp<0xB1>(m);              // sum over the 16 lanes of a row group
-                    m += v2a_dpp<0x4E>(m);
-                    m += v2a_dpp<0x141>(m);
-                    m += v2a_dpp<0x140>(m);
-                    if (l16 == 0) rm[jt][i] = m;
+                for (int r = 0; r < 4; ++r) {
+                    x[r] = c0[r] * w[r] * a.scale;
+                    x[4 + r] = c1[r] * w[4 + r] * a.scale;
                 }
-                col += __shfl_xor(col, 16, 64);
-                col += __shfl_xor(col, 32, 64);
-                if (lane < 16) cm[is >> 5][j] = col;
+                la_put<DT>(dst, u, lane, x);
+                if (!third) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) { raw[at][r] = c0[r]; raw[at][4 + r] = c1[r]; }
+                } else {
+                    float col = 0.f;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const int i = is + (e < 4 ? e : 12 + e) + l4;
+                        float m = i > j ? x[e] * raw[at][e] : 0.f;
+                        col += m;
+                        m += v2a_dpp<0xB1>(m);              // sum over the 16 lanes of a row group
+                        m += v2a_dpp<0x4E>(m);
+                        m += v2a_dpp<0x141>(m);
+                        m += v2a_dpp<0x140>(m);
+                        if (l16 == 0) rm[jt][i] = m;
+                    }
+                    col += __shfl_xor(col, 16, 64);
+                    col += __shfl_xor(col, 32, 64);
+                    if (lane < 16) cm[is >> 5][j] = col;
+                }
             }
-        }
-    };
-    f32x4 acc[4];
-    auto clear = [&]() {
+        };
+        auto clear = [&]() __attribute__((always_inline)) {
 #pragma unroll
-        for (int t = 0; t < 4; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    };
-    // the part through the state: rows of `st` times the tokens' rows in `t`, weighted by w, and its product with the tokens' own rows in `own`
-    auto through_state = [&](const float (&x)[KK][8], const char* t, const float* w, float mul, const char* own, float* dst) {
+            for (int t = 0; t < 4; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        };
+        // a state's rows (or columns) times the tokens' rows in `t`, weighted by w
+        auto through = [&](const f32x4 (&x)[KK][2], const char* t, const float* w, float mul) __attribute__((always_inline)) {
 #pragma unroll
-        for (int kk = 0; kk < KK; ++kk)
-            if (kk * 32 < Dv) {
+            for (int kk = 0; kk < KK; ++kk) {
+                float y[8];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) { y[r] = x[kk][0][r]; y[4 + r] = x[kk][1][r]; }
                 typename LaOp<DT>::C2 sf;
-                la_split(x[kk], sf);
+                la_split(y, sf);
 #pragma unroll
                 for (int tt = 0; tt < 4; ++tt) {
                     typename LaOp<DT>::In tf;
                     TT::nat(t, tt * 16, kk, lane, tf);
                     la_mma(acc[tt], sf, tf);
                 }
+                __builtin_amdgcn_sched_barrier(0);
             }
 #pragma unroll
-        for (int tt = 0; tt < 4; ++tt) {
-            acc[tt] *= w[tt * 16 + l16] * mul;
-            float y[4];
-            TT::four(own, tt * 16 + l16, w0 + l4, y);
-            float s = (acc[tt][0] * y[0] + acc[tt][1] * y[1]) + (acc[tt][2] * y[2] + acc[tt][3] * y[3]);
-            s += __shfl_xor(s, 16, 64);
-            s += __shfl_xor(s, 32, 64);
-            if (lane < 16) dst[tt * 16 + lane] = s;
-        }
-    };
-    // the part within the chunk: columns w0 .. of the tokens in `t` times the shared scores
-    auto within = [&](const char* t, const char* units, bool mirrored) {
+            for (int tt = 0; tt < 4; ++tt) acc[tt] *= w[tt * 16 + l16] * mul;
+        };
+        // and its product with the tokens' own rows: this wave's share
+        auto with_own = [&](const char* own, float* dst) __attribute__((always_inline)) {
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
-            if (ks * 32 < nv) {
-                typename LaOp<DT>::In tf;
-                TT::template tr<4>(t, ks, w0, lane, tf);
+            for (int tt = 0; tt < 4; ++tt) {
+                float y[4];
+                TT::four(own, tt * 16 + l16, w0 + l4, y);
+                float s = (acc[tt][0] * y[0] + acc[tt][1] * y[1]) + (acc[tt][2] * y[2] + acc[tt][3] * y[3]);
+                s += __shfl_xor(s, 16, 64);
+                s += __shfl_xor(s, 32, 64);
+                if (lane < 16) dst[tt * 16 + lane] = s;
+            }
+        };
+        // the part within the chunk: columns w0 .. of the tokens in `t` times the shared scores
+        auto within = [&](const char* t, const char* units, bool mirrored) __attribute__((always_inline)) {
 #pragma unroll
-                for (int u = 0; u < 6; ++u) {
-                    const int tile = mirrored ? 3 - la_unit_tile(u) : la_unit_tile(u);
-                    if ((mirrored ? 1 - la_unit_step(u) : la_unit_step(u)) != ks || tile * 16 >= nv) continue;
-                    typename LaOp<DT>::C2 xf;
-                    la_get<DT>(units, u, lane, xf);
-                    la_mma(acc[tile], tf, xf);
+            for (int ks = 0; ks < 2; ++ks)
+                if (ks * 32 < nv) {
+                    typename LaOp<DT>::In tf;
+                    TT::template tr<4>(t, ks, w0, lane, tf);
+#pragma unroll
+                    for (int u = 0; u < 6; ++u) {
+                        const int tile = mirrored ? 3 - la_unit_tile(u) : la_unit_tile(u);
+                        if ((mirrored ? 1 - la_unit_step(u) : la_unit_step(u)) != ks || tile * 16 >= nv) continue;
+                        typename LaOp<DT>::C2 xf;
+                        la_get<DT>(units, u, lane, xf);
+                        la_mma(acc[tile], tf, xf);
+                    }
                 }
-            }
-    };
-    auto emit = [&](void* base, int f32, int Hx, int hx, int Dx) {
+        };
+        auto emit = [&](void* base, int f32, int Hx, int hx, int Dx) __attribute__((always_inline)) {
 #pragma unroll
-        for (int tt = 0; tt < 4; ++tt) {
-            const int r = tt * 16 + l16;
-            put(base, f32, Hx, hx, Dx, r, w0 + l4, r < nv ? acc[tt] : f32x4{0.f, 0.f, 0.f, 0.f});
+            for (int tt = 0; tt < 4; ++tt) {
+                const int r = tt * 16 + l16;
+                put(base, f32, Hx, hx, Dx, c, r, w0 + l4, r < nv ? acc[tt] : f32x4{0.f, 0.f, 0.f, 0.f});
+            }
+        };
+        const float* sp = state_of(c);
+        unit1();
+        if constexpr (NBUF == 3) {
+            unit23(sd, sv, s2, false);
+            unit23(sq, sk, s3, true);
         }
-    };
-    unit1();
-    if constexpr (NBUF == 3) {
-        unit23(sd, sv, s2, Dv, false);
-        unit23(sq, sk, s3, Dk, true);
-    }
-    __syncthreads();
-    clear();
-    through_state(xs, sd, gt.wq, a.scale, sq, sr[wid]);
-    within(sk, s1, false);
-    emit(p.dq, p.fq, a.Hq, hq, Dk);
-    if constexpr (NBUF == 1) {
         __syncthreads();
-        unit23(sd, sv, s2, Dv, false);
-        __syncthreads();
-    }
-    clear();
-    through_state(xe, sv, gt.wk, 1.f, sk, sc[wid]);
-    within(sq, s2, true);
-    emit(p.dk, p.fk, a.Hk, hk, Dk);
-    if constexpr (NBUF == 1) {
-        __syncthreads();
-        unit23(sq, sk, s3, Dk, true);
-        __syncthreads();
-    }
-    clear();
-    if (Ep) {
+        fetch(c - 1);
+        clear();
+        if (sp) through(xs, sd, gt.wq, a.scale);
+        with_own(sq, sr[wid]);
+        within(sk, s1, false);
+        emit(p.dq, p.fq, a.Hq, hq, Dk);
+        if (c > clo) state_rows(state_of(c - 1), xs);
+        gates(c - 1);
+        fetch_g(c - 2);
+        if constexpr (NBUF == 1) {
+            __syncthreads();
+            unit23(sd, sv, s2, false);
+            __syncthreads();
+        }
+        clear();
+        if (have_e) through(e1, sv, gt.wk, 1.f);
+        with_own(sk, sc[wid]);
+        within(sq, s2, true);
+        emit(p.dk, p.fk, a.Hk, hk, Dk);
+        if constexpr (NBUF == 1) {
+            __syncthreads();
+            unit23(sq, sk, s3, true);
+            __syncthreads();
+        }
+        clear();
+        if (have_e) through(e2, sk, gt.wk, 1.f);
+        within(sd, s3, true);
+        emit(p.dv, p.fv, a.Hv, hv, Dv);
+        // E of the chunk before, if anybody reads it (a loop of no rounds, not a branch: the accumulators keep one definition)
+        const int nks = c > clo || p.e_first ? (nv > 32 ? 2 : 1) : 0;
+        have_e = true;
+        const float tot = gt.total;
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk)
-            if (kk * 32 < Dk) {
-                float x[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int d = kk * 32 + l4 * 2 + e;
-                    x[e] = d < Dk && w0 + l16 < Dv ? Ep[(long long)d * Dv + w0 + l16] : 0.f;
-                }
-                typename LaOp<DT>::C2 ef;
-                la_split(x, ef);
-#pragma unroll
-                for (int tt = 0; tt < 4; ++tt) {
-                    typename LaOp<DT>::In kf;
-                    TT::nat(sk, tt * 16, kk, lane, kf);
-                    la_mma(acc[tt], ef, kf);
-                }
+            for (int half = 0; half < 2; ++half) {
+                e1[kk][half] *= tot;
+                e2[kk][half] *= tot;
             }
+#pragma unroll 1
+        for (int ks = 0; ks < nks; ++ks) {
+            const float* wsrc = gt.wq + ks * 32 + l4;
+            const float4 wa = *(const float4*)wsrc, wb = *(const float4*)(wsrc + 16);
+            const float w[8] = {wa.x * a.scale, wa.y * a.scale, wa.z * a.scale, wa.w * a.scale,
+                                wb.x * a.scale, wb.y * a.scale, wb.z * a.scale, wb.w * a.scale};
+            auto weighted = [&](const typename LaOp<DT>::In& f, typename LaOp<DT>::C3& o) __attribute__((always_inline)) {
+                float x[8];
+                la_join(f, x);
 #pragma unroll
-        for (int tt = 0; tt < 4; ++tt) acc[tt] *= gt.wk[tt * 16 + l16];
+                for (int e = 0; e < 8; ++e) x[e] *= w[e];
+                la_split(x, o);
+            };
+            typename LaOp<DT>::In qf, df;
+            typename LaOp<DT>::C3 qw, dw;
+            TT::template tr<4>(sq, ks, w0, lane, qf);
+            TT::template tr<4>(sd, ks, w0, lane, df);
+            weighted(qf, qw);
+            weighted(df, dw);
+#pragma unroll
+            for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    TT::template tr<8>(sd, ks, kk * 32 + half * 4, lane, df);
+                    la_mma(e1[kk][half], df, qw);
+                    TT::template tr<8>(sq, ks, kk * 32 + half * 4, lane, qf);
+                    la_mma(e2[kk][half], qf, dw);
+                }
+        }
     }
-    within(sd, s3, true);
-    emit(p.dv, p.fv, a.Hv, hv, Dv);
     __syncthreads();
-    if (wid == 0) {
-        double up = 0.0, down = 0.0, z = 0.0;
+    if (wid == 0 && cfirst >= clo) decays(clo);
+    if (p.e_first && clo == 0 && w0 + l16 < Dk)
 #pragma unroll
-        for (int w = 0; w < NW; ++w) {
-            up += sr[w][lane];
-            down += sc[w][lane];
-            z += sz[w];
-        }
-        up += (double)((rm[0][lane] + rm[1][lane]) + (rm[2][lane] + rm[3][lane])) - (double)(cm[0][lane] + cm[1][lane]);
-        if (lane >= nv) up = down = 0.0;
-        const double own = down;
+        for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const double x = __shfl_down(up, o, 64), y = __shfl_up(down, o, 64);
-            if (lane + o < 64) up += x;
-            if (lane >= o) down += y;
-        }
-        const bool gone = __builtin_amdgcn_exp2f(la_clampg(rg) * LA_LOG2E) == 0.f;
-        double d = z * (double)gt.total + up + (down - own);
-        if (gone || lane >= nv) d = 0.0;
-        if (p.dg && lane < rows) p.dg[((long long)b * a.T + t0 + lane) * a.H + h] = (float)d;
-        if (p.dg_part) {
-            d = wave_sum_d(d);
-            if (lane == 0) p.dg_part[(long long)c * a.B * a.H + bh] = (float)d;
-        }
-    }
+            for (int half = 0; half < 2; ++half) {
+                const int d = kk * 32 + l4 * 2 + half * 4;
+                if (d < Dv) la_store4<0>(p.e_first + bh * SS + (w0 + l16) * Dv + d, e1[kk][half], Dv - d, p.vst);
+            }
 }
 
 // gradients of shared heads: the heads of a group summed in order, rounded once
@@ -1134,11 +1221,11 @@ size_t la_up(size_t n) { return (n + 255) & ~(size_t)255; }
     } while (0)
 
 // How a call is cut: columns of the state per workgroup (dvt) and segments of the sequence.  One workgroup per CU and more keep the chip busy;
-// where (row, head) pairs and column tiles are fewer, the chunks are cut into segments of at least four, whose states come from a first pass.
+// where (row, head) pairs and column tiles are fewer, the chunks are cut into segments of at least `least`, whose states come from a first pass.
 struct LaPlan {
     int dvt, ndv, NC, cps, nseg;
 };
-LaPlan la_plan(int BH, int T, int Dv) {
+LaPlan la_plan(int BH, int T, int Dv, int target, int least) {
     LaPlan p;
     p.dvt = Dv <= 32 ? 32 : Dv <= 64 ? 64 : 128;
     p.ndv = cdiv(Dv, p.dvt);
@@ -1146,14 +1233,15 @@ LaPlan la_plan(int BH, int T, int Dv) {
     p.nseg = 1;
     p.cps = p.NC;
     const long wg = (long)BH * p.ndv;
-    if (p.NC >= 8 && wg < 512) {
-        const int want = cdiv(512, wg);
-        p.cps = cdiv(p.NC, want);
-        if (p.cps < 4) p.cps = 4;
+    if (p.NC >= 2 * least && wg < target) {
+        p.cps = cdiv(p.NC, cdiv(target, wg));
+        if (p.cps < least) p.cps = least;
         p.nseg = cdiv(p.NC, p.cps);
     }
     return p;
 }
+LaPlan la_plan_fwd(int BH, int T, int Dv) { return la_plan(BH, T, Dv, 512, 2); }
+LaPlan la_plan_bwd(int BH, int T, int Dv) { return la_plan(BH, T, Dv, 512, 2); }
 
 int la_vec(const void* p, const long long* st, int B, int T, int H, int D, int dtype) {
     const long long es = dtype == 0 ? 4 : 2;
@@ -1177,18 +1265,25 @@ template <bool OUT> int la_launch_scan(const LaArgs& a, const LaScan& p, int dvt
     return dtype == 0 ? la_scan_dk<0, OUT>(a, p, dvt, s) : dtype == 1 ? la_scan_dk<1, OUT>(a, p, dvt, s) : la_scan_dk<2, OUT>(a, p, dvt, s);
 }
 
-// A recurrence over the whole sequence: local states and their combination where there are segments, then the pass itself
+// States before the segments: local ones, then their combination
+int la_segments(const LaArgs& a, LaScan p, const LaPlan& pl, int dtype, hipStream_t s) {
+    p.vst = a.Dv % 4 == 0;
+    p.NC = pl.NC; p.cps = pl.cps; p.nseg = pl.nseg; p.ndv = pl.ndv;
+    p.local = 1; p.chunk = nullptr; p.last = nullptr;
+    const int rc = la_launch_scan<false>(a, p, pl.dvt, dtype, s);
+    if (rc != V2A_OK) return rc;
+    const long long SS = (long long)a.Dk * a.Dv;
+    hipLaunchKernelGGL(la_combine, dim3(cdiv(SS, 256), (unsigned)(a.B * a.H)), dim3(256), 0, s, p.seg, p.seg_decay, p.init, pl.nseg, SS);
+    V2A_CHECK_LAUNCH();
+    return V2A_OK;
+}
+// A recurrence over the whole sequence
 template <bool OUT> int la_recur(const LaArgs& a, LaScan p, const LaPlan& pl, int dtype, hipStream_t s) {
     p.vst = a.Dv % 4 == 0 && (((uintptr_t)p.init | (uintptr_t)p.last) & 15) == 0;      // the workspace is aligned
     p.NC = pl.NC; p.cps = pl.cps; p.nseg = pl.nseg; p.ndv = pl.ndv;
-    const long long SS = (long long)a.Dk * a.Dv;
     if (pl.nseg > 1) {
-        LaScan l = p;
-        l.local = 1; l.chunk = nullptr; l.last = nullptr;
-        const int rc = la_launch_scan<false>(a, l, pl.dvt, dtype, s);
+        const int rc = la_segments(a, p, pl, dtype, s);
         if (rc != V2A_OK) return rc;
-        hipLaunchKernelGGL(la_combine, dim3(cdiv(SS, 256), (unsigned)(a.B * a.H)), dim3(256), 0, s, p.seg, p.seg_decay, p.init, pl.nseg, SS);
-        V2A_CHECK_LAUNCH();
     }
     return la_launch_scan<OUT>(a, p, pl.dvt, dtype, s);
 }
@@ -1202,7 +1297,7 @@ LaFwdWs la_fwd_ws(const LaPlan& p, size_t BH, size_t SS) {
     }
     return w;
 }
-struct LaBwdWs { size_t seg, decay, sch, ech, q, k, v, part, total; };
+struct LaBwdWs { size_t seg, decay, sch, q, k, v, part, total; };
 LaBwdWs la_bwd_ws(const LaPlan& p, size_t B, size_t T, size_t H, int Hq, int Hk, int Hv, size_t Dk, size_t Dv, int per_token) {
     LaBwdWs w{};
     const size_t SS = Dk * Dv, BH = B * H, n = B * T * H;
@@ -1211,7 +1306,6 @@ LaBwdWs la_bwd_ws(const LaPlan& p, size_t B, size_t T, size_t H, int Hq, int Hk,
     w.seg = take(p.nseg > 1 ? BH * p.nseg * SS * 4 : 0);
     w.decay = take(p.nseg > 1 ? BH * p.nseg * 4 : 0);
     w.sch = take(p.NC > 1 ? BH * p.NC * SS * 4 : 0);
-    w.ech = take(p.NC > 1 ? BH * p.NC * SS * 4 : 0);
     w.q = take((size_t)Hq < H ? n * Dk * 4 : 0);
     w.k = take((size_t)Hk < H ? n * Dk * 4 : 0);
     w.v = take((size_t)Hv < H ? n * Dv * 4 : 0);
@@ -1226,7 +1320,7 @@ extern "C" {
 
 size_t v2a_linattn_fwd_workspace_bytes(int B, int T, int H, int Dk, int Dv, int dtype) {
     if (!la_dims(B, T, H, H, H, H, Dk, Dv, dtype) || B == 0) return 0;
-    return la_fwd_ws(la_plan(B * H, T, Dv), (size_t)B * H, (size_t)Dk * Dv).total;
+    return la_fwd_ws(la_plan_fwd(B * H, T, Dv), (size_t)B * H, (size_t)Dk * Dv).total;
 }
 
 int v2a_linattn_fwd(const void* q, const void* k, const void* v, const float* g, const float* state, const int32_t* lens, void* out, float* state_out,
@@ -1235,7 +1329,7 @@ int v2a_linattn_fwd(const void* q, const void* k, const void* v, const float* g,
     if (!strides || !la_dims(B, T, H, Hq, Hk, Hv, Dk, Dv, dtype)) return V2A_ERR_ARG;
     if (B == 0 || (T == 0 && !state_out)) return V2A_OK;
     if (T > 0 && (!q || !k || !v || !g || !out)) return V2A_ERR_ARG;
-    const LaPlan pl = la_plan(B * H, T, Dv);
+    const LaPlan pl = la_plan_fwd(B * H, T, Dv);
     const LaFwdWs w = la_fwd_ws(pl, (size_t)B * H, (size_t)Dk * Dv);
     if (ws_bytes < w.total || (w.total && !ws)) return V2A_ERR_WORKSPACE;
     const LaArgs a = la_args(q, k, v, g, state, lens, nullptr, strides, B, T, H, Hq, Hk, Hv, Dk, Dv, scale);
@@ -1254,7 +1348,7 @@ int v2a_linattn_fwd(const void* q, const void* k, const void* v, const float* g,
 
 size_t v2a_linattn_bwd_workspace_bytes(int B, int T, int H, int Hq, int Hk, int Hv, int Dk, int Dv, int dtype, int per_token_decay) {
     if (!la_dims(B, T, H, Hq, Hk, Hv, Dk, Dv, dtype)) return 0;
-    return la_bwd_ws(la_plan(B * H, T, Dv), B, T, H, Hq, Hk, Hv, Dk, Dv, per_token_decay).total;
+    return la_bwd_ws(la_plan_bwd(B * H, T, Dv), B, T, H, Hq, Hk, Hv, Dk, Dv, per_token_decay).total;
 }
 
 int v2a_linattn_bwd(const void* q, const void* k, const void* v, const float* g, const float* state, const int32_t* lens, const void* dout,
@@ -1262,7 +1356,7 @@ int v2a_linattn_bwd(const void* q, const void* k, const void* v, const float* g,
                     int Hv, int Dk, int Dv, int dtype, int per_token_decay, float scale, void* ws, size_t ws_bytes, hipStream_t s) {
     if (!strides || !la_dims(B, T, H, Hq, Hk, Hv, Dk, Dv, dtype)) return V2A_ERR_ARG;
     if (B > 0 && T > 0 && (!q || !k || !v || !g || !dout || !dq || !dk || !dv)) return V2A_ERR_ARG;
-    const LaPlan pl = la_plan(B * H, T, Dv);
+    const LaPlan pl = la_plan_bwd(B * H, T, Dv);
     const LaBwdWs w = la_bwd_ws(pl, B, T, H, Hq, Hk, Hv, Dk, Dv, per_token_decay);
     if (ws_bytes < w.total || (w.total && !ws)) return V2A_ERR_WORKSPACE;
     const LaArgs a = la_args(q, k, v, g, state, lens, dout, strides, B, T, H, Hq, Hk, Hv, Dk, Dv, scale);
@@ -1280,15 +1374,22 @@ int v2a_linattn_bwd(const void* q, const void* k, const void* v, const float* g,
             rc = la_recur<false>(a, f, pl, dtype, s);
             if (rc != V2A_OK) return rc;
         }
-        if (pl.NC > 1 || dstate) {
+        if (pl.nseg > 1) {
             LaScan r = p;
-            r.init = dstate_out; r.chunk = pl.NC > 1 ? at(w.ech) : nullptr; r.last = dstate; r.rev = 1; r.vx = vq; r.vy = vd;
+            r.init = dstate_out; r.rev = 1; r.vx = vq; r.vy = vd;
+            rc = la_segments(a, r, pl, dtype, s);
+            if (rc != V2A_OK) return rc;
+        }
+        if (T == 0 && dstate) {              // no tokens: the gradient passes through
+            LaScan r = p;
+            r.init = dstate_out; r.rev = 1; r.last = dstate;
             rc = la_recur<false>(a, r, pl, dtype, s);
             if (rc != V2A_OK) return rc;
         }
         if (T > 0) {
             LaBwd d{};
-            d.s_chunk = at(w.sch); d.e_chunk = at(w.ech); d.s_first = state; d.e_last = dstate_out;
+            d.s_chunk = at(w.sch); d.s_first = state; d.e_last = dstate_out; d.e_seg = at(w.seg); d.e_first = dstate;
+            d.cps = pl.cps; d.nseg = pl.nseg;
             d.fq = Hq < H; d.fk = Hk < H; d.fv = Hv < H;
             d.dq = d.fq ? (void*)at(w.q) : dq;
             d.dk = d.fk ? (void*)at(w.k) : dk;
@@ -1296,13 +1397,13 @@ int v2a_linattn_bwd(const void* q, const void* k, const void* v, const float* g,
             d.dg = per_token_decay ? dg : nullptr;
             d.dg_part = per_token_decay || !dg ? nullptr : at(w.part);
             d.NC = pl.NC; d.vq = vq; d.vk = vk; d.vv = vv; d.vd = vd;
-            d.vst = Dv % 4 == 0 && (((uintptr_t)state | (uintptr_t)dstate_out) & 15) == 0;
-            const dim3 grid((unsigned)((long long)B * H * pl.NC));
+            d.vst = Dv % 4 == 0 && (((uintptr_t)state | (uintptr_t)dstate_out | (uintptr_t)dstate) & 15) == 0;
+            const dim3 grid((unsigned)((long long)B * H * pl.nseg));
             const int Dm = Dk > Dv ? Dk : Dv;
 #define CALL(DT)                                                                                                        \
-    if (Dm <= 32) hipLaunchKernelGGL((la_bwd_chunk<DT, 32>), grid, dim3(128), 0, s, a, d);                              \
-    else if (Dm <= 64) hipLaunchKernelGGL((la_bwd_chunk<DT, 64>), grid, dim3(256), 0, s, a, d);                         \
-    else hipLaunchKernelGGL((la_bwd_chunk<DT, 128>), grid, dim3(512), 0, s, a, d)
+    if (Dm <= 32) hipLaunchKernelGGL((la_bwd_chunks<DT, 32>), grid, dim3(128), 0, s, a, d);                              \
+    else if (Dm <= 64) hipLaunchKernelGGL((la_bwd_chunks<DT, 64>), grid, dim3(256), 0, s, a, d);                         \
+    else hipLaunchKernelGGL((la_bwd_chunks<DT, 128>), grid, dim3(512), 0, s, a, d)
             LA_BY_TYPE(dtype, CALL);
 #undef CALL
             V2A_CHECK_LAUNCH();
