@@ -41,7 +41,7 @@ __device__ __forceinline__ float la_clampg(float g) { return g < LA_GMIN ? LA_GM
 // state is an fp32 result and lives long.  Sums are fp32.  fp32 inputs use the fp32 MFMA (16 x 16 x 4) in the same slot order.
 // Running log decays are summed in fp64 and kept as a float pair: W of two tokens behind a reset (g clamped at -1000) keeps its digits.
 constexpr int LA_C = 64;
-constexpr float LA_LOG2E = 1.44269504088896340736f;
+#define LA_FENCE __builtin_amdgcn_sched_barrier(0)      // between stages: moved up, the next one's operands fill the registers
 typedef __attribute__((ext_vector_type(4))) unsigned int la_u32x4;
 typedef __attribute__((ext_vector_type(2))) unsigned int la_u32x2;
 typedef __attribute__((ext_vector_type(4))) __bf16 la_bf16x4;
@@ -165,6 +165,14 @@ template <int DT, int D> struct LaTile {
     }
 };
 
+// A value that is the same in all lanes, cut off from where it came from: what is computed from it is computed here and now.  Hoisted out of the
+// chunk loop, the row offsets of all operands together overflow the scalar registers, whose spills take vector registers and instructions.
+template <typename T> __device__ __forceinline__ T la_here(T x) {
+    asm volatile("" : "+s"(x));
+    return x;
+}
+template <typename T> __device__ __forceinline__ T* la_at(const void* base, unsigned off) { return (T*)((char*)base + off); }
+
 // Global rows -> registers (load) -> LDS (store), so that the next chunk's rows are under way while this one is computed.  Rows from nv on
 // and columns from Dx on are zeros and not read.  vec: base, strides and Dx allow 16-byte loads; else element by element.
 template <int DT, int D, int NTH> struct LaLoad {
@@ -173,16 +181,21 @@ template <int DT, int D, int NTH> struct LaLoad {
     static_assert(LA_C * CPR % NTH == 0, "whole 16-byte pieces per thread");
     static_assert(NTH % CPR == 0, "a thread's pieces share their columns");
     la_u32x4 r[N];
-    // thread t owns columns EPC (t % CPR) .. of rows t / CPR + i NTH / CPR
-    __device__ __forceinline__ void load(const E* p, long long st, int nv, int Dx, int vec) {
+    // Thread t owns columns EPC (t % CPR) .. of rows t / CPR + i NTH / CPR.  p is the same in all lanes: with the lane's part of the address in
+    // 32 bits (which `vec` vouches for) the rest stays in scalar registers.
+    __device__ __forceinline__ void load(const E* p, long long st_, int nv_, int Dx, int vec) {
+        const long long st = la_here(st_);
+        const int nv = la_here(nv_);
         const int row = threadIdx.x / CPR, c = (threadIdx.x % CPR) * EPC;
-        const E* q = p + row * st + c;
+        const unsigned off = ((unsigned)row * (unsigned)st + (unsigned)c) * (unsigned)sizeof(E);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             r[i] = la_u32x4{0u, 0u, 0u, 0u};
             if (row + i * (NTH / CPR) < nv && c < Dx) {
-                if (vec) r[i] = *(const la_u32x4*)q;
+                const E* u = p + st * (i * (NTH / CPR));
+                if (vec) r[i] = *la_at<la_u32x4>(u, off);
                 else {
+                    const E* q = u + row * st + c;
 #pragma unroll
                     for (int e = 0; e < EPC; ++e)
                         if (c + e < Dx) {
@@ -191,7 +204,6 @@ template <int DT, int D, int NTH> struct LaLoad {
                         }
                 }
             }
-            q += st * (NTH / CPR);
         }
     }
     __device__ __forceinline__ void store(char* t) const {
@@ -230,6 +242,13 @@ template <int CTRL> __device__ __forceinline__ double la_row_shr(double x) {
 __device__ __forceinline__ double la_lane(double x, int l) {
     const la_u32x2 u = __builtin_bit_cast(la_u32x2, x);
     return __builtin_bit_cast(double, la_u32x2{(unsigned)__builtin_amdgcn_readlane((int)u[0], l), (unsigned)__builtin_amdgcn_readlane((int)u[1], l)});
+}
+// sum over the four lanes l, l ^ 16, l ^ 32, l ^ 48 in each of them, by row swaps of the vector unit (no trip through LDS)
+__device__ __forceinline__ float la_rows_sum(float x) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 // inclusive sum over the 64 lanes: inside the rows by DPP, over the rows by readlane (twelve ds_bpermute round trips otherwise: 1000 cycles)
 __device__ __forceinline__ double la_running(double x, int lane) {
@@ -584,7 +603,7 @@ __global__ __launch_bounds__(64 * NW, (la_scan_waves<DT, DK, NT, NW, OUT>())) vo
                     if (r >= nv)
 #pragma unroll
                         for (int n = 0; n < NT; ++n) O[n][it] = f32x4{0.f, 0.f, 0.f, 0.f};
-                    E* q = out + r * ot + d;
+                    E* q = la_at<E>(out + it * 16 * ot + dv0, ((unsigned)(lane & 15) * (unsigned)ot + (unsigned)((lane >> 4) * 4 * NT)) * (unsigned)sizeof(E));
                     if constexpr (NT == 2 && DT != 0) {
                         if (p.vo && d + 8 <= Dv) {
                             *(la_u32x4*)q = la_u32x4{v2a_pack_h2<DT == 2>(O[0][it][0], O[0][it][1]), v2a_pack_h2<DT == 2>(O[0][it][2], O[0][it][3]),
@@ -715,23 +734,33 @@ __global__ __launch_bounds__(4 * D) void la_bwd_chunks(LaArgs a, LaBwd p) {
     const E* G = (const E*)a.dout + b * a.ds[0] + h * a.ds[2];
     const float* g = a.g + b * a.gs[0] + h * a.gs[2];
 
-    // one row of four values of a gradient: shared heads keep fp32 per head (rows of H heads), others their own type
-    auto put = [&](void* base, int f32, int Hx, int hx, int Dx, int c, int row, int d, const f32x4& x) __attribute__((always_inline)) {
-        const long long t = (long long)c * LA_C + row;
-        if (d >= Dx || t >= a.T) return;
-        if (f32) la_store4<0>((float*)base + (((long long)b * a.T + t) * a.H + h) * Dx + d, x, Dx - d, Dx % 4 == 0);
-        else la_store4<DT>((E*)base + (((long long)b * a.T + t) * Hx + hx) * Dx + d, x, Dx - d, Dx % 4 == 0);
+    // four values of each of the rows l16, l16 + 16, .. of a gradient: shared heads keep fp32 per head (rows of H heads), others their own type
+    auto put = [&](void* base, int f32, int Hx, int hx, int Dx, int c, const f32x4 (&x)[4]) __attribute__((always_inline)) {
+        const int left = la_here(a.T - c * LA_C), room = Dx - w0 - l4, ld = la_here((f32 ? a.H : Hx) * Dx);
+        const long long at = ((long long)b * a.T + (long long)c * LA_C) * ld + (f32 ? h : hx) * Dx + w0;
+        const unsigned off = (unsigned)l16 * (unsigned)ld + (unsigned)l4;
+        if (room <= 0) return;
+        auto rows = [&](auto&& one) __attribute__((always_inline)) {
+#pragma unroll
+            for (int tt = 0; tt < 4; ++tt)
+                if (tt * 16 + l16 < left) one(at + (long long)(tt * 16) * ld, x[tt]);
+        };
+        if (Dx % 4 == 0) {
+            if (f32) rows([&](long long o, const f32x4& y) { *la_at<f32x4>((float*)base + o, off * 4u) = y; });
+            else rows([&](long long o, const f32x4& y) { la_store4<DT>(la_at<E>((E*)base + o, off * (unsigned)sizeof(E)), y, 4, true); });
+        } else {
+            if (f32) rows([&](long long o, const f32x4& y) { la_store4<0>(la_at<float>((float*)base + o, off * 4u), y, room, false); });
+            else rows([&](long long o, const f32x4& y) { la_store4<DT>(la_at<E>((E*)base + o, off * (unsigned)sizeof(E)), y, room, false); });
+        }
     };
     // this segment's chunks chi, chi - 1, .. clo; those from nvc on have no tokens
     const int chi = p.NC - 1 - seg * p.cps, clo = chi - p.cps + 1 > 0 ? chi - p.cps + 1 : 0;
     const int nvc = (len + LA_C - 1) / LA_C, cfirst = chi < nvc ? chi : nvc - 1;
     for (int c = chi; c > cfirst && c >= clo; --c) {
-        const f32x4 z = {0.f, 0.f, 0.f, 0.f};
-        for (int r = l16; r < LA_C; r += 16) {
-            put(p.dq, p.fq, a.Hq, hq, Dk, c, r, w0 + l4, z);
-            put(p.dk, p.fk, a.Hk, hk, Dk, c, r, w0 + l4, z);
-            put(p.dv, p.fv, a.Hv, hv, Dv, c, r, w0 + l4, z);
-        }
+        const f32x4 z[4] = {};
+        put(p.dq, p.fq, a.Hq, hq, Dk, c, z);
+        put(p.dk, p.fk, a.Hk, hk, Dk, c, z);
+        put(p.dv, p.fv, a.Hv, hv, Dv, c, z);
         if (wid == 0 && p.dg && c * LA_C + lane < a.T) p.dg[((long long)b * a.T + (long long)c * LA_C + lane) * a.H + h] = 0.f;
         if (threadIdx.x == 0 && p.dg_part) p.dg_part[(long long)c * a.B * a.H + bh] = 0.f;
     }
@@ -750,7 +779,7 @@ __global__ __launch_bounds__(4 * D) void la_bwd_chunks(LaArgs a, LaBwd p) {
                 const int d = kk * 32 + l4 * 2 + half * 4;
                 x[kk][half] = f32x4{0.f, 0.f, 0.f, 0.f};
                 if (st && w0 + l16 < Dk && d < Dv) {
-                    const float* q = st + (w0 + l16) * Dv + d;
+                    const float* q = la_at<float>(st, (unsigned)((w0 + l16) * Dv + l4 * 2) * 4u) + kk * 32 + half * 4;
                     if (p.vst) x[kk][half] = *(const f32x4*)q;
                     else
 #pragma unroll
@@ -774,7 +803,7 @@ __global__ __launch_bounds__(4 * D) void la_bwd_chunks(LaArgs a, LaBwd p) {
                 }
     }
     LaLoad<DT, D, NTH> rq, rk, rv, rd;
-    float rg = 0.f, rgn = 0.f;      // this chunk's and the next one's decays, in the first / last wave
+    float rgn = 0.f;      // the next chunk's decays, in the last wave
     auto valid = [&](int c) { return len - c * LA_C < LA_C ? len - c * LA_C : LA_C; };
     auto fetch = [&](int c) __attribute__((always_inline)) {
         if (c < clo) return;
@@ -798,28 +827,35 @@ __global__ __launch_bounds__(4 * D) void la_bwd_chunks(LaArgs a, LaBwd p) {
     }
     f32x4 acc[4];
     float raw[3][8];
-    // d decay of the chunk whose parts are in LDS (first wave, lane = token)
-    auto decays = [&](int c) __attribute__((always_inline)) {
+    // d decay of a chunk (first wave, lane = token): its parts are gathered from LDS while the next chunk's rows are stored, and summed up later
+    double up = 0.0, down = 0.0, cross = 0.0;
+    bool gone = false;
+    auto gather = [&](int c) __attribute__((always_inline)) {
         const int nv = valid(c);
-        double up = 0.0, down = 0.0, z = 0.0;
+        const LaGate& gt = gts[c & 1];
+        float u = 0.f, dn = 0.f, z = 0.f;
 #pragma unroll
         for (int w = 0; w < NW; ++w) {
-            up += sr[w][lane];
-            down += sc[w][lane];
+            u += sr[w][lane];
+            dn += sc[w][lane];
             z += sz[w];
         }
         // parts that no unit of the lower triangle wrote are left out
+        float r = 0.f, m = 0.f;
 #pragma unroll
         for (int jt = 0; jt < 4; ++jt)
-            if (lane >= jt * 16) up += rm[jt][lane];
-        if (lane < 32) up -= cm[0][lane];
-        if (nv > 32) up -= cm[1][lane];
-        if (lane >= nv) up = down = 0.0;
-        const double down_to = la_running(down, lane) - down, all = la_running(up, lane), up_from = la_lane(all, 63) - all + up;
-        const float gg = lane < nv ? g[((long long)c * LA_C + lane) * a.gs[1]] : 0.f;
-        const bool gone = __builtin_amdgcn_exp2f(la_clampg(gg) * LA_LOG2E) == 0.f;
-        double d = z * (double)gts[c & 1].total + up_from + down_to;
-        if (gone || lane >= nv) d = 0.0;
+            if (lane >= jt * 16) r += rm[jt][lane];
+        if (lane < 32) m += cm[0][lane];
+        if (nv > 32) m += cm[1][lane];
+        const float g2 = lane ? (gt.hi[lane] - gt.hi[lane - 1]) + (gt.lo[lane] - gt.lo[lane - 1]) : gt.hi[0];
+        gone = __builtin_amdgcn_exp2f(g2) == 0.f || lane >= nv;
+        up = lane < nv ? ((double)u + (double)r) - (double)m : 0.0;
+        down = lane < nv ? (double)dn : 0.0;
+        cross = (double)z * (double)gt.total;
+    };
+    auto decays = [&](int c) __attribute__((always_inline)) {
+        const double to = la_running(down, lane) - down, all = la_running(up, lane), from = la_lane(all, 63) - all + up;
+        double d = gone ? 0.0 : cross + from + to;
         const long long t = (long long)c * LA_C + lane;
         if (p.dg && t < a.T) p.dg[((long long)b * a.T + t) * a.H + h] = (float)d;
         if (p.dg_part) {
@@ -835,7 +871,7 @@ __global__ __launch_bounds__(4 * D) void la_bwd_chunks(LaArgs a, LaBwd p) {
         rk.store(sk);
         rv.store(sv);
         rd.store(sd);
-        if (wid == 0 && c < cfirst) decays(c + 1);
+        if (wid == 0 && c < cfirst) gather(c + 1);
         __syncthreads();
         {
             float z = 0.f;
@@ -925,8 +961,7 @@ __global__ __launch_bounds__(4 * D) void la_bwd_chunks(LaArgs a, LaBwd p) {
                         m += v2a_dpp<0x140>(m);
                         if (l16 == 0) rm[jt][i] = m;
                     }
-                    col += __shfl_xor(col, 16, 64);
-                    col += __shfl_xor(col, 32, 64);
+                    col = la_rows_sum(col);
                     if (lane < 16) cm[is >> 5][j] = col;
                 }
             }
@@ -961,9 +996,7 @@ __global__ __launch_bounds__(4 * D) void la_bwd_chunks(LaArgs a, LaBwd p) {
             for (int tt = 0; tt < 4; ++tt) {
                 float y[4];
                 TT::four(own, tt * 16 + l16, w0 + l4, y);
-                float s = (acc[tt][0] * y[0] + acc[tt][1] * y[1]) + (acc[tt][2] * y[2] + acc[tt][3] * y[3]);
-                s += __shfl_xor(s, 16, 64);
-                s += __shfl_xor(s, 32, 64);
+                const float s = la_rows_sum((acc[tt][0] * y[0] + acc[tt][1] * y[1]) + (acc[tt][2] * y[2] + acc[tt][3] * y[3]));
                 if (lane < 16) dst[tt * 16 + lane] = s;
             }
         };
@@ -987,23 +1020,27 @@ __global__ __launch_bounds__(4 * D) void la_bwd_chunks(LaArgs a, LaBwd p) {
         auto emit = [&](void* base, int f32, int Hx, int hx, int Dx) __attribute__((always_inline)) {
 #pragma unroll
             for (int tt = 0; tt < 4; ++tt) {
-                const int r = tt * 16 + l16;
-                put(base, f32, Hx, hx, Dx, c, r, w0 + l4, r < nv ? acc[tt] : f32x4{0.f, 0.f, 0.f, 0.f});
+                if (tt * 16 + l16 >= nv) acc[tt] = f32x4{0.f, 0.f, 0.f, 0.f};
             }
+            put(base, f32, Hx, hx, Dx, c, acc);
         };
         const float* sp = state_of(c);
+        if (wid == 0 && c < cfirst) decays(c + 1);
         unit1();
         if constexpr (NBUF == 3) {
             unit23(sd, sv, s2, false);
             unit23(sq, sk, s3, true);
         }
         __syncthreads();
-        fetch(c - 1);
         clear();
+        fetch(c - 1);
         if (sp) through(xs, sd, gt.wq, a.scale);
         with_own(sq, sr[wid]);
+        LA_FENCE;
         within(sk, s1, false);
+        LA_FENCE;
         emit(p.dq, p.fq, a.Hq, hq, Dk);
+        LA_FENCE;
         if (c > clo) state_rows(state_of(c - 1), xs);
         gates(c - 1);
         fetch_g(c - 2);
@@ -1015,8 +1052,11 @@ __global__ __launch_bounds__(4 * D) void la_bwd_chunks(LaArgs a, LaBwd p) {
         clear();
         if (have_e) through(e1, sv, gt.wk, 1.f);
         with_own(sk, sc[wid]);
+        LA_FENCE;
         within(sq, s2, true);
+        LA_FENCE;
         emit(p.dk, p.fk, a.Hk, hk, Dk);
+        LA_FENCE;
         if constexpr (NBUF == 1) {
             __syncthreads();
             unit23(sq, sk, s3, true);
@@ -1025,7 +1065,9 @@ __global__ __launch_bounds__(4 * D) void la_bwd_chunks(LaArgs a, LaBwd p) {
         clear();
         if (have_e) through(e2, sk, gt.wk, 1.f);
         within(sd, s3, true);
+        LA_FENCE;
         emit(p.dv, p.fv, a.Hv, hv, Dv);
+        LA_FENCE;
         // E of the chunk before, if anybody reads it (a loop of no rounds, not a branch: the accumulators keep one definition)
         const int nks = c > clo || p.e_first ? (nv > 32 ? 2 : 1) : 0;
         have_e = true;
@@ -1068,7 +1110,10 @@ __global__ __launch_bounds__(4 * D) void la_bwd_chunks(LaArgs a, LaBwd p) {
         }
     }
     __syncthreads();
-    if (wid == 0 && cfirst >= clo) decays(clo);
+    if (wid == 0 && cfirst >= clo) {
+        gather(clo);
+        decays(clo);
+    }
     if (p.e_first && clo == 0 && w0 + l16 < Dk)
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk)
@@ -1199,7 +1244,8 @@ __global__ __launch_bounds__(256) void la_step_kernel(const void* q_, const void
 
 bool la_dims(int B, int T, int H, int Hq, int Hk, int Hv, int Dk, int Dv, int dtype) {
     return B >= 0 && T >= 0 && H > 0 && Hq > 0 && Hk > 0 && Hv > 0 && H % Hq == 0 && H % Hk == 0 && H % Hv == 0 && Dk > 0 && Dk <= LA_DMAX && Dv > 0 &&
-           Dv <= LA_DMAX && dtype >= 0 && dtype <= 2 && (long long)B * H * (T / 64 + 1) < (1ll << 23);      // grid x block stays below 2^32 threads
+           Dv <= LA_DMAX && dtype >= 0 && dtype <= 2 && (long long)B * H * (T / 64 + 1) < (1ll << 23) &&      // grid x block stays below 2^32 threads,
+           (long long)H * LA_DMAX < (1ll << 24);                                                      // 16 rows of all heads below 2^31 bytes
 }
 
 LaArgs la_args(const void* q, const void* k, const void* v, const float* g, const float* state, const int32_t* lens, const void* dout, const int64_t* st, int B,
@@ -1246,6 +1292,7 @@ LaPlan la_plan_bwd(int BH, int T, int Dv) { return la_plan(BH, T, Dv, 512, 2); }
 int la_vec(const void* p, const long long* st, int B, int T, int H, int D, int dtype) {
     const long long es = dtype == 0 ? 4 : 2;
     if (((uintptr_t)p & 15) || D * es % 16) return 0;
+    if (T > 1 && (st[1] < 0 || st[1] * es * LA_C > 0x7fffffffll)) return 0;      // rows of a chunk within 32-bit offsets
     return !((B > 1 && st[0] * es % 16) || (T > 1 && st[1] * es % 16) || (H > 1 && st[2] * es % 16));
 }
 
