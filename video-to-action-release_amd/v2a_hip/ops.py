@@ -1527,65 +1527,71 @@ _SEQ_DT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _I64x8, _I64x12, _I64x15 = ctypes.c_int64 * 8, ctypes.c_int64 * 12, ctypes.c_int64 * 15
 
 
-def _need(ok, what):
-    if not ok:
-        raise ValueError(what)
-
-
 def _same_device(t, *others):
     """The operands of one call live on one GPU; the launch goes to torch's current stream of that GPU."""
-    _need(t.is_cuda, "need CUDA tensors")
+    if not t.is_cuda:
+        raise ValueError("need CUDA tensors")
+    i = t.get_device()
     for o in others:
-        _need(o is None or o.device == t.device, "operands on different devices")
+        if o is not None and o.get_device() != i:
+            raise ValueError("operands on different devices")
 
 
-def _on_device_of(i):
-    """Decorator: argument `i` names the GPU the call runs on (the current one or not)."""
-    def wrap(fn):
-        @functools.wraps(fn)
-        def call(*a, **kw):
-            t = a[i] if len(a) > i else None
-            if isinstance(t, torch.Tensor) and t.is_cuda and t.get_device() != torch.cuda.current_device():
-                with torch.cuda.device(t.device):
-                    return fn(*a, **kw)
-            return fn(*a, **kw)
-        return call
-    return wrap
+def _on_device_of_first(fn):
+    """Decorator: the first operand names the GPU the call runs on (the current one or not)."""
+    @functools.wraps(fn)
+    def call(t, *a, **kw):
+        if t.is_cuda and t.get_device() != torch.cuda.current_device():
+            with torch.cuda.device(t.device):
+                return fn(t, *a, **kw)
+        return fn(t, *a, **kw)
+    return call
 
 
 def _la_heads(q, k, v, g, lead):
     """Checks shared by the linear-attention calls (lead = leading dimensions of q / k / v) -> (H, Hq, Hk, Hv, Dk, Dv, dtype id)."""
-    nd = lead + 2
-    _need(q.dim() == nd and k.dim() == nd and v.dim() == nd, f"q, k, v: need {nd} dimensions")
-    _need(q.dtype in _SEQ_DT and k.dtype == q.dtype and v.dtype == q.dtype, "q, k, v: need one type of fp32 / bf16 / fp16")
-    _need(q.shape[:lead] == k.shape[:lead] == v.shape[:lead], "q, k, v: different batch or length")
-    Hq, Dk = q.shape[lead:]
-    Hk, Hv, Dv = k.shape[lead], v.shape[lead], v.shape[-1]
-    _need(k.shape[-1] == Dk, "q and k: different head widths")
-    _need(0 < Dk <= 128 and 0 < Dv <= 128, "head widths: 1 to 128")
-    _need(q.stride(-1) == 1 or Dk == 1, "q: last dimension must be contiguous")
-    _need(k.stride(-1) == 1 or Dk == 1, "k: last dimension must be contiguous")
-    _need(v.stride(-1) == 1 or Dv == 1, "v: last dimension must be contiguous")
-    _need(g.dtype == torch.float32 and g.dim() in (1, lead + 1), "log_decay: need fp32 [H] or one value per token and head")
-    H = g.shape[-1]
-    _need(g.dim() == 1 or g.shape[:-1] == q.shape[:lead], "log_decay: batch or length differ from q")
-    _need(H > 0 and Hq > 0 and Hk > 0 and Hv > 0 and H % Hq == 0 and H % Hk == 0 and H % Hv == 0, "heads of q, k and v must divide those of log_decay")
-    return H, Hq, Hk, Hv, Dk, Dv, _SEQ_DT[q.dtype]
+    qs, ks, vs, gs = q.shape, k.shape, v.shape, g.shape
+    if not len(qs) == len(ks) == len(vs) == lead + 2:
+        raise ValueError(f"q, k, v: need {lead + 2} dimensions")
+    dt = _SEQ_DT.get(q.dtype)
+    if dt is None or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError("q, k, v: need one type of fp32 / bf16 / fp16")
+    if not qs[:lead] == ks[:lead] == vs[:lead]:
+        raise ValueError("q, k, v: different batch or length")
+    Hq, Dk = qs[lead:]
+    Hk, Hv, Dv = ks[lead], vs[lead], vs[-1]
+    if ks[-1] != Dk:
+        raise ValueError("q and k: different head widths")
+    if not (0 < Dk <= 128 and 0 < Dv <= 128):
+        raise ValueError("head widths: 1 to 128")
+    for t, d, what in ((q, Dk, "q"), (k, Dk, "k"), (v, Dv, "v")):
+        if t.stride(-1) != 1 and d != 1:
+            raise ValueError(what + ": last dimension must be contiguous")
+    if g.dtype != torch.float32 or len(gs) not in (1, lead + 1):
+        raise ValueError("log_decay: need fp32 [H] or one value per token and head")
+    H = gs[-1]
+    if len(gs) != 1 and gs[:-1] != qs[:lead]:
+        raise ValueError("log_decay: batch or length differ from q")
+    if not (H > 0 and Hq > 0 and Hk > 0 and Hv > 0) or H % Hq or H % Hk or H % Hv:
+        raise ValueError("heads of q, k and v must divide those of log_decay")
+    return H, Hq, Hk, Hv, Dk, Dv, dt
 
 
 def _la_state(t, shape, what):
-    _need(t.dtype == torch.float32 and t.is_contiguous() and tuple(t.shape) == shape, f"{what}: need contiguous fp32 {list(shape)}")
+    if t.dtype != torch.float32 or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{what}: need contiguous fp32 {list(shape)}")
 
 
 def _la_lens(lens, B):
-    _need(lens.dtype == torch.int32 and lens.is_contiguous() and tuple(lens.shape) == (B,), f"lens: need contiguous int32 [{B}]")
+    if lens.dtype != torch.int32 or lens.shape != (B,) or not lens.is_contiguous():
+        raise ValueError(f"lens: need contiguous int32 [{B}]")
 
 
 def _g_strides(g, lead):
     return (0,) * lead + (g.stride(0),) if g.dim() == 1 else g.stride()
 
 
-@_on_device_of(0)
+@_on_device_of_first
 def linear_attention_fwd(q, k, v, log_decay, state=None, lens=None, scale=None, want_state=False):
     """out_t = scale * S_t^T q_t with S_t = exp(log_decay_t) S_{t-1} + k_t v_t^T: causal attention without a softmax, whose state S (fp32,
     [Dk,Dv] per row and head) is all that later tokens need.  -> (out [B,T,H,Dv] in q's type, last state [B,H,Dk,Dv] or None).
@@ -1596,51 +1602,53 @@ def linear_attention_fwd(q, k, v, log_decay, state=None, lens=None, scale=None, 
     lens[b] tokens; what is behind them is not read, out is 0 there and the last state is the one after them.  scale: 1 / sqrt(Dk) by default."""
     H, Hq, Hk, Hv, Dk, Dv, dt = _la_heads(q, k, v, log_decay, 2)
     _same_device(q, k, v, log_decay, state, lens)
-    B, T = q.shape[0], q.shape[1]
+    B, T = q.shape[:2]
     if state is not None:
         _la_state(state, (B, H, Dk, Dv), "state")
     if lens is not None:
         _la_lens(lens, B)
-    out = torch.empty((B, T, H, Dv), dtype=q.dtype, device=q.device)
-    last = torch.empty((B, H, Dk, Dv), dtype=torch.float32, device=q.device) if want_state else None
+    out = q.new_empty((B, T, H, Dv))
+    last = log_decay.new_empty((B, H, Dk, Dv)) if want_state else None
     nb = lib.v2a_linattn_fwd_workspace_bytes(B, T, H, Dk, Dv, dt)
-    ws = torch.empty(nb, dtype=torch.uint8, device=q.device) if nb else None
+    ws = q.new_empty(nb, dtype=torch.uint8) if nb else None
     st = _I64x12(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *_g_strides(log_decay, 2))
     check(lib.v2a_linattn_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), _p(state), _p(lens), out.data_ptr(), _p(last), st, B, T, H,
-                              Hq, Hk, Hv, Dk, Dv, dt, Dk ** -0.5 if scale is None else float(scale), _p(ws), nb, _stream()), "linear_attention_fwd")
+                              Hq, Hk, Hv, Dk, Dv, dt, Dk ** -0.5 if scale is None else scale, _p(ws), nb, _stream()), "linear_attention_fwd")
     return out, last
 
 
-@_on_device_of(0)
+@_on_device_of_first
 def linear_attention_bwd(q, k, v, log_decay, dout, state=None, lens=None, scale=None, dstate=None):
     """Gradient of linear_attention_fwd (same q .. scale): dout [B,T,H,Dv] in q's type, dstate = gradient of the last state (None: 0)
     -> (dq, dk, dv in q's type, d log_decay fp32 in log_decay's shape, gradient of `state` or None without one).  Nothing but the inputs is
     kept from the forward.  Sums over shared heads and over broadcast decays have a fixed order."""
     H, Hq, Hk, Hv, Dk, Dv, dt = _la_heads(q, k, v, log_decay, 2)
     _same_device(q, k, v, log_decay, dout, state, lens, dstate)
-    B, T = q.shape[0], q.shape[1]
-    _need(tuple(dout.shape) == (B, T, H, Dv) and dout.dtype == q.dtype, f"dout: need {[B, T, H, Dv]} in q's type")
-    _need(dout.stride(-1) == 1 or Dv == 1, "dout: last dimension must be contiguous")
+    B, T = q.shape[:2]
+    if dout.shape != (B, T, H, Dv) or dout.dtype != q.dtype:
+        raise ValueError(f"dout: need {[B, T, H, Dv]} in q's type")
+    if dout.stride(-1) != 1 and Dv != 1:
+        raise ValueError("dout: last dimension must be contiguous")
     if state is not None:
         _la_state(state, (B, H, Dk, Dv), "state")
     if dstate is not None:
         _la_state(dstate, (B, H, Dk, Dv), "dstate")
     if lens is not None:
         _la_lens(lens, B)
-    dq, dk, dv = (torch.empty((B, T, h, d), dtype=q.dtype, device=q.device) for h, d in ((Hq, Dk), (Hk, Dk), (Hv, Dv)))
-    dg = torch.empty(log_decay.shape, dtype=torch.float32, device=q.device)
-    ds0 = None if state is None else torch.empty((B, H, Dk, Dv), dtype=torch.float32, device=q.device)
+    dq, dk, dv = q.new_empty((B, T, Hq, Dk)), q.new_empty((B, T, Hk, Dk)), q.new_empty((B, T, Hv, Dv))
+    dg = log_decay.new_empty(log_decay.shape)
+    ds0 = None if state is None else log_decay.new_empty((B, H, Dk, Dv))
     tok = 1 if log_decay.dim() == 3 else 0
     nb = lib.v2a_linattn_bwd_workspace_bytes(B, T, H, Hq, Hk, Hv, Dk, Dv, dt, tok)
-    ws = torch.empty(nb, dtype=torch.uint8, device=q.device) if nb else None
+    ws = q.new_empty(nb, dtype=torch.uint8) if nb else None
     st = _I64x15(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *_g_strides(log_decay, 2), *dout.stride()[:3])
     check(lib.v2a_linattn_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), _p(state), _p(lens), dout.data_ptr(), _p(dstate), dq.data_ptr(),
                               dk.data_ptr(), dv.data_ptr(), dg.data_ptr(), _p(ds0), st, B, T, H, Hq, Hk, Hv, Dk, Dv, dt, tok,
-                              Dk ** -0.5 if scale is None else float(scale), _p(ws), nb, _stream()), "linear_attention_bwd")
+                              Dk ** -0.5 if scale is None else scale, _p(ws), nb, _stream()), "linear_attention_bwd")
     return dq, dk, dv, dg, ds0
 
 
-@_on_device_of(0)
+@_on_device_of_first
 def linear_attention_step(q, k, v, log_decay, state, slots=None, scale=None):
     """One token for each of B rows: S <- exp(log_decay) S + k v^T in place, -> out [B,H,Dv] = scale * S^T q (the recurrent form of
     linear_attention_fwd).  q [B,Hq,Dk], k [B,Hk,Dk], v [B,Hv,Dv], log_decay [H] or [B,H]; state fp32 [N,H,Dk,Dv], contiguous.
@@ -1649,60 +1657,73 @@ def linear_attention_step(q, k, v, log_decay, state, slots=None, scale=None):
     H, Hq, Hk, Hv, Dk, Dv, dt = _la_heads(q, k, v, log_decay, 1)
     _same_device(q, k, v, log_decay, state, slots)
     B = q.shape[0]
-    _need(state.dim() == 4, "state: need [N,H,Dk,Dv]")
+    if state.dim() != 4:
+        raise ValueError("state: need [N,H,Dk,Dv]")
     N = state.shape[0]
     _la_state(state, (N, H, Dk, Dv), "state")
     if slots is not None:
         _la_lens(slots, B)
-    else:
-        _need(N == B, "state: need one row per row of q, or slots")
-    out = torch.empty((B, H, Dv), dtype=q.dtype, device=q.device)
+    elif N != B:
+        raise ValueError("state: need one row per row of q, or slots")
+    out = q.new_empty((B, H, Dv))
     st = _I64x8(*q.stride()[:2], *k.stride()[:2], *v.stride()[:2], *_g_strides(log_decay, 1))
     check(lib.v2a_linattn_step(q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), state.data_ptr(), _p(slots), out.data_ptr(), st, B, N, H, Hq, Hk,
-                               Hv, Dk, Dv, dt, Dk ** -0.5 if scale is None else float(scale), _stream()), "linear_attention_step")
+                               Hv, Dk, Dv, dt, Dk ** -0.5 if scale is None else scale, _stream()), "linear_attention_step")
     return out
 
 
 def _ids(ids):
-    _need(ids.dtype in (torch.int64, torch.int32) and ids.is_contiguous() and ids.dim() > 0, "ids: need contiguous int64 or int32 of one dimension or more")
-    return ids.numel(), ids.shape[-1], 1 if ids.dtype == torch.int64 else 0
+    wide = ids.dtype == torch.int64
+    if not (wide or ids.dtype == torch.int32) or ids.dim() == 0 or not ids.is_contiguous():
+        raise ValueError("ids: need contiguous int64 or int32 of one dimension or more")
+    return ids.numel(), ids.shape[-1], 1 if wide else 0
 
 
-@_on_device_of(0)
+@_on_device_of_first
 def embed_fwd(ids, table, scale=1.0, pos=None):
     """out[..., t, :] = scale * table[ids[..., t]] + pos[t]  (fp32 arithmetic, rounded once to table's type).  ids int64 / int32 [..., T];
     table [V,D] fp32 / bf16 / fp16 (rows may be strided); pos [>= T, D] in table's type or None.  An id outside [0, V) is an empty place: a
     zero row."""
     N, T, wide = _ids(ids)
     _same_device(ids, table, pos)
-    _need(table.dim() == 2 and table.dtype in _SEQ_DT and table.shape[0] > 0 and table.shape[1] > 0, "table: need [V,D] fp32 / bf16 / fp16")
+    dt = _SEQ_DT.get(table.dtype)
+    if dt is None or table.dim() != 2 or table.numel() == 0:
+        raise ValueError("table: need [V,D] fp32 / bf16 / fp16")
     V, D = table.shape
-    _need(table.stride(1) == 1 or D == 1, "table: last dimension must be contiguous")
+    if table.stride(1) != 1 and D != 1:
+        raise ValueError("table: last dimension must be contiguous")
     if pos is not None:
-        _need(pos.dim() == 2 and pos.dtype == table.dtype and pos.shape[0] >= T and pos.shape[1] == D, f"pos: need [>= {T},{D}] in table's type")
-        _need(pos.stride(1) == 1 or D == 1, "pos: last dimension must be contiguous")
-    out = torch.empty((*ids.shape, D), dtype=table.dtype, device=table.device)
+        if pos.dim() != 2 or pos.dtype != table.dtype or pos.shape[0] < T or pos.shape[1] != D:
+            raise ValueError(f"pos: need [>= {T},{D}] in table's type")
+        if pos.stride(1) != 1 and D != 1:
+            raise ValueError("pos: last dimension must be contiguous")
+    out = table.new_empty((*ids.shape, D))
     if N:
         check(lib.v2a_embed_fwd(ids.data_ptr(), wide, table.data_ptr(), _p(pos), out.data_ptr(), N, T, V, D, table.stride(0), 0 if pos is None else pos.stride(0),
-                                _SEQ_DT[table.dtype], float(scale), _stream()), "embed_fwd")
+                                dt, scale, _stream()), "embed_fwd")
     return out
 
 
-@_on_device_of(0)
+@_on_device_of_first
 def embed_bwd(ids, dout, vocab, scale=1.0, pos_rows=None):
     """Gradient of embed_fwd: dout [..., T, D] -> (dtable [vocab,D], dpos [pos_rows,D] or None without pos_rows), in dout's type, summed in
     fp32 over the tokens of each row in a fixed order.  Rows that no token names are 0."""
     N, T, wide = _ids(ids)
     _same_device(ids, dout)
-    _need(dout.dim() == ids.dim() + 1 and dout.shape[:-1] == ids.shape and dout.shape[-1] > 0, "dout: need ids' shape and the width")
-    _need(dout.dtype in _SEQ_DT and dout.is_contiguous(), "dout: need contiguous fp32 / bf16 / fp16")
-    _need(0 < vocab < 2 ** 31 - 1, "vocab: 1 to 2^31 - 2")
-    _need(pos_rows is None or pos_rows >= T, "pos_rows: fewer than the tokens of a row")
-    D = dout.shape[-1]
-    dtable = torch.empty((vocab, D), dtype=dout.dtype, device=dout.device)
-    dpos = None if pos_rows is None else torch.empty((pos_rows, D), dtype=dout.dtype, device=dout.device)
-    nb = lib.v2a_embed_bwd_workspace_bytes(N, vocab, D, _SEQ_DT[dout.dtype])
-    ws = torch.empty(nb, dtype=torch.uint8, device=dout.device) if nb else None
-    check(lib.v2a_embed_bwd(ids.data_ptr(), wide, dout.data_ptr(), dtable.data_ptr(), _p(dpos), N, max(T, 1), vocab, D, pos_rows or 0, _SEQ_DT[dout.dtype],
-                            float(scale), _p(ws), nb, _stream()), "embed_bwd")
+    D = dout.shape[-1] if dout.dim() else 0
+    if dout.dim() != ids.dim() + 1 or dout.shape[:-1] != ids.shape or D == 0:
+        raise ValueError("dout: need ids' shape and the width")
+    dt = _SEQ_DT.get(dout.dtype)
+    if dt is None or not dout.is_contiguous():
+        raise ValueError("dout: need contiguous fp32 / bf16 / fp16")
+    if not 0 < vocab < 2 ** 31 - 1:
+        raise ValueError("vocab: 1 to 2^31 - 2")
+    if pos_rows is not None and not T <= pos_rows < 2 ** 31:
+        raise ValueError("pos_rows: fewer than the tokens of a row, or over 2^31")
+    dtable = dout.new_empty((vocab, D))
+    dpos = None if pos_rows is None else dout.new_empty((pos_rows, D))
+    nb = lib.v2a_embed_bwd_workspace_bytes(N, vocab, D, dt)
+    ws = dout.new_empty(nb, dtype=torch.uint8) if nb else None
+    check(lib.v2a_embed_bwd(ids.data_ptr(), wide, dout.data_ptr(), dtable.data_ptr(), _p(dpos), N, max(T, 1), vocab, D, pos_rows or 0, dt, scale, _p(ws), nb,
+                            _stream()), "embed_bwd")
     return dtable, dpos
