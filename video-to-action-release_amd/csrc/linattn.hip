@@ -326,19 +326,21 @@ template <int DT> __device__ __forceinline__ void la_store4(typename LaT<DT>::T*
     }
 }
 
-struct LaScan {
+struct LaDir {                  // one direction of the recurrence
     const float* init;          // state before the first chunk in scan order (NULL: 0)
     float* seg;                 // [B H][nseg][Dk][Dv]: local states of the segments (local) / states before them (otherwise, nseg > 1)
     float* seg_decay;           // [B H][nseg]
+    int rev, vx, vy, pad;       // rev: from the last chunk to the first; v: 16-byte loads allowed
+};
+struct LaScan {
+    LaDir dir[2];
     float* chunk;               // state before each chunk in scan order, [B H][NC][Dk][Dv] (NULL: not kept)
     float* last;                // state behind the last chunk (NULL)
     void* out;
-    int NC, cps, nseg, ndv, local, rev, vx, vy, vq, vo, vst;
+    int ndir;                   // 2: both directions, alternate workgroups
+    int NC, cps, nseg, ndv, local, vq, vo, vst;
 };
 
-// One workgroup walks the chunks of one segment of one (row, head) for NW * NT * 16 columns of the state, which stays in registers as
-// accumulators: wave w owns columns 16 NT w .. and all Dk rows.  OUT: the outputs too.  rev: the recurrence of the state's gradient, from the
-// last chunk to the first, E <- exp(G_64) E + scale sum_i exp(G_i) q_i dout_i^T (x = q, y = dout), else x = k, y = v.
 template <int DT, int DK, int NT, int NW, bool OUT> constexpr int la_scan_lds() {
     return LaTile<DT, DK>::BYTES * (OUT ? 2 : 1) + LaTile<DT, 16 * NT * NW>::BYTES + (OUT ? 6 * la_unit_bytes<DT>() : 0);
 }
@@ -362,16 +364,20 @@ __global__ __launch_bounds__(64 * NW, (la_scan_waves<DT, DK, NT, NW, OUT>())) vo
     char* sp = sq + QB;
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int blk = blockIdx.x;
+    const LaDir& m = p.dir[p.ndir == 2 ? blk & 1 : 0];
+    if (p.ndir == 2) blk >>= 1;
+    const int rev = m.rev;
     const int dvt = blk % p.ndv;
     blk /= p.ndv;
     const int seg = blk % p.nseg, bh = blk / p.nseg, b = bh / a.H, h = bh % a.H;
+    if (!OUT && p.local && seg == p.nseg - 1) return;      // nothing follows it
     const int len = la_len(a, b), Dk = a.Dk, Dv = a.Dv, dv0 = dvt * DVT + wid * NT * 16;
     const int hq = h / (a.H / a.Hq), hk = h / (a.H / a.Hk), hv = h / (a.H / a.Hv);
     const int yroom = Dv - dvt * DVT < DVT ? Dv - dvt * DVT : DVT;
-    const E* X = p.rev ? (const E*)a.q + b * a.qs[0] + hq * a.qs[2] : (const E*)a.k + b * a.ks[0] + hk * a.ks[2];
-    const E* Y = (p.rev ? (const E*)a.dout + b * a.ds[0] + h * a.ds[2] : (const E*)a.v + b * a.vs[0] + hv * a.vs[2]) + dvt * DVT;
+    const E* X = rev ? (const E*)a.q + b * a.qs[0] + hq * a.qs[2] : (const E*)a.k + b * a.ks[0] + hk * a.ks[2];
+    const E* Y = (rev ? (const E*)a.dout + b * a.ds[0] + h * a.ds[2] : (const E*)a.v + b * a.vs[0] + hv * a.vs[2]) + dvt * DVT;
     const E* Q = (const E*)a.q + b * a.qs[0] + hq * a.qs[2];
-    const long long sxt = p.rev ? a.qs[1] : a.ks[1], syt = p.rev ? a.ds[1] : a.vs[1];
+    const long long sxt = rev ? a.qs[1] : a.ks[1], syt = rev ? a.ds[1] : a.vs[1];
     const float* g = a.g + b * a.gs[0] + h * a.gs[2];
     const long long SS = (long long)Dk * Dv;
 
@@ -460,16 +466,16 @@ __global__ __launch_bounds__(64 * NW, (la_scan_waves<DT, DK, NT, NW, OUT>())) vo
     for (int i = 0; i < DK / 16; ++i)
 #pragma unroll
         for (int n = 0; n < NT; ++n) S[i][n] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (const float* s0 = p.local ? nullptr : seg ? p.seg + ((long long)bh * p.nseg + seg) * SS : p.init ? p.init + bh * SS : nullptr) get_state(s0);
+    if (const float* s0 = p.local ? nullptr : seg ? m.seg + ((long long)bh * p.nseg + seg) * SS : m.init ? m.init + bh * SS : nullptr) get_state(s0);
     LaLoad<DT, DK, NTH> rx, rq;
     LaLoad<DT, DVT, NTH> ry;
     float rg = 0.f;
     const int ibeg = seg * p.cps, iend = (seg + 1) * p.cps < p.NC ? (seg + 1) * p.cps : p.NC;
     // chunks with tokens: the first ones of the sequence.  The others leave the state as it is and are walked apart from the main loop, so
     // that the accumulators have one definition in it (a second path through the loop doubled their registers).
-    const int nvc = (len + LA_C - 1) / LA_C, vlo = p.rev ? p.NC - nvc : 0, vhi = p.rev ? p.NC : nvc;
+    const int nvc = (len + LA_C - 1) / LA_C, vlo = rev ? p.NC - nvc : 0, vhi = rev ? p.NC : nvc;
     const int vbeg = vlo > ibeg ? (vlo < iend ? vlo : iend) : ibeg, vend = vhi < iend ? (vhi > vbeg ? vhi : vbeg) : iend;
-    auto chunk_of = [&](int i) { return p.rev ? p.NC - 1 - i : i; };
+    auto chunk_of = [&](int i) { return rev ? p.NC - 1 - i : i; };
     auto valid = [&](int i) {
         const int n = len - chunk_of(i) * LA_C;
         return n > LA_C ? LA_C : n;
@@ -477,8 +483,8 @@ __global__ __launch_bounds__(64 * NW, (la_scan_waves<DT, DK, NT, NW, OUT>())) vo
     // The next chunk's rows are requested behind the score barrier: the work behind it is as long as the loads take, and their registers are
     // free before it.  Its decays are summed by the last wave meanwhile (gts[i & 1] belongs to chunk i), from values requested a chunk earlier.
     auto first = [&](int i) { return (long long)chunk_of(i) * LA_C; };
-    auto fetch_x = [&](int i) { if (i < vend) rx.load(X + first(i) * sxt, sxt, valid(i), Dk, p.vx); };
-    auto fetch_y = [&](int i) { if (i < vend) ry.load(Y + first(i) * syt, syt, valid(i), yroom, p.vy); };
+    auto fetch_x = [&](int i) { if (i < vend) rx.load(X + first(i) * sxt, sxt, valid(i), Dk, m.vx); };
+    auto fetch_y = [&](int i) { if (i < vend) ry.load(Y + first(i) * syt, syt, valid(i), yroom, m.vy); };
     auto fetch_q = [&](int i) { if constexpr (OUT) if (i < vend) rq.load(Q + first(i) * a.qs[1], a.qs[1], valid(i), Dk, p.vq); };
     auto fetch_g = [&](int i) { if (wid == NW - 1 && i < vend && lane < valid(i)) rg = g[(first(i) + lane) * a.gs[1]]; };
     auto gates = [&](int i) { if (wid == NW - 1 && i < vend) la_gates(gts[i & 1], rg, lane < valid(i), lane); };
@@ -512,7 +518,7 @@ __global__ __launch_bounds__(64 * NW, (la_scan_waves<DT, DK, NT, NW, OUT>())) vo
         if constexpr (OUT) rq.store(sq);
         __syncthreads();
         const LaGate& gt = gts[i & 1];
-        const bool live = i > vbeg || seg || p.init;                      // the state is not 0
+        const bool live = i > vbeg || seg || m.init;                      // the state is not 0
         const bool keep = !OUT || i + 1 < vend || p.last;                 // somebody reads it
         const int nks = nv > 32 ? 2 : 1;
         if constexpr (OUT) {
@@ -632,9 +638,9 @@ __global__ __launch_bounds__(64 * NW, (la_scan_waves<DT, DK, NT, NW, OUT>())) vo
 #pragma unroll 1
         for (int ks = 0; ks < nku; ++ks) {
             typename LaOp<DT>::C3 yw[NT];
-            const float* wsrc = (p.rev ? gt.wq : gt.wk) + ks * 32 + (lane >> 4) * 4;
+            const float* wsrc = (rev ? gt.wq : gt.wk) + ks * 32 + (lane >> 4) * 4;
             const float4 w0 = *(const float4*)wsrc, w1 = *(const float4*)(wsrc + 16);
-            const float sc = p.rev ? a.scale : 1.f;
+            const float sc = rev ? a.scale : 1.f;
             const float w[8] = {w0.x * sc, w0.y * sc, w0.z * sc, w0.w * sc, w1.x * sc, w1.y * sc, w1.z * sc, w1.w * sc};
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
@@ -662,13 +668,16 @@ __global__ __launch_bounds__(64 * NW, (la_scan_waves<DT, DK, NT, NW, OUT>())) vo
     }
     for (int i = vend; i < iend; ++i) skip(i);
     if (p.local) {
-        put_state(p.seg + ((long long)bh * p.nseg + seg) * SS);
-        if (threadIdx.x == 0 && dvt == 0) p.seg_decay[(long long)bh * p.nseg + seg] = fac;
+        put_state(m.seg + ((long long)bh * p.nseg + seg) * SS);
+        if (threadIdx.x == 0 && dvt == 0) m.seg_decay[(long long)bh * p.nseg + seg] = fac;
     } else if (p.last && iend == p.NC) put_state(p.last + bh * SS);
 }
 
 // Local states of the segments -> states before them: S_0 = init, S_{s+1} = decay_s S_s + local_s, in place
-__global__ __launch_bounds__(256) void la_combine(float* seg, const float* seg_decay, const float* init, int nseg, long long SS) {
+__global__ __launch_bounds__(256) void la_combine(LaScan p, int nseg, long long SS) {
+    const LaDir& m = p.dir[blockIdx.z];
+    float* const seg = m.seg;
+    const float *const seg_decay = m.seg_decay, *const init = m.init;
     const long long bh = blockIdx.y, e = (long long)blockIdx.x * 256 + threadIdx.x;
     if (e >= SS) return;
     float s = init ? init[bh * SS + e] : 0.f;
@@ -1297,7 +1306,7 @@ int la_vec(const void* p, const long long* st, int B, int T, int H, int D, int d
 }
 
 template <int DT, int DK, bool OUT> int la_scan_dv(const LaArgs& a, const LaScan& p, int dvt, hipStream_t s) {
-    const dim3 grid((unsigned)((long long)a.B * a.H * p.ndv * p.nseg));
+    const dim3 grid((unsigned)((long long)a.B * a.H * p.ndv * p.nseg * p.ndir));
     if (dvt == 32) hipLaunchKernelGGL((la_scan<DT, DK, 1, 2, OUT>), grid, dim3(128), 0, s, a, p);
     else if (dvt == 64) hipLaunchKernelGGL((la_scan<DT, DK, 1, 4, OUT>), grid, dim3(256), 0, s, a, p);
     else if constexpr (DK == 32 || (OUT && DT == 1)) hipLaunchKernelGGL((la_scan<DT, DK, 2, 4, OUT>), grid, dim3(256), 0, s, a, p);
@@ -1320,18 +1329,15 @@ int la_segments(const LaArgs& a, LaScan p, const LaPlan& pl, int dtype, hipStrea
     const int rc = la_launch_scan<false>(a, p, pl.dvt, dtype, s);
     if (rc != V2A_OK) return rc;
     const long long SS = (long long)a.Dk * a.Dv;
-    hipLaunchKernelGGL(la_combine, dim3(cdiv(SS, 256), (unsigned)(a.B * a.H)), dim3(256), 0, s, p.seg, p.seg_decay, p.init, pl.nseg, SS);
+    hipLaunchKernelGGL(la_combine, dim3(cdiv(SS, 256), (unsigned)(a.B * a.H), p.ndir), dim3(256), 0, s, p, pl.nseg, SS);
     V2A_CHECK_LAUNCH();
     return V2A_OK;
 }
-// A recurrence over the whole sequence
+// A recurrence over the whole sequence; the states before its segments are there
 template <bool OUT> int la_recur(const LaArgs& a, LaScan p, const LaPlan& pl, int dtype, hipStream_t s) {
-    p.vst = a.Dv % 4 == 0 && (((uintptr_t)p.init | (uintptr_t)p.last) & 15) == 0;      // the workspace is aligned
+    p.ndir = 1;
+    p.vst = a.Dv % 4 == 0 && (((uintptr_t)p.dir[0].init | (uintptr_t)p.last) & 15) == 0;      // the workspace is aligned
     p.NC = pl.NC; p.cps = pl.cps; p.nseg = pl.nseg; p.ndv = pl.ndv;
-    if (pl.nseg > 1) {
-        const int rc = la_segments(a, p, pl, dtype, s);
-        if (rc != V2A_OK) return rc;
-    }
     return la_launch_scan<OUT>(a, p, pl.dvt, dtype, s);
 }
 
@@ -1344,7 +1350,7 @@ LaFwdWs la_fwd_ws(const LaPlan& p, size_t BH, size_t SS) {
     }
     return w;
 }
-struct LaBwdWs { size_t seg, decay, sch, q, k, v, part, total; };
+struct LaBwdWs { size_t seg, decay, seg2, decay2, sch, q, k, v, part, total; };
 LaBwdWs la_bwd_ws(const LaPlan& p, size_t B, size_t T, size_t H, int Hq, int Hk, int Hv, size_t Dk, size_t Dv, int per_token) {
     LaBwdWs w{};
     const size_t SS = Dk * Dv, BH = B * H, n = B * T * H;
@@ -1352,6 +1358,8 @@ LaBwdWs la_bwd_ws(const LaPlan& p, size_t B, size_t T, size_t H, int Hq, int Hk,
     auto take = [&](size_t bytes) { const size_t o = at; at += la_up(bytes); return o; };
     w.seg = take(p.nseg > 1 ? BH * p.nseg * SS * 4 : 0);
     w.decay = take(p.nseg > 1 ? BH * p.nseg * 4 : 0);
+    w.seg2 = take(p.nseg > 1 ? BH * p.nseg * SS * 4 : 0);
+    w.decay2 = take(p.nseg > 1 ? BH * p.nseg * 4 : 0);
     w.sch = take(p.NC > 1 ? BH * p.NC * SS * 4 : 0);
     w.q = take((size_t)Hq < H ? n * Dk * 4 : 0);
     w.k = take((size_t)Hk < H ? n * Dk * 4 : 0);
@@ -1381,15 +1389,21 @@ int v2a_linattn_fwd(const void* q, const void* k, const void* v, const float* g,
     if (ws_bytes < w.total || (w.total && !ws)) return V2A_ERR_WORKSPACE;
     const LaArgs a = la_args(q, k, v, g, state, lens, nullptr, strides, B, T, H, Hq, Hk, Hv, Dk, Dv, scale);
     LaScan p{};
-    p.init = state;
-    p.seg = (float*)((char*)ws + w.seg);
-    p.seg_decay = (float*)((char*)ws + w.decay);
+    LaDir& m = p.dir[0];
+    m.init = state;
+    m.seg = (float*)((char*)ws + w.seg);
+    m.seg_decay = (float*)((char*)ws + w.decay);
+    m.vx = la_vec(k, a.ks, B, T, Hk, Dk, dtype);
+    m.vy = la_vec(v, a.vs, B, T, Hv, Dv, dtype);
+    p.ndir = 1;
     p.last = state_out;
     p.out = out;
-    p.vx = la_vec(k, a.ks, B, T, Hk, Dk, dtype);
-    p.vy = la_vec(v, a.vs, B, T, Hv, Dv, dtype);
     p.vq = la_vec(q, a.qs, B, T, Hq, Dk, dtype);
     p.vo = Dv % (dtype == 0 ? 4 : 8) == 0 && ((uintptr_t)out & 15) == 0;
+    if (pl.nseg > 1) {
+        const int rc = la_segments(a, p, pl, dtype, s);
+        if (rc != V2A_OK) return rc;
+    }
     return la_recur<true>(a, p, pl, dtype, s);
 }
 
@@ -1410,32 +1424,30 @@ int v2a_linattn_bwd(const void* q, const void* k, const void* v, const float* g,
     auto at = [&](size_t o) { return (float*)((char*)ws + o); };
     int rc = V2A_OK;
     if (B > 0) {
-        LaScan p{};
-        p.seg = at(w.seg);
-        p.seg_decay = at(w.decay);
         const int vq = la_vec(q, a.qs, B, T, Hq, Dk, dtype), vk = la_vec(k, a.ks, B, T, Hk, Dk, dtype), vv = la_vec(v, a.vs, B, T, Hv, Dv, dtype);
         const int vd = la_vec(dout, a.ds, B, T, H, Dv, dtype);
-        if (pl.NC > 1) {
-            LaScan f = p;
-            f.init = state; f.chunk = at(w.sch); f.vx = vk; f.vy = vv;
-            rc = la_recur<false>(a, f, pl, dtype, s);
+        LaScan p{};
+        p.dir[0] = LaDir{state, at(w.seg), at(w.decay), 0, vk, vv, 0};
+        p.dir[1] = LaDir{dstate_out, at(w.seg2), at(w.decay2), 1, vq, vd, 0};
+        if (pl.nseg > 1) {                   // states before the segments, and gradients of those behind them
+            p.ndir = 2;
+            rc = la_segments(a, p, pl, dtype, s);
             if (rc != V2A_OK) return rc;
         }
-        if (pl.nseg > 1) {
-            LaScan r = p;
-            r.init = dstate_out; r.rev = 1; r.vx = vq; r.vy = vd;
-            rc = la_segments(a, r, pl, dtype, s);
+        if (pl.NC > 1) {                     // states before the chunks
+            p.chunk = at(w.sch);
+            rc = la_recur<false>(a, p, pl, dtype, s);
             if (rc != V2A_OK) return rc;
         }
         if (T == 0 && dstate) {              // no tokens: the gradient passes through
-            LaScan r = p;
-            r.init = dstate_out; r.rev = 1; r.last = dstate;
+            LaScan r{};
+            r.dir[0] = p.dir[1]; r.last = dstate;
             rc = la_recur<false>(a, r, pl, dtype, s);
             if (rc != V2A_OK) return rc;
         }
         if (T > 0) {
             LaBwd d{};
-            d.s_chunk = at(w.sch); d.s_first = state; d.e_last = dstate_out; d.e_seg = at(w.seg); d.e_first = dstate;
+            d.s_chunk = at(w.sch); d.s_first = state; d.e_last = dstate_out; d.e_seg = at(w.seg2); d.e_first = dstate;
             d.cps = pl.cps; d.nseg = pl.nseg;
             d.fq = Hq < H; d.fk = Hk < H; d.fv = Hv < H;
             d.dq = d.fq ? (void*)at(w.q) : dq;

@@ -1537,15 +1537,24 @@ def _same_device(t, *others):
             raise ValueError("operands on different devices")
 
 
+_device_now = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
 def _on_device_of_first(fn):
     """Decorator: the first operand names the GPU the call runs on (the current one or not)."""
     @functools.wraps(fn)
     def call(t, *a, **kw):
-        if t.is_cuda and t.get_device() != torch.cuda.current_device():
-            with torch.cuda.device(t.device):
+        i = t.get_device()
+        if i >= 0 and i != _device_now():
+            with torch.cuda.device(i):
                 return fn(t, *a, **kw)
         return fn(t, *a, **kw)
     return call
+
+
+def _stream_of(t):
+    """Raw handle of torch's current stream on t's device, which is the current one here."""
+    return _raw_stream(t.get_device()) if _raw_stream is not None else _stream()
 
 
 def _la_heads(q, k, v, g, lead):
@@ -1613,7 +1622,7 @@ def linear_attention_fwd(q, k, v, log_decay, state=None, lens=None, scale=None, 
     ws = q.new_empty(nb, dtype=torch.uint8) if nb else None
     st = _I64x12(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *_g_strides(log_decay, 2))
     check(lib.v2a_linattn_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), _p(state), _p(lens), out.data_ptr(), _p(last), st, B, T, H,
-                              Hq, Hk, Hv, Dk, Dv, dt, Dk ** -0.5 if scale is None else scale, _p(ws), nb, _stream()), "linear_attention_fwd")
+                              Hq, Hk, Hv, Dk, Dv, dt, Dk ** -0.5 if scale is None else scale, _p(ws), nb, _stream_of(q)), "linear_attention_fwd")
     return out, last
 
 
@@ -1644,7 +1653,7 @@ def linear_attention_bwd(q, k, v, log_decay, dout, state=None, lens=None, scale=
     st = _I64x15(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *_g_strides(log_decay, 2), *dout.stride()[:3])
     check(lib.v2a_linattn_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), _p(state), _p(lens), dout.data_ptr(), _p(dstate), dq.data_ptr(),
                               dk.data_ptr(), dv.data_ptr(), dg.data_ptr(), _p(ds0), st, B, T, H, Hq, Hk, Hv, Dk, Dv, dt, tok,
-                              Dk ** -0.5 if scale is None else scale, _p(ws), nb, _stream()), "linear_attention_bwd")
+                              Dk ** -0.5 if scale is None else scale, _p(ws), nb, _stream_of(q)), "linear_attention_bwd")
     return dq, dk, dv, dg, ds0
 
 
@@ -1668,7 +1677,7 @@ def linear_attention_step(q, k, v, log_decay, state, slots=None, scale=None):
     out = q.new_empty((B, H, Dv))
     st = _I64x8(*q.stride()[:2], *k.stride()[:2], *v.stride()[:2], *_g_strides(log_decay, 1))
     check(lib.v2a_linattn_step(q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), state.data_ptr(), _p(slots), out.data_ptr(), st, B, N, H, Hq, Hk,
-                               Hv, Dk, Dv, dt, Dk ** -0.5 if scale is None else scale, _stream()), "linear_attention_step")
+                               Hv, Dk, Dv, dt, Dk ** -0.5 if scale is None else scale, _stream_of(q)), "linear_attention_step")
     return out
 
 
@@ -1700,7 +1709,7 @@ def embed_fwd(ids, table, scale=1.0, pos=None):
     out = table.new_empty((*ids.shape, D))
     if N:
         check(lib.v2a_embed_fwd(ids.data_ptr(), wide, table.data_ptr(), _p(pos), out.data_ptr(), N, T, V, D, table.stride(0), 0 if pos is None else pos.stride(0),
-                                dt, scale, _stream()), "embed_fwd")
+                                dt, scale, _stream_of(table)), "embed_fwd")
     return out
 
 
@@ -1725,5 +1734,5 @@ def embed_bwd(ids, dout, vocab, scale=1.0, pos_rows=None):
     nb = lib.v2a_embed_bwd_workspace_bytes(N, vocab, D, dt)
     ws = dout.new_empty(nb, dtype=torch.uint8) if nb else None
     check(lib.v2a_embed_bwd(ids.data_ptr(), wide, dout.data_ptr(), dtable.data_ptr(), _p(dpos), N, max(T, 1), vocab, D, pos_rows or 0, dt, scale, _p(ws), nb,
-                            _stream()), "embed_bwd")
+                            _stream_of(dout)), "embed_bwd")
     return dtable, dpos
