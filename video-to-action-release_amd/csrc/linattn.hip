@@ -1,14 +1,16 @@
 // Linear attention with a decay for each head:  S_t = a_t S_{t-1} + k_t v_t^T (fp32, Dk x Dv),  a_t = exp(g_t),  o_t = scale * S_t^T q_t.
 // Whole sequences (v2a_linattn_fwd / v2a_linattn_bwd) and single tokens on a pool of states (v2a_linattn_step).
 #include "common.h"
+#include <type_traits>
 
 namespace {
 
 constexpr int LA_DMAX = 128;            // largest head width
 constexpr float LA_GMIN = -1000.f;      // decays below exp(-1000) are 0 in fp32 already; the clamp makes -inf (a reset) ordinary arithmetic
 
-template <int DT> struct LaT;           // element types: 0 fp32, 1 bf16, 2 fp16
+template <int DT> struct LaT;           // element types: 0 fp32, 1 bf16, 2 fp16; in the chunked kernels also 3: fp32 computed in bf16 planes
 template <> struct LaT<0> { typedef float T; static __device__ __forceinline__ float ld(float x) { return x; } static __device__ __forceinline__ float st(float x) { return x; } };
+template <> struct LaT<3> : LaT<0> {};
 template <> struct LaT<1> { typedef unsigned short T; static __device__ __forceinline__ float ld(T x) { return v2a_h2f<false>(x); } static __device__ __forceinline__ T st(float x) { return v2a_f2h<false>(x); } };
 template <> struct LaT<2> { typedef unsigned short T; static __device__ __forceinline__ float ld(T x) { return v2a_h2f<true>(x); } static __device__ __forceinline__ T st(float x) { return v2a_f2h<true>(x); } };
 
@@ -38,7 +40,10 @@ __device__ __forceinline__ float la_clampg(float g) { return g < LA_GMIN ? LA_GM
 // 8 g ..: one 16-byte read of a row; the state's rows are dealt to its accumulators so that two of them are such an operand as well.
 // Number formats: bf16 inputs are one exact 8-bit plane, fp16 inputs two (8 + 3 bits, exact); factors computed in fp32 (scores, states)
 // are fed as two planes (off by at most 2^-17 of the value), decay-weighted values of the state update as three (exact fp32), because the
-// state is an fp32 result and lives long.  Sums are fp32.  fp32 inputs use the fp32 MFMA (16 x 16 x 4) in the same slot order.
+// state is an fp32 result and lives long.  Sums are fp32.  fp32 inputs are three planes in LDS, fp32 factors too, and a product is the six
+// plane products of 2^-16 and more (each dropped one is below 2^-24 of it): 96 cycles of the matrix unit against 256 of the fp32 MFMA.  Where
+// planes cost the second workgroup on a CU (heads up to 64 wide) or do not fit at all (the four tiles of the gradient), tiles stay fp32 and the
+// fp32 MFMA (16 x 16 x 4) takes them in the same slot order.
 // Running log decays are summed in fp64 and kept as a float pair: W of two tokens behind a reset (g clamped at -1000) keeps its digits.
 constexpr int LA_C = 64;
 #define LA_FENCE __builtin_amdgcn_sched_barrier(0)      // between stages: moved up, the next one's operands fill the registers
@@ -49,12 +54,13 @@ typedef __attribute__((address_space(3))) la_bf16x4 la_lds_bf16x4;
 
 template <int NP> struct LaP { la_u32x4 p[NP]; };      // eight values as NP bf16 planes
 struct LaF { float x[8]; };                            // eight fp32 values
-template <int DT> struct LaOp {                        // operand of an input tile; LDS bytes of a tile element
-    typedef LaP<DT == 2 ? 2 : 1> In;
-    typedef LaP<2> C2;
+template <int DT> struct LaOp {                        // operands: of an input tile, of a score or state, of a weighted value
+    static constexpr int NP = DT;
+    typedef LaP<NP> In;
+    typedef LaP<DT == 3 ? 3 : 2> C2;
     typedef LaP<3> C3;
-    static constexpr int NP = DT == 2 ? 2 : 1;
 };
+template <int DT> constexpr bool la_f32() { return DT == 0 || DT == 3; }      // element type
 template <> struct LaOp<0> {
     typedef LaF In;
     typedef LaF C2;
@@ -113,7 +119,7 @@ template <int A = 0, int B = 0, bool ALL = false> __device__ __forceinline__ voi
 }
 template <int DT> __device__ __forceinline__ void la_mma_in(f32x4& c, const typename LaOp<DT>::In& a, const typename LaOp<DT>::In& b) {
     if constexpr (DT == 0) la_mma(c, a, b);
-    else la_mma<LaOp<DT>::NP, LaOp<DT>::NP, true>(c, a, b);
+    else la_mma<LaOp<DT>::NP, LaOp<DT>::NP, DT != 3>(c, a, b);
 }
 
 // A 64 x D tile in LDS, rows padded by 16 bytes.  nat: lane % 16 = row, slots along the row; tr: lane % 16 = column, slots down the rows
@@ -177,7 +183,7 @@ template <typename T> __device__ __forceinline__ T* la_at(const void* base, unsi
 // and columns from Dx on are zeros and not read.  vec: base, strides and Dx allow 16-byte loads; else element by element.
 template <int DT, int D, int NTH> struct LaLoad {
     typedef typename LaT<DT>::T E;
-    static constexpr int EPC = DT == 0 ? 4 : 8, CPR = D / EPC, N = LA_C * CPR / NTH;
+    static constexpr int EPC = la_f32<DT>() ? 4 : 8, CPR = D / EPC, N = LA_C * CPR / NTH;
     static_assert(LA_C * CPR % NTH == 0, "whole 16-byte pieces per thread");
     static_assert(NTH % CPR == 0, "a thread's pieces share their columns");
     la_u32x4 r[N];
@@ -199,7 +205,7 @@ template <int DT, int D, int NTH> struct LaLoad {
 #pragma unroll
                     for (int e = 0; e < EPC; ++e)
                         if (c + e < Dx) {
-                            if constexpr (DT == 0) r[i][e] = __float_as_uint(q[e]);
+                            if constexpr (la_f32<DT>()) r[i][e] = __float_as_uint(q[e]);
                             else r[i][e >> 1] |= (unsigned int)q[e] << (16 * (e & 1));
                         }
                 }
@@ -211,7 +217,15 @@ template <int DT, int D, int NTH> struct LaLoad {
         char* q = t + threadIdx.x / CPR * TT::PITCH + (threadIdx.x % CPR) * EPC * (DT == 0 ? 4 : 2);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            if constexpr (DT == 2) {
+            if constexpr (DT == 3) {
+                unsigned int h[2], m[2], l[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) v2a_split3x2(__uint_as_float(r[i][2 * e]), __uint_as_float(r[i][2 * e + 1]), h[e], m[e], l[e]);
+                char* w = q + i * (NTH / CPR) * TT::PITCH;
+                *(la_u32x2*)w = la_u32x2{h[0], h[1]};
+                *(la_u32x2*)(w + TT::PLANE) = la_u32x2{m[0], m[1]};
+                *(la_u32x2*)(w + 2 * TT::PLANE) = la_u32x2{l[0], l[1]};
+            } else if constexpr (DT == 2) {
                 la_u32x4 hi, lo;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
@@ -275,7 +289,7 @@ __device__ constexpr int la_unit_tile(int u) { return u == 0 ? 0 : u == 1 ? 1 : 
 __device__ constexpr int la_unit_step(int u) { return u == 3 || u == 5 ? 1 : 0; }
 __device__ constexpr int la_unit_wave(int u, int nw) { return nw == 1 ? 0 : nw == 2 ? u / 3 : nw == 4 ? (u < 2 ? 0 : u < 4 ? 1 : u - 2) : u; }
 __device__ __forceinline__ int la_unit(int tile, int step) { return step == 0 ? (tile < 3 ? tile : 4) : tile == 2 ? 3 : 5; }
-template <int DT> constexpr int la_unit_bytes() { return 64 * 32; }      // two planes of 16 bytes a lane, or eight floats
+template <int DT> constexpr int la_unit_bytes() { return DT == 3 ? 64 * 48 : 64 * 32; }      // planes of 16 bytes a lane, or eight floats
 
 template <int DT> __device__ __forceinline__ void la_put(char* p, int u, int lane, const float* x) {
     typename LaOp<DT>::C2 o;
@@ -287,6 +301,7 @@ template <int DT> __device__ __forceinline__ void la_put(char* p, int u, int lan
     } else {
         q[0] = o.p[0];
         q[64] = o.p[1];
+        if constexpr (DT == 3) q[128] = o.p[2];
     }
 }
 template <int DT> __device__ __forceinline__ void la_get(const char* p, int u, int lane, typename LaOp<DT>::C2& o) {
@@ -298,6 +313,7 @@ template <int DT> __device__ __forceinline__ void la_get(const char* p, int u, i
     } else {
         o.p[0] = a;
         o.p[1] = b;
+        if constexpr (DT == 3) o.p[2] = q[128];
     }
 }
 
@@ -317,7 +333,7 @@ template <bool SLOTS_I> __device__ __forceinline__ void la_weights(const LaGate&
 
 template <int DT> __device__ __forceinline__ void la_store4(typename LaT<DT>::T* p, const f32x4& x, int room, bool vec) {
     if (vec && room >= 4) {
-        if constexpr (DT == 0) *(f32x4*)p = x;
+        if constexpr (la_f32<DT>()) *(f32x4*)p = x;
         else *(la_u32x2*)p = la_u32x2{v2a_pack_h2<DT == 2>(x[0], x[1]), v2a_pack_h2<DT == 2>(x[2], x[3])};
     } else {
 #pragma unroll
@@ -610,7 +626,7 @@ __global__ __launch_bounds__(64 * NW, (la_scan_waves<DT, DK, NT, NW, OUT>())) vo
 #pragma unroll
                         for (int n = 0; n < NT; ++n) O[n][it] = f32x4{0.f, 0.f, 0.f, 0.f};
                     E* q = la_at<E>(out + it * 16 * ot + dv0, ((unsigned)(lane & 15) * (unsigned)ot + (unsigned)((lane >> 4) * 4 * NT)) * (unsigned)sizeof(E));
-                    if constexpr (NT == 2 && DT != 0) {
+                    if constexpr (NT == 2 && !la_f32<DT>()) {
                         if (p.vo && d + 8 <= Dv) {
                             *(la_u32x4*)q = la_u32x4{v2a_pack_h2<DT == 2>(O[0][it][0], O[0][it][1]), v2a_pack_h2<DT == 2>(O[0][it][2], O[0][it][3]),
                                                      v2a_pack_h2<DT == 2>(O[1][it][0], O[1][it][1]), v2a_pack_h2<DT == 2>(O[1][it][2], O[1][it][3])};
@@ -673,26 +689,33 @@ __global__ __launch_bounds__(64 * NW, (la_scan_waves<DT, DK, NT, NW, OUT>())) vo
     } else if (p.last && iend == p.NC) put_state(p.last + bh * SS);
 }
 
-// Local states of the segments -> states before them: S_0 = init, S_{s+1} = decay_s S_s + local_s, in place
-__global__ __launch_bounds__(256) void la_combine(LaScan p, int nseg, long long SS) {
+// Local states of the segments -> states before them: S_0 = init, S_{s+1} = decay_s S_s + local_s, in place; W neighbours a lane, eight segments
+// a round and the next round's loads ahead of this one's stores
+template <int W>
+__global__ __launch_bounds__(64) void la_combine(LaScan p, int nseg, long long SS) {
+    typedef typename std::conditional<W == 4, f32x4, float>::type V;
     const LaDir& m = p.dir[blockIdx.z];
-    float* const seg = m.seg;
-    const float *const seg_decay = m.seg_decay, *const init = m.init;
-    const long long bh = blockIdx.y, e = (long long)blockIdx.x * 256 + threadIdx.x;
+    const long long bh = blockIdx.y, e = ((long long)blockIdx.x * 64 + threadIdx.x) * W;
     if (e >= SS) return;
-    float s = init ? init[bh * SS + e] : 0.f;
-    float* q = seg + bh * nseg * SS + e;
-    const float* f = seg_decay + bh * nseg;
-    for (int i0 = 0; i0 < nseg; i0 += 8) {
-        float x[8];
+    V s = m.init ? *(const V*)(m.init + bh * SS + e) : V{};
+    float* q = m.seg + bh * nseg * SS + e;
+    const float* f = m.seg_decay + bh * nseg;
+    V x[8], y[8];
+    auto get = [&](int i0, V (&v)[8]) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = i0 + j + 1 < nseg ? q[(i0 + j) * SS] : 0.f;
+        for (int j = 0; j < 8; ++j) v[j] = i0 + j + 1 < nseg ? *(const V*)(q + (i0 + j) * SS) : V{};
+    };
+    get(0, x);
+    for (int i0 = 0; i0 < nseg; i0 += 8) {
+        get(i0 + 8, y);
 #pragma unroll
         for (int j = 0; j < 8; ++j)
             if (i0 + j < nseg) {
-                q[(i0 + j) * SS] = s;
+                *(V*)(q + (i0 + j) * SS) = s;
                 s = s * f[i0 + j] + x[j];
             }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = y[j];
     }
 }
 
@@ -1280,9 +1303,10 @@ size_t la_up(size_t n) { return (n + 255) & ~(size_t)255; }
 struct LaPlan {
     int dvt, ndv, NC, cps, nseg;
 };
-LaPlan la_plan(int BH, int T, int Dv, int target, int least) {
+LaPlan la_plan(int BH, int T, int Dk, int Dv, int dtype, int target) {
+    constexpr int least = 2;
     LaPlan p;
-    p.dvt = Dv <= 32 ? 32 : Dv <= 64 ? 64 : 128;
+    p.dvt = Dv <= 32 ? 32 : Dv <= 64 || (dtype == 0 && Dk > 64) ? 64 : 128;
     p.ndv = cdiv(Dv, p.dvt);
     p.NC = cdiv(T, LA_C);
     p.nseg = 1;
@@ -1295,8 +1319,12 @@ LaPlan la_plan(int BH, int T, int Dv, int target, int least) {
     }
     return p;
 }
-LaPlan la_plan_fwd(int BH, int T, int Dv) { return la_plan(BH, T, Dv, 512, 2); }
-LaPlan la_plan_bwd(int BH, int T, int Dv) { return la_plan(BH, T, Dv, 512, 2); }
+// as many workgroups as fit the chip at once, by their LDS: two on a CU where they take 80 KB at most, else one.  More segments than that only
+// add states: 8 x 2048 tokens x 8 heads fp32 took 137 us with 256 workgroups, 144 with 512, 167 with 1024; 1 x 32768 x 8 bf16 182, 153, 180
+LaPlan la_plan_fwd(int BH, int T, int Dk, int Dv, int dtype) {
+    return la_plan(BH, T, Dk, Dv, dtype, dtype == 1 || (Dk <= 64 && Dv <= 64) ? 512 : 256);
+}
+LaPlan la_plan_bwd(int BH, int T, int Dk, int Dv, int dtype) { return la_plan(BH, T, Dk, Dv, dtype, Dk <= 32 && Dv <= 32 ? 512 : dtype == 1 && Dk <= 64 && Dv <= 64 ? 512 : 256); }
 
 int la_vec(const void* p, const long long* st, int B, int T, int H, int D, int dtype) {
     const long long es = dtype == 0 ? 4 : 2;
@@ -1305,20 +1333,34 @@ int la_vec(const void* p, const long long* st, int B, int T, int H, int D, int d
     return !((B > 1 && st[0] * es % 16) || (T > 1 && st[1] * es % 16) || (H > 1 && st[2] * es % 16));
 }
 
+// fp32 by the fp32 MFMA: where its tiles leave room for two workgroups on a CU and three planes of them do not (64 x 10 tokens x 8 heads of 48:
+// 10.6 us against 15.3; 8 x 2048 tokens x 8 heads 64 / 128, which do not fit twice either way: 100 us against 75)
+bool la_plain_fp32(int Dk, int dvt) { return Dk <= 64 && dvt <= 64; }
+
 template <int DT, int DK, bool OUT> int la_scan_dv(const LaArgs& a, const LaScan& p, int dvt, hipStream_t s) {
     const dim3 grid((unsigned)((long long)a.B * a.H * p.ndv * p.nseg * p.ndir));
-    if (dvt == 32) hipLaunchKernelGGL((la_scan<DT, DK, 1, 2, OUT>), grid, dim3(128), 0, s, a, p);
-    else if (dvt == 64) hipLaunchKernelGGL((la_scan<DT, DK, 1, 4, OUT>), grid, dim3(256), 0, s, a, p);
-    else if constexpr (DK == 32 || (OUT && DT == 1)) hipLaunchKernelGGL((la_scan<DT, DK, 2, 4, OUT>), grid, dim3(256), 0, s, a, p);
-    else hipLaunchKernelGGL((la_scan<DT, DK, 1, 8, OUT>), grid, dim3(512), 0, s, a, p);
+    if constexpr (!(DT == 3 && DK < 128)) {
+        if (dvt == 32) hipLaunchKernelGGL((la_scan<DT, DK, 1, 2, OUT>), grid, dim3(128), 0, s, a, p);
+        else if (dvt == 64) hipLaunchKernelGGL((la_scan<DT, DK, 1, 4, OUT>), grid, dim3(256), 0, s, a, p);
+    }
+    if constexpr (DT != 0 && !(DT == 3 && DK == 128)) {      // fp32: planes of 128 columns, and of 64 beside keys over 64 wide (all three tiles: 157 KB)
+        if (dvt == 128) {
+            if constexpr (DK == 32 || (OUT && DT == 1)) hipLaunchKernelGGL((la_scan<DT, DK, 2, 4, OUT>), grid, dim3(256), 0, s, a, p);
+            else hipLaunchKernelGGL((la_scan<DT, DK, 1, 8, OUT>), grid, dim3(512), 0, s, a, p);
+        }
+    }
     V2A_CHECK_LAUNCH();
     return V2A_OK;
 }
 template <int DT, bool OUT> int la_scan_dk(const LaArgs& a, const LaScan& p, int dvt, hipStream_t s) {
-    return a.Dk <= 32 ? la_scan_dv<DT, 32, OUT>(a, p, dvt, s) : a.Dk <= 64 ? la_scan_dv<DT, 64, OUT>(a, p, dvt, s) : la_scan_dv<DT, 128, OUT>(a, p, dvt, s);
+    if (a.Dk <= 32) return la_scan_dv<DT, 32, OUT>(a, p, dvt, s);
+    if (a.Dk <= 64) return la_scan_dv<DT, 64, OUT>(a, p, dvt, s);
+    if constexpr (DT == 0) return V2A_ERR_ARG;      // la_plain_fp32
+    else return la_scan_dv<DT, 128, OUT>(a, p, dvt, s);
 }
 template <bool OUT> int la_launch_scan(const LaArgs& a, const LaScan& p, int dvt, int dtype, hipStream_t s) {
-    return dtype == 0 ? la_scan_dk<0, OUT>(a, p, dvt, s) : dtype == 1 ? la_scan_dk<1, OUT>(a, p, dvt, s) : la_scan_dk<2, OUT>(a, p, dvt, s);
+    if (dtype == 0) return la_plain_fp32(a.Dk, dvt) ? la_scan_dk<0, OUT>(a, p, dvt, s) : la_scan_dk<3, OUT>(a, p, dvt, s);
+    return dtype == 1 ? la_scan_dk<1, OUT>(a, p, dvt, s) : la_scan_dk<2, OUT>(a, p, dvt, s);
 }
 
 // States before the segments: local ones, then their combination
@@ -1329,7 +1371,10 @@ int la_segments(const LaArgs& a, LaScan p, const LaPlan& pl, int dtype, hipStrea
     const int rc = la_launch_scan<false>(a, p, pl.dvt, dtype, s);
     if (rc != V2A_OK) return rc;
     const long long SS = (long long)a.Dk * a.Dv;
-    hipLaunchKernelGGL(la_combine, dim3(cdiv(SS, 256), (unsigned)(a.B * a.H), p.ndir), dim3(256), 0, s, p, pl.nseg, SS);
+    const uintptr_t at = (uintptr_t)p.dir[0].init | (uintptr_t)(p.ndir == 2 ? p.dir[1].init : nullptr);
+    if (SS % 4 == 0 && (at & 15) == 0)
+        hipLaunchKernelGGL((la_combine<4>), dim3(cdiv(SS, 256), (unsigned)(a.B * a.H), p.ndir), dim3(64), 0, s, p, pl.nseg, SS);
+    else hipLaunchKernelGGL((la_combine<1>), dim3(cdiv(SS, 64), (unsigned)(a.B * a.H), p.ndir), dim3(64), 0, s, p, pl.nseg, SS);
     V2A_CHECK_LAUNCH();
     return V2A_OK;
 }
@@ -1375,7 +1420,7 @@ extern "C" {
 
 size_t v2a_linattn_fwd_workspace_bytes(int B, int T, int H, int Dk, int Dv, int dtype) {
     if (!la_dims(B, T, H, H, H, H, Dk, Dv, dtype) || B == 0) return 0;
-    return la_fwd_ws(la_plan_fwd(B * H, T, Dv), (size_t)B * H, (size_t)Dk * Dv).total;
+    return la_fwd_ws(la_plan_fwd(B * H, T, Dk, Dv, dtype), (size_t)B * H, (size_t)Dk * Dv).total;
 }
 
 int v2a_linattn_fwd(const void* q, const void* k, const void* v, const float* g, const float* state, const int32_t* lens, void* out, float* state_out,
@@ -1384,7 +1429,7 @@ int v2a_linattn_fwd(const void* q, const void* k, const void* v, const float* g,
     if (!strides || !la_dims(B, T, H, Hq, Hk, Hv, Dk, Dv, dtype)) return V2A_ERR_ARG;
     if (B == 0 || (T == 0 && !state_out)) return V2A_OK;
     if (T > 0 && (!q || !k || !v || !g || !out)) return V2A_ERR_ARG;
-    const LaPlan pl = la_plan_fwd(B * H, T, Dv);
+    const LaPlan pl = la_plan_fwd(B * H, T, Dk, Dv, dtype);
     const LaFwdWs w = la_fwd_ws(pl, (size_t)B * H, (size_t)Dk * Dv);
     if (ws_bytes < w.total || (w.total && !ws)) return V2A_ERR_WORKSPACE;
     const LaArgs a = la_args(q, k, v, g, state, lens, nullptr, strides, B, T, H, Hq, Hk, Hv, Dk, Dv, scale);
@@ -1409,7 +1454,7 @@ int v2a_linattn_fwd(const void* q, const void* k, const void* v, const float* g,
 
 size_t v2a_linattn_bwd_workspace_bytes(int B, int T, int H, int Hq, int Hk, int Hv, int Dk, int Dv, int dtype, int per_token_decay) {
     if (!la_dims(B, T, H, Hq, Hk, Hv, Dk, Dv, dtype)) return 0;
-    return la_bwd_ws(la_plan_bwd(B * H, T, Dv), B, T, H, Hq, Hk, Hv, Dk, Dv, per_token_decay).total;
+    return la_bwd_ws(la_plan_bwd(B * H, T, Dk, Dv, dtype), B, T, H, Hq, Hk, Hv, Dk, Dv, per_token_decay).total;
 }
 
 int v2a_linattn_bwd(const void* q, const void* k, const void* v, const float* g, const float* state, const int32_t* lens, const void* dout,
@@ -1417,7 +1462,7 @@ int v2a_linattn_bwd(const void* q, const void* k, const void* v, const float* g,
                     int Hv, int Dk, int Dv, int dtype, int per_token_decay, float scale, void* ws, size_t ws_bytes, hipStream_t s) {
     if (!strides || !la_dims(B, T, H, Hq, Hk, Hv, Dk, Dv, dtype)) return V2A_ERR_ARG;
     if (B > 0 && T > 0 && (!q || !k || !v || !g || !dout || !dq || !dk || !dv)) return V2A_ERR_ARG;
-    const LaPlan pl = la_plan_bwd(B * H, T, Dv);
+    const LaPlan pl = la_plan_bwd(B * H, T, Dk, Dv, dtype);
     const LaBwdWs w = la_bwd_ws(pl, B, T, H, Hq, Hk, Hv, Dk, Dv, per_token_decay);
     if (ws_bytes < w.total || (w.total && !ws)) return V2A_ERR_WORKSPACE;
     const LaArgs a = la_args(q, k, v, g, state, lens, dout, strides, B, T, H, Hq, Hk, Hv, Dk, Dv, scale);
@@ -1459,12 +1504,11 @@ int v2a_linattn_bwd(const void* q, const void* k, const void* v, const float* g,
             d.vst = Dv % 4 == 0 && (((uintptr_t)state | (uintptr_t)dstate_out | (uintptr_t)dstate) & 15) == 0;
             const dim3 grid((unsigned)((long long)B * H * pl.nseg));
             const int Dm = Dk > Dv ? Dk : Dv;
-#define CALL(DT)                                                                                                        \
-    if (Dm <= 32) hipLaunchKernelGGL((la_bwd_chunks<DT, 32>), grid, dim3(128), 0, s, a, d);                              \
-    else if (Dm <= 64) hipLaunchKernelGGL((la_bwd_chunks<DT, 64>), grid, dim3(256), 0, s, a, d);                         \
-    else hipLaunchKernelGGL((la_bwd_chunks<DT, 128>), grid, dim3(512), 0, s, a, d)
-            LA_BY_TYPE(dtype, CALL);
-#undef CALL
+#define BWD(DT, D) hipLaunchKernelGGL((la_bwd_chunks<DT, D>), grid, dim3(4 * D), 0, s, a, d)
+            if (Dm <= 32) { if (dtype == 0) BWD(0, 32); else if (dtype == 1) BWD(1, 32); else BWD(2, 32); }
+            else if (Dm <= 64) { if (dtype == 0) BWD(0, 64); else if (dtype == 1) BWD(1, 64); else BWD(2, 64); }
+            else { if (dtype == 0) BWD(0, 128); else if (dtype == 1) BWD(1, 128); else BWD(2, 128); }
+#undef BWD
             V2A_CHECK_LAUNCH();
             const long long rows = (long long)B * T;
 #define CALL(DT)                                                                                                                               \
