@@ -12,7 +12,7 @@
 
 namespace {
 
-constexpr int EM_SORT_T = 1024, EM_WAVES = EM_SORT_T / 64, EM_KPT = 4, EM_SMALL = EM_SORT_T * EM_KPT, EM_BINS = 1024, EM_TILES = 64;
+constexpr int EM_SORT_T = 1024, EM_WAVES = EM_SORT_T / 64, EM_KPT = 4, EM_SUB = EM_SORT_T * EM_KPT, EM_SMALL = 2 * EM_SUB, EM_BINS = 1024, EM_TILES = 64;
 
 template <int DT> struct EmT { typedef unsigned short T; static constexpr int EPC = 8; };
 template <> struct EmT<0> { typedef float T; static constexpr int EPC = 4; };
@@ -102,11 +102,12 @@ struct EmSort {
     unsigned* hist;                         // [ntiles][2^bits]
 };
 
-// Stable rank of each of this wave's 64 * EM_KPT keys (key j of lane l is number 64 j + l) among the wave's equal digits, which also counts
+// Stable rank of each of this wave's 64 * KPT keys (key j of lane l is number 64 j + l) among the wave's equal digits, which also counts
 // them: lanes with the digit's bits all equal find each other by ballots.
-__device__ __forceinline__ void em_wave_rank(const unsigned (&dig)[EM_KPT], const bool (&on)[EM_KPT], int bits, unsigned short* count, int lane, unsigned (&rank)[EM_KPT]) {
+template <int KPT>
+__device__ __forceinline__ void em_wave_rank(const unsigned (&dig)[KPT], const bool (&on)[KPT], int bits, unsigned short* count, int lane, unsigned (&rank)[KPT]) {
 #pragma unroll
-    for (int j = 0; j < EM_KPT; ++j) {
+    for (int j = 0; j < KPT; ++j) {
         unsigned long long same = __ballot(on[j]);
         for (int b = 0; b < bits; ++b) {
             const unsigned long long m = __ballot((dig[j] >> b) & 1);
@@ -158,12 +159,13 @@ struct EmSortLds {
 
 // up to EM_SMALL tokens: one workgroup, all digits, through LDS
 __device__ void em_sort_small(const EmSort& s, EmSortLds& L, unsigned (*xch)[EM_SMALL]) {
+    constexpr int KPT = EM_SMALL / EM_SORT_T;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, bins = 1 << s.bits;
-    unsigned key[EM_KPT], pos[EM_KPT];
-    bool on[EM_KPT];
+    unsigned key[KPT], pos[KPT];
+    bool on[KPT];
 #pragma unroll
-    for (int j = 0; j < EM_KPT; ++j) {
-        const unsigned i = w * 64 * EM_KPT + j * 64 + lane;
+    for (int j = 0; j < KPT; ++j) {
+        const unsigned i = w * 64 * KPT + j * 64 + lane;
         on[j] = i < s.N;
         pos[j] = i;
         key[j] = on[j] ? em_key(s.ids, s.wide, i, s.V) : 0u;
@@ -171,9 +173,9 @@ __device__ void em_sort_small(const EmSort& s, EmSortLds& L, unsigned (*xch)[EM_
     for (int p = 0; p < s.passes; ++p) {
         for (int i = threadIdx.x; i < EM_WAVES * EM_BINS / 2; i += EM_SORT_T) ((unsigned*)L.count)[i] = 0u;
         __syncthreads();
-        unsigned dig[EM_KPT], rank[EM_KPT];
+        unsigned dig[KPT], rank[KPT];
 #pragma unroll
-        for (int j = 0; j < EM_KPT; ++j) dig[j] = (key[j] >> (p * s.bits)) & (bins - 1);
+        for (int j = 0; j < KPT; ++j) dig[j] = (key[j] >> (p * s.bits)) & (bins - 1);
         em_wave_rank(dig, on, s.bits, L.count[w], lane, rank);
         __syncthreads();
         unsigned total = 0;
@@ -182,7 +184,7 @@ __device__ void em_sort_small(const EmSort& s, EmSortLds& L, unsigned (*xch)[EM_
         L.base[threadIdx.x] = em_scan(total, L.tmp);
         __syncthreads();
 #pragma unroll
-        for (int j = 0; j < EM_KPT; ++j)
+        for (int j = 0; j < KPT; ++j)
             if (on[j]) {
                 const unsigned d = L.base[dig[j]] + L.count[w][dig[j]] + rank[j];
                 xch[0][d] = key[j];
@@ -190,8 +192,8 @@ __device__ void em_sort_small(const EmSort& s, EmSortLds& L, unsigned (*xch)[EM_
             }
         __syncthreads();
 #pragma unroll
-        for (int j = 0; j < EM_KPT; ++j) {
-            const unsigned i = w * 64 * EM_KPT + j * 64 + lane;
+        for (int j = 0; j < KPT; ++j) {
+            const unsigned i = w * 64 * KPT + j * 64 + lane;
             if (on[j]) {
                 key[j] = xch[0][i];
                 pos[j] = xch[1][i];
@@ -200,8 +202,8 @@ __device__ void em_sort_small(const EmSort& s, EmSortLds& L, unsigned (*xch)[EM_
         __syncthreads();
     }
 #pragma unroll
-    for (int j = 0; j < EM_KPT; ++j) {
-        const unsigned i = w * 64 * EM_KPT + j * 64 + lane;
+    for (int j = 0; j < KPT; ++j) {
+        const unsigned i = w * 64 * KPT + j * 64 + lane;
         if (on[j]) {
             s.key[i] = key[j];
             s.pos[i] = pos[j];
@@ -242,7 +244,7 @@ __global__ __launch_bounds__(EM_SORT_T) void embed_scatter_kernel(EmSort s, int 
     const unsigned start = em_scan(total, L.tmp) + before;
     L.base[threadIdx.x] = start;
     const unsigned a = blockIdx.x * s.tile, end = s.N - a < s.tile ? s.N : a + s.tile;
-    for (unsigned a0 = a; a0 < end; a0 += EM_SMALL) {
+    for (unsigned a0 = a; a0 < end; a0 += EM_SUB) {
         for (int i = threadIdx.x; i < EM_WAVES * EM_BINS / 2; i += EM_SORT_T) ((unsigned*)L.count)[i] = 0u;
         unsigned key[EM_KPT], pos[EM_KPT], dig[EM_KPT], rank[EM_KPT];
         bool on[EM_KPT];
@@ -412,56 +414,69 @@ __global__ __launch_bounds__(256) void embed_pieces_kernel(const unsigned* key, 
     else whole();
 }
 
-// Rows that cross pieces: the piece in which one begins adds its part 1 and the parts 0 of the pieces behind it, wave w those of w, w + 16, ..
-// One workgroup per (16 pieces, 256 columns), most of which have nothing to do; a run's end is found first, 64 borders at a time, so that the
-// sum has known bounds and eight loads under way.
-constexpr int EM_JOIN = 16;
+// Rows that cross pieces: the piece in which one begins adds its part 1 and the parts 0 of the pieces behind it, in order.  One wave per
+// (piece, 256 columns), most of which have nothing to do; a run's end is found first, 64 borders at a time, so that the sum has known bounds and
+// loads under way.  Runs over more than EM_LONG pieces are left to the whole workgroup: wave w adds pieces w, w + 16, .., the sums of the waves
+// in order.  (All runs by the workgroup, one after the other, took 22 us where many short ones lie close together, against 10.)
+constexpr int EM_JOIN = 16, EM_LONG = 32;
 template <int DT>
-__global__ __launch_bounds__(1024) void embed_join_kernel(const unsigned* key, EmGrad g, EmShape e, const float* part, int Dp, unsigned ts) {
+__global__ __launch_bounds__(64 * EM_JOIN) void embed_join_kernel(const unsigned* key, EmGrad g, EmShape e, const float* part, int Dp, unsigned ts) {
     typedef typename EmT<DT>::T E;
-    constexpr int NWV = 16;
-    __shared__ float sum[NWV][256];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    __shared__ float sum[EM_JOIN][256];
+    __shared__ unsigned ends[EM_JOIN], ids[EM_JOIN];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const unsigned np = (e.N - 1) / ts + 1;
-    const unsigned long long mine = (unsigned long long)blockIdx.x * EM_JOIN + lane, b = (mine + 1) * ts;
-    bool owns = false;
-    unsigned id = 0;
-    if (lane < EM_JOIN && b < e.N) {
-        const size_t a = mine * ts;
-        id = key[b - 1];
-        owns = id < e.V && key[b] == id && !(key[a] == id && a > 0 && key[a - 1] == id);
-    }
-    for (unsigned long long todo = __ballot(owns); todo; todo &= todo - 1) {
-        const int at = __ffsll((unsigned long long)todo) - 1;
-        const unsigned t = blockIdx.x * EM_JOIN + at, cur = __shfl(id, at, 64);
-        unsigned lo = t + 2, hi = np;          // the first piece from t + 2 on that begins with another id lies in [lo, hi]
-        while (lo < hi) {
-            const unsigned step = (hi - lo + 63) / 64, i = lo + lane * step;
-            const unsigned n = __popcll(__ballot(i < hi && key[(size_t)i * ts] == cur));      // sorted: a prefix of the probes
-            if (n == 0) { hi = lo; break; }
-            const unsigned top = lo + n * step;
-            lo = lo + (n - 1) * step + 1;
-            hi = top < hi ? top : hi;
-        }
-        const unsigned end = hi;
-        const int c0 = blockIdx.y * 256, c = c0 + lane * 4;
-        float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (c < e.D) {
-            if (w == 0) s = *(const float4*)(part + ((size_t)t * 2 + 1) * Dp + c);
-#pragma unroll 8
-            for (unsigned i = t + 1 + w; i < end; i += NWV) {
-                const float4 x = *(const float4*)(part + (size_t)i * 2 * Dp + c);
-                s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
+    const unsigned long long t = (unsigned long long)blockIdx.x * EM_JOIN + w, a = t * ts, b = a + ts;
+    const int c0 = blockIdx.y * 256, c = c0 + lane * 4;
+    const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto add = [](float4& s, const float4& x) { s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w; };
+    unsigned end = 0, cur = 0;
+    if (b < e.N) {
+        cur = key[b - 1];
+        const bool owns = cur < e.V && key[b] == cur && !(key[a] == cur && a > 0 && key[a - 1] == cur);
+        if (owns) {
+            unsigned lo = (unsigned)t + 2, hi = np;      // the first piece from t + 2 on that begins with another id lies in [lo, hi]
+            while (lo < hi) {
+                const unsigned step = (hi - lo + 63) / 64, i = lo + lane * step;
+                const unsigned n = __popcll(__ballot(i < hi && key[(size_t)i * ts] == cur));      // sorted: a prefix of the probes
+                if (n == 0) { hi = lo; break; }
+                const unsigned top = lo + n * step;
+                lo = lo + (n - 1) * step + 1;
+                hi = top < hi ? top : hi;
             }
-            *(float4*)&sum[w][lane * 4] = s;
+            end = hi;
         }
+    }
+    const bool wide = end > t + 1 + EM_LONG;
+    if (lane == 0) { ends[w] = wide ? end : 0u; ids[w] = cur; }
+    if (end && !wide && c < e.D) {
+        float4 s = *(const float4*)(part + (t * 2 + 1) * Dp + c);
+#pragma unroll 8
+        for (unsigned i = (unsigned)t + 1; i < end; ++i) add(s, *(const float4*)(part + (size_t)i * 2 * Dp + c));
+        const float x[4] = {s.x, s.y, s.z, s.w};
+        E* q = (E*)g.dtable + (size_t)cur * e.D + c;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (c + r < e.D) q[r] = em_r<DT>(x[r] * g.scale);
+    }
+    __syncthreads();
+    for (int o = 0; o < EM_JOIN; ++o) {
+        if (ends[o] == 0) continue;
+        const size_t t0 = (size_t)blockIdx.x * EM_JOIN + o;
+        float4 s = zero;
+        if (c < e.D) {
+            if (w == 0) s = *(const float4*)(part + (t0 * 2 + 1) * Dp + c);
+#pragma unroll 8
+            for (unsigned i = (unsigned)t0 + 1 + w; i < ends[o]; i += EM_JOIN) add(s, *(const float4*)(part + (size_t)i * 2 * Dp + c));
+        }
+        *(float4*)&sum[w][lane * 4] = s;
         __syncthreads();
         const int d = threadIdx.x;
         if (d < 256 && c0 + d < e.D) {
             float y = sum[0][d];
 #pragma unroll
-            for (int i = 1; i < NWV; ++i) y += sum[i][d];
-            ((E*)g.dtable)[(size_t)cur * e.D + c0 + d] = em_r<DT>(y * g.scale);
+            for (int i = 1; i < EM_JOIN; ++i) y += sum[i][d];
+            ((E*)g.dtable)[(size_t)ids[o] * e.D + c0 + d] = em_r<DT>(y * g.scale);
         }
         __syncthreads();
     }
@@ -556,7 +571,7 @@ int v2a_embed_bwd(const void* ids, int ids64, const void* dout, void* dtable, vo
     q.key = (unsigned*)(base + w.key); q.pos = (unsigned*)(base + w.pos);
     q.key2 = (unsigned*)(base + w.key2); q.pos2 = (unsigned*)(base + w.pos2);
     q.hist = (unsigned*)(base + w.hist);
-    q.tile = EM_SMALL;
+    q.tile = EM_SUB;
     while (cdiv(N, q.tile) > EM_TILES) q.tile *= 2;
     q.ntiles = cdiv(N, q.tile);
     EmGrad g{};
@@ -588,7 +603,7 @@ int v2a_embed_bwd(const void* ids, int ids64, const void* dout, void* dtable, vo
 #undef CALL
     V2A_CHECK_LAUNCH();
     if (pieces > 1) {
-#define CALL(DT, W) hipLaunchKernelGGL((embed_join_kernel<DT>), dim3(cdiv(pieces - 1, EM_JOIN), cdiv(D, 256)), dim3(1024), 0, s, q.key, g, e, (const float*)(base + w.part), w.Dp, w.ts)
+#define CALL(DT, W) hipLaunchKernelGGL((embed_join_kernel<DT>), dim3(cdiv(pieces - 1, EM_JOIN), cdiv(D, 256)), dim3(64 * EM_JOIN), 0, s, q.key, g, e, (const float*)(base + w.part), w.Dp, w.ts)
         EM_BY_TYPE(dtype, false, CALL);
 #undef CALL
         V2A_CHECK_LAUNCH();

@@ -88,10 +88,10 @@ __device__ __forceinline__ void la_split(const float* x, LaF& o) {
 template <int NP> __device__ __forceinline__ void la_join(const LaP<NP>& o, float* x) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        x[2 * e] = 0.f;
-        x[2 * e + 1] = 0.f;
+        x[2 * e] = __uint_as_float(o.p[NP - 1][e] << 16);
+        x[2 * e + 1] = __uint_as_float(o.p[NP - 1][e] & 0xffff0000u);
 #pragma unroll
-        for (int n = NP - 1; n >= 0; --n) {
+        for (int n = NP - 2; n >= 0; --n) {
             x[2 * e] += __uint_as_float(o.p[n][e] << 16);
             x[2 * e + 1] += __uint_as_float(o.p[n][e] & 0xffff0000u);
         }
@@ -160,9 +160,11 @@ template <int DT, int D> struct LaTile {
             const float4 a = *(const float4*)(q + col * 4);
             x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
         } else {
-            x[0] = x[1] = x[2] = x[3] = 0.f;
+            const la_u32x2 z = *(const la_u32x2*)(q + (NP - 1) * PLANE + col * 2);
+            x[0] = __uint_as_float(z[0] << 16); x[1] = __uint_as_float(z[0] & 0xffff0000u);
+            x[2] = __uint_as_float(z[1] << 16); x[3] = __uint_as_float(z[1] & 0xffff0000u);
 #pragma unroll
-            for (int n = NP - 1; n >= 0; --n) {
+            for (int n = NP - 2; n >= 0; --n) {
                 const la_u32x2 a = *(const la_u32x2*)(q + n * PLANE + col * 2);
                 x[0] += __uint_as_float(a[0] << 16); x[1] += __uint_as_float(a[0] & 0xffff0000u);
                 x[2] += __uint_as_float(a[1] << 16); x[3] += __uint_as_float(a[1] & 0xffff0000u);
@@ -924,8 +926,7 @@ __global__ __launch_bounds__(4 * D) void la_bwd_chunks(LaArgs a, LaBwd p) {
                 if ((NBUF == 3 && NW == 8 ? 6 + u / 3 : la_unit_wave(u, NW)) != wid || it * 16 >= nv) continue;
                 f32x4 c0 = {0.f, 0.f, 0.f, 0.f}, c1 = {0.f, 0.f, 0.f, 0.f};
                 const bool two = js + 16 <= it * 16;
-#pragma unroll 2
-                for (int kk = 0; kk < KK; ++kk) {
+                for (int kk = 0; kk * 32 < Dv; ++kk) {
                     typename LaOp<DT>::In df, vf;
                     TT::nat(sd, it * 16, kk, lane, df);
                     TT::nat(sv, js, kk, lane, vf);
@@ -947,7 +948,7 @@ __global__ __launch_bounds__(4 * D) void la_bwd_chunks(LaArgs a, LaBwd p) {
             }
         };
         // W (x . y) with lane = j, slots = i: the operands of dk (x = do, y = v) and dv (x = q, y = k); unit u is tile 3 - tile(u), step 1 - step(u)
-        auto unit23 = [&](const char* sx, const char* sy, char* dst, bool third) __attribute__((always_inline)) {
+        auto unit23 = [&](const char* sx, const char* sy, char* dst, int Dx, bool third) __attribute__((always_inline)) {
 #pragma unroll
             for (int u = 0; u < 6; ++u) {
                 const int jt = 3 - la_unit_tile(u), is = 32 - la_unit_step(u) * 32;
@@ -956,8 +957,7 @@ __global__ __launch_bounds__(4 * D) void la_bwd_chunks(LaArgs a, LaBwd p) {
                 if (la_unit_wave(u, NW) != wid || jt * 16 >= nv || is >= nv) continue;
                 f32x4 c0 = {0.f, 0.f, 0.f, 0.f}, c1 = {0.f, 0.f, 0.f, 0.f};
                 const bool first = is + 16 > jt * 16;
-#pragma unroll 2
-                for (int kk = 0; kk < KK; ++kk) {
+                for (int kk = 0; kk * 32 < Dx; ++kk) {
                     typename LaOp<DT>::In xf, yf;
                     TT::nat(sy, jt * 16, kk, lane, yf);
                     if (first) {
@@ -1002,14 +1002,15 @@ __global__ __launch_bounds__(4 * D) void la_bwd_chunks(LaArgs a, LaBwd p) {
 #pragma unroll
             for (int t = 0; t < 4; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
         };
-        // a state's rows (or columns) times the tokens' rows in `t`, weighted by w
-        auto through = [&](const f32x4 (&x)[KK][2], const char* t, const float* w, float mul) __attribute__((always_inline)) {
+        // a state's rows (or columns) times the tokens' rows in `t`, weighted by w.  `form` is the state's: three planes (exact fp32) for
+        // dq and dk, whose products with q and k make the fp32 d decay, two for dv
+        auto through = [&](const f32x4 (&x)[KK][2], const char* t, const float* w, float mul, auto form) __attribute__((always_inline)) {
 #pragma unroll
             for (int kk = 0; kk < KK; ++kk) {
                 float y[8];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) { y[r] = x[kk][0][r]; y[4 + r] = x[kk][1][r]; }
-                typename LaOp<DT>::C2 sf;
+                decltype(form) sf;
                 la_split(y, sf);
 #pragma unroll
                 for (int tt = 0; tt < 4; ++tt) {
@@ -1060,13 +1061,13 @@ __global__ __launch_bounds__(4 * D) void la_bwd_chunks(LaArgs a, LaBwd p) {
         if (wid == 0 && c < cfirst) decays(c + 1);
         unit1();
         if constexpr (NBUF == 3) {
-            unit23(sd, sv, s2, false);
-            unit23(sq, sk, s3, true);
+            unit23(sd, sv, s2, Dv, false);
+            unit23(sq, sk, s3, Dk, true);
         }
         __syncthreads();
         clear();
         fetch(c - 1);
-        if (sp) through(xs, sd, gt.wq, a.scale);
+        if (sp && w0 < Dk) through(xs, sd, gt.wq, a.scale, typename LaOp<DT>::C3());
         with_own(sq, sr[wid]);
         LA_FENCE;
         within(sk, s1, false);
@@ -1078,11 +1079,11 @@ __global__ __launch_bounds__(4 * D) void la_bwd_chunks(LaArgs a, LaBwd p) {
         fetch_g(c - 2);
         if constexpr (NBUF == 1) {
             __syncthreads();
-            unit23(sd, sv, s2, false);
+            unit23(sd, sv, s2, Dv, false);
             __syncthreads();
         }
         clear();
-        if (have_e) through(e1, sv, gt.wk, 1.f);
+        if (have_e && w0 < Dk) through(e1, sv, gt.wk, 1.f, typename LaOp<DT>::C3());
         with_own(sk, sc[wid]);
         LA_FENCE;
         within(sq, s2, true);
@@ -1091,11 +1092,11 @@ __global__ __launch_bounds__(4 * D) void la_bwd_chunks(LaArgs a, LaBwd p) {
         LA_FENCE;
         if constexpr (NBUF == 1) {
             __syncthreads();
-            unit23(sq, sk, s3, true);
+            unit23(sq, sk, s3, Dk, true);
             __syncthreads();
         }
         clear();
-        if (have_e) through(e2, sk, gt.wk, 1.f);
+        if (have_e && w0 < Dv) through(e2, sk, gt.wk, 1.f, typename LaOp<DT>::C2());
         within(sd, s3, true);
         LA_FENCE;
         emit(p.dv, p.fv, a.Hv, hv, Dv);
@@ -1232,7 +1233,7 @@ __global__ __launch_bounds__(256) void la_step_kernel(const void* q_, const void
             for (int j = 0; j < AHEAD; ++j) {
                 const int r = r1 + j * rg;
                 if (r < Dk && c < Dv) {
-                    if constexpr (W == 4) *(f32x4*)y[j] = *(const f32x4*)(S + r * Dv + c);
+                    if constexpr (W == 4) *(f32x4*)y[j] = __builtin_nontemporal_load((const f32x4*)(S + r * Dv + c));
                     else y[j][0] = S[r * Dv + c];
                 }
             }
@@ -1246,7 +1247,7 @@ __global__ __launch_bounds__(256) void la_step_kernel(const void* q_, const void
                         y[j][i] = y[j][i] * w + kr * vv[i];
                         o[i] += qr * y[j][i];
                     }
-                    if constexpr (W == 4) *(f32x4*)(S + r * Dv + c) = *(const f32x4*)y[j];
+                    if constexpr (W == 4) __builtin_nontemporal_store(*(const f32x4*)y[j], (f32x4*)(S + r * Dv + c));
                     else S[r * Dv + c] = y[j][0];
                 }
             }
