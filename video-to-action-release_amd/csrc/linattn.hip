@@ -743,22 +743,26 @@ struct LaBwd {
 // Wave w owns rows 16 w .. of S, E, dq^T, dk^T and columns 16 w .. of dv^T; as dk contracts E over its columns and dv over its rows, E is
 // kept twice, by rows and by columns, which costs 48 more MFMA per wave and chunk but no exchange.  Scores are computed once, by units, and
 // shared through LDS; the next chunk's rows are on their way meanwhile.
+// TH 2: two waves share each block of 16 rows and take half of the chunk's tokens each (E in both): where the LDS allows one workgroup of narrow
+// heads on a CU, its D / 16 waves alone would leave the matrix units waiting.
+template <int DT, int D> constexpr int la_bwd_halves() { return D == 32 || (D == 64 && DT != 1) ? 2 : 1; }
 template <int DT, int D>
-__global__ __launch_bounds__(4 * D) void la_bwd_chunks(LaArgs a, LaBwd p) {
+__global__ __launch_bounds__((4 * D * la_bwd_halves<DT, D>())) void la_bwd_chunks(LaArgs a, LaBwd p) {
     typedef typename LaT<DT>::T E;
     typedef LaTile<DT, D> TT;
-    constexpr int NW = D / 16, NTH = 64 * NW, KK = D / 32;
+    constexpr int TH = la_bwd_halves<DT, D>(), NB = D / 16, NW = NB * TH, NTH = 64 * NW, KK = D / 32, TPW = 4 / TH;
+    constexpr bool AHEAD = DT != 0 || D < 128;      // fp32 rows of 128: their registers would spill
     constexpr int UB = 6 * la_unit_bytes<DT>();
     constexpr int NBUF = 4 * TT::BYTES + 3 * UB + 10240 <= 160 * 1024 ? 3 : 1;      // score buffers: all three at once where they fit
     __shared__ __attribute__((aligned(16))) char sm[4 * TT::BYTES + NBUF * UB];
     __shared__ __attribute__((aligned(16))) LaGate gts[2];
-    __shared__ float sr[NW][LA_C], sc[NW][LA_C], rm[4][LA_C], cm[2][LA_C], sz[NW];
+    __shared__ float sr[NB][LA_C], sc[NB][LA_C], rm[4][LA_C], cm[2][LA_C], sz[NB];
     char *sq = sm, *sk = sq + TT::BYTES, *sv = sk + TT::BYTES, *sd = sv + TT::BYTES, *s1 = sd + TT::BYTES;
     char *s2 = s1 + (NBUF == 3 ? UB : 0), *s3 = s2 + (NBUF == 3 ? UB : 0);
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int l16 = lane & 15, l4 = (lane >> 4) * 4;
+    const int l16 = lane & 15, l4 = (lane >> 4) * 4, blk = TH == 1 ? wid : wid % NB, t0 = TH == 1 ? 0 : wid / NB * TPW;      // rows 16 blk .., token tiles t0 ..
     const int seg = blockIdx.x % p.nseg, bh = blockIdx.x / p.nseg, b = bh / a.H, h = bh % a.H;
-    const int Dk = a.Dk, Dv = a.Dv, w0 = wid * 16;
+    const int Dk = a.Dk, Dv = a.Dv, w0 = blk * 16;
     const int hq = h / (a.H / a.Hq), hk = h / (a.H / a.Hk), hv = h / (a.H / a.Hv);
     const long long SS = (long long)Dk * Dv;
     const int len = la_len(a, b);
@@ -768,16 +772,16 @@ __global__ __launch_bounds__(4 * D) void la_bwd_chunks(LaArgs a, LaBwd p) {
     const E* G = (const E*)a.dout + b * a.ds[0] + h * a.ds[2];
     const float* g = a.g + b * a.gs[0] + h * a.gs[2];
 
-    // four values of each of the rows l16, l16 + 16, .. of a gradient: shared heads keep fp32 per head (rows of H heads), others their own type
-    auto put = [&](void* base, int f32, int Hx, int hx, int Dx, int c, const f32x4 (&x)[4]) __attribute__((always_inline)) {
+    // four values of each of the rows l16 of this wave's token tiles of a gradient: shared heads keep fp32 per head (rows of H heads), others their own type
+    auto put = [&](void* base, int f32, int Hx, int hx, int Dx, int c, const f32x4 (&x)[TPW]) __attribute__((always_inline)) {
         const int left = la_here(a.T - c * LA_C), room = Dx - w0 - l4, ld = la_here((f32 ? a.H : Hx) * Dx);
         const long long at = ((long long)b * a.T + (long long)c * LA_C) * ld + (f32 ? h : hx) * Dx + w0;
         const unsigned off = (unsigned)l16 * (unsigned)ld + (unsigned)l4;
         if (room <= 0) return;
         auto rows = [&](auto&& one) __attribute__((always_inline)) {
 #pragma unroll
-            for (int tt = 0; tt < 4; ++tt)
-                if (tt * 16 + l16 < left) one(at + (long long)(tt * 16) * ld, x[tt]);
+            for (int tt = 0; tt < TPW; ++tt)
+                if ((t0 + tt) * 16 + l16 < left) one(at + (long long)((t0 + tt) * 16) * ld, x[tt]);
         };
         if (Dx % 4 == 0) {
             if (f32) rows([&](long long o, const f32x4& y) { *la_at<f32x4>((float*)base + o, off * 4u) = y; });
@@ -791,7 +795,7 @@ __global__ __launch_bounds__(4 * D) void la_bwd_chunks(LaArgs a, LaBwd p) {
     const int chi = p.NC - 1 - seg * p.cps, clo = chi - p.cps + 1 > 0 ? chi - p.cps + 1 : 0;
     const int nvc = (len + LA_C - 1) / LA_C, cfirst = chi < nvc ? chi : nvc - 1;
     for (int c = chi; c > cfirst && c >= clo; --c) {
-        const f32x4 z[4] = {};
+        const f32x4 z[TPW] = {};
         put(p.dq, p.fq, a.Hq, hq, Dk, c, z);
         put(p.dk, p.fk, a.Hk, hk, Dk, c, z);
         put(p.dv, p.fv, a.Hv, hv, Dv, c, z);
@@ -841,12 +845,12 @@ __global__ __launch_bounds__(4 * D) void la_bwd_chunks(LaArgs a, LaBwd p) {
     auto valid = [&](int c) { return len - c * LA_C < LA_C ? len - c * LA_C : LA_C; };
     auto fetch = [&](int c) __attribute__((always_inline)) {
         if (c < clo) return;
-        const long long t0 = (long long)c * LA_C;
+        const long long f0 = (long long)c * LA_C;
         const int nv = valid(c);
-        rq.load(Q + t0 * a.qs[1], a.qs[1], nv, Dk, p.vq);
-        rk.load(K + t0 * a.ks[1], a.ks[1], nv, Dk, p.vk);
-        rv.load(V + t0 * a.vs[1], a.vs[1], nv, Dv, p.vv);
-        rd.load(G + t0 * a.ds[1], a.ds[1], nv, Dv, p.vd);
+        rq.load(Q + f0 * a.qs[1], a.qs[1], nv, Dk, p.vq);
+        rk.load(K + f0 * a.ks[1], a.ks[1], nv, Dk, p.vk);
+        rv.load(V + f0 * a.vs[1], a.vs[1], nv, Dv, p.vv);
+        rd.load(G + f0 * a.ds[1], a.ds[1], nv, Dv, p.vd);
     };
     auto fetch_g = [&](int c) { if (wid == NW - 1 && c >= clo && lane < valid(c)) rgn = g[((long long)c * LA_C + lane) * a.gs[1]]; };
     auto gates = [&](int c) { if (wid == NW - 1 && c >= clo) la_gates(gts[c & 1], rgn, lane < valid(c), lane); };
@@ -859,7 +863,7 @@ __global__ __launch_bounds__(4 * D) void la_bwd_chunks(LaArgs a, LaBwd p) {
         gates(cfirst);
         fetch_g(cfirst - 1);
     }
-    f32x4 acc[4];
+    f32x4 acc[TPW];
     float raw[3][8];
     // d decay of a chunk (first wave, lane = token): its parts are gathered from LDS while the next chunk's rows are stored, and summed up later
     double up = 0.0, down = 0.0, cross = 0.0;
@@ -869,7 +873,7 @@ __global__ __launch_bounds__(4 * D) void la_bwd_chunks(LaArgs a, LaBwd p) {
         const LaGate& gt = gts[c & 1];
         float u = 0.f, dn = 0.f, z = 0.f;
 #pragma unroll
-        for (int w = 0; w < NW; ++w) {
+        for (int w = 0; w < NB; ++w) {
             u += sr[w][lane];
             dn += sc[w][lane];
             z += sz[w];
@@ -900,6 +904,7 @@ __global__ __launch_bounds__(4 * D) void la_bwd_chunks(LaArgs a, LaBwd p) {
     for (int c = cfirst; c >= clo; --c) {
         const int nv = valid(c);
         const LaGate& gt = gts[c & 1];
+        if (!AHEAD && c < cfirst) fetch(c);
         __syncthreads();
         rq.store(sq);
         rk.store(sk);
@@ -916,7 +921,7 @@ __global__ __launch_bounds__(4 * D) void la_bwd_chunks(LaArgs a, LaBwd p) {
 #pragma unroll
                     for (int r = 0; r < 4; ++r) z += xs[kk][half][r] * e1[kk][half][r];
             z = wave_sum(z);
-            if (lane == 0) sz[wid] = z;
+            if (lane == 0 && t0 == 0) sz[blk] = z;
         }
         // W (do . v) with lane = i, slots = j: the operand of dq
         auto unit1 = [&]() __attribute__((always_inline)) {
@@ -1000,7 +1005,7 @@ __global__ __launch_bounds__(4 * D) void la_bwd_chunks(LaArgs a, LaBwd p) {
         };
         auto clear = [&]() __attribute__((always_inline)) {
 #pragma unroll
-            for (int t = 0; t < 4; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int t = 0; t < TPW; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
         };
         // a state's rows (or columns) times the tokens' rows in `t`, weighted by w.  `form` is the state's: three planes (exact fp32) for
         // dq and dk, whose products with q and k make the fp32 d decay, two for dv
@@ -1013,24 +1018,24 @@ __global__ __launch_bounds__(4 * D) void la_bwd_chunks(LaArgs a, LaBwd p) {
                 decltype(form) sf;
                 la_split(y, sf);
 #pragma unroll
-                for (int tt = 0; tt < 4; ++tt) {
+                for (int tt = 0; tt < TPW; ++tt) {
                     typename LaOp<DT>::In tf;
-                    TT::nat(t, tt * 16, kk, lane, tf);
+                    TT::nat(t, (t0 + tt) * 16, kk, lane, tf);
                     la_mma(acc[tt], sf, tf);
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
 #pragma unroll
-            for (int tt = 0; tt < 4; ++tt) acc[tt] *= w[tt * 16 + l16] * mul;
+            for (int tt = 0; tt < TPW; ++tt) acc[tt] *= w[(t0 + tt) * 16 + l16] * mul;
         };
         // and its product with the tokens' own rows: this wave's share
         auto with_own = [&](const char* own, float* dst) __attribute__((always_inline)) {
 #pragma unroll
-            for (int tt = 0; tt < 4; ++tt) {
+            for (int tt = 0; tt < TPW; ++tt) {
                 float y[4];
-                TT::four(own, tt * 16 + l16, w0 + l4, y);
+                TT::four(own, (t0 + tt) * 16 + l16, w0 + l4, y);
                 const float s = la_rows_sum((acc[tt][0] * y[0] + acc[tt][1] * y[1]) + (acc[tt][2] * y[2] + acc[tt][3] * y[3]));
-                if (lane < 16) dst[tt * 16 + lane] = s;
+                if (lane < 16) dst[(t0 + tt) * 16 + lane] = s;
             }
         };
         // the part within the chunk: columns w0 .. of the tokens in `t` times the shared scores
@@ -1044,16 +1049,17 @@ __global__ __launch_bounds__(4 * D) void la_bwd_chunks(LaArgs a, LaBwd p) {
                     for (int u = 0; u < 6; ++u) {
                         const int tile = mirrored ? 3 - la_unit_tile(u) : la_unit_tile(u);
                         if ((mirrored ? 1 - la_unit_step(u) : la_unit_step(u)) != ks || tile * 16 >= nv) continue;
+                        if (TH == 2 && tile / TPW * TPW != t0) continue;
                         typename LaOp<DT>::C2 xf;
                         la_get<DT>(units, u, lane, xf);
-                        la_mma(acc[tile], tf, xf);
+                        la_mma(acc[tile % TPW], tf, xf);
                     }
                 }
         };
         auto emit = [&](void* base, int f32, int Hx, int hx, int Dx) __attribute__((always_inline)) {
 #pragma unroll
-            for (int tt = 0; tt < 4; ++tt) {
-                if (tt * 16 + l16 >= nv) acc[tt] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int tt = 0; tt < TPW; ++tt) {
+                if ((t0 + tt) * 16 + l16 >= nv) acc[tt] = f32x4{0.f, 0.f, 0.f, 0.f};
             }
             put(base, f32, Hx, hx, Dx, c, acc);
         };
@@ -1066,9 +1072,9 @@ __global__ __launch_bounds__(4 * D) void la_bwd_chunks(LaArgs a, LaBwd p) {
         }
         __syncthreads();
         clear();
-        fetch(c - 1);
+        if (AHEAD) fetch(c - 1);
         if (sp && w0 < Dk) through(xs, sd, gt.wq, a.scale, typename LaOp<DT>::C3());
-        with_own(sq, sr[wid]);
+        with_own(sq, sr[blk]);
         LA_FENCE;
         within(sk, s1, false);
         LA_FENCE;
@@ -1084,7 +1090,7 @@ __global__ __launch_bounds__(4 * D) void la_bwd_chunks(LaArgs a, LaBwd p) {
         }
         clear();
         if (have_e && w0 < Dk) through(e1, sv, gt.wk, 1.f, typename LaOp<DT>::C3());
-        with_own(sk, sc[wid]);
+        with_own(sk, sc[blk]);
         LA_FENCE;
         within(sq, s2, true);
         LA_FENCE;
@@ -1147,7 +1153,7 @@ __global__ __launch_bounds__(4 * D) void la_bwd_chunks(LaArgs a, LaBwd p) {
         gather(clo);
         decays(clo);
     }
-    if (p.e_first && clo == 0 && w0 + l16 < Dk)
+    if (p.e_first && clo == 0 && t0 == 0 && w0 + l16 < Dk)
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
@@ -1505,9 +1511,9 @@ int v2a_linattn_bwd(const void* q, const void* k, const void* v, const float* g,
             d.vst = Dv % 4 == 0 && (((uintptr_t)state | (uintptr_t)dstate_out | (uintptr_t)dstate) & 15) == 0;
             const dim3 grid((unsigned)((long long)B * H * pl.nseg));
             const int Dm = Dk > Dv ? Dk : Dv;
-#define BWD(DT, D) hipLaunchKernelGGL((la_bwd_chunks<DT, D>), grid, dim3(4 * D), 0, s, a, d)
+#define BWD(DT, D) hipLaunchKernelGGL((la_bwd_chunks<DT, D>), grid, dim3(4 * D * la_bwd_halves<DT, D>()), 0, s, a, d)
             if (Dm <= 32) { if (dtype == 0) BWD(0, 32); else if (dtype == 1) BWD(1, 32); else BWD(2, 32); }
-            else if (Dm <= 64) { if (dtype == 0) BWD(0, 64); else if (dtype == 1) BWD(1, 64); else BWD(2, 64); }
+            else if (Dm <= 64) { if (dtype == 0) BWD(3, 64); else if (dtype == 1) BWD(1, 64); else BWD(2, 64); }
             else { if (dtype == 0) BWD(0, 128); else if (dtype == 1) BWD(1, 128); else BWD(2, 128); }
 #undef BWD
             V2A_CHECK_LAUNCH();
