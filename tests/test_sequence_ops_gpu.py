@@ -108,6 +108,10 @@ SHAPES = [
     (2, 200, 4, 2, 4, 4, 24, 128, "head", True),
     (1, 777, 2, 1, 1, 2, 40, 72, "token", True),
     (1, 1100, 1, 1, 1, 1, 128, 128, "token", False),
+    (1, 320, 2, 2, 2, 2, 100, 33, "token", True),
+    (1, 400, 3, 3, 1, 3, 33, 128, "head", True),
+    (2, 260, 2, 1, 2, 2, 32, 20, "token", True),
+    (1, 192, 2, 2, 2, 1, 80, 48, "token", True),
 ]
 
 
@@ -234,7 +238,8 @@ def check_step(c, t, S, slots=None, scale=None):
 
 @pytest.mark.parametrize("dt", [F32, BF, FP], ids=["fp32", "bf16", "fp16"])
 @pytest.mark.parametrize("shape", [(1, 1, 1, 1, 1, 1, 1), (1, 8, 8, 8, 8, 48, 48), (5, 6, 2, 6, 3, 33, 17), (3, 4, 4, 1, 1, 128, 128), (2, 2, 2, 2, 2, 100, 64),
-                                   (2, 2, 1, 2, 2, 16, 126)], ids=lambda s: "x".join(map(str, s)))
+                                   (2, 2, 1, 2, 2, 16, 126), (2, 3, 3, 1, 3, 20, 33), (1, 2, 2, 2, 2, 65, 63), (3, 1, 1, 1, 1, 128, 65),
+                                   (2, 2, 2, 2, 2, 3, 4)], ids=lambda s: "x".join(map(str, s)))
 def test_step(shape, dt):
     B, H, Hq, Hk, Hv, Dk, Dv = shape
     c = make(sum(shape), B, 2, H, Hq, Hk, Hv, Dk, Dv, dt, "token" if B > 1 else "head")
@@ -447,6 +452,9 @@ def test_embedding_of_views_and_of_nothing():
     for empty in (ids[:0], ids[:, :0].contiguous()):
         dtab, dpos = ops().embed_bwd(empty, torch.zeros(*empty.shape, 33).cuda(), 50, pos_rows=17)
         assert not dtab.any() and not dpos.any() and dpos.shape == (17, 33)
+    dout = torch.randn(3 * 17 * 64 + 1, generator=g).cuda()
+    d1, d2 = dout[1:].view(3, 17, 64), dout[1:].clone().view(3, 17, 64)            # an odd first element: the same sums
+    assert all(torch.equal(x, y) for x, y in zip(ops().embed_bwd(ids, d1, 50, pos_rows=17), ops().embed_bwd(ids, d2, 50, pos_rows=17)))
     none = torch.full((4, 5), -1).cuda()
     dtab, dpos = ops().embed_bwd(none, torch.full((4, 5, 33), math.nan).cuda(), 50, pos_rows=6)
     assert not dtab.any() and not dpos.any() and not ops().embed_fwd(none, table, pos=pos).any()

@@ -1261,13 +1261,13 @@ __global__ __launch_bounds__(256) void la_step_kernel(const void* q_, const void
 #pragma unroll
         for (int i = 0; i < W; ++i)
             for (int m = lv; m < 64; m *= 2) o[i] += __shfl_xor(o[i], m, 64);
-        if (W == 4) {
-            if (lane < lv && c < Dv) *(f32x4*)&red[x >> 6][c] = f32x4{o[0], o[W > 1 ? 1 : 0], o[W > 2 ? 2 : 0], o[W > 3 ? 3 : 0]};
-        } else if (lv >= 64) {              // one value a lane, 128 lanes a row: waves 0 and 2 hold columns 0 .. 63, 1 and 3 the others
-            if (c < Dv) red[(x >> 6) & 2][c] = o[0], red[((x >> 6) & 2) + 1][c] = 0.f;
-        } else if (lane < lv && c < Dv) red[x >> 6][c] = o[0];
+        // one sum a wave, or one a pair of waves where 128 lanes share a row
+        const int groups = lv > 64 ? 2 : 4, mine = lv > 64 ? x >> 7 : x >> 6;
+        if ((lane < lv || lv > 64) && c < Dv)
+#pragma unroll
+            for (int i = 0; i < W; ++i) red[mine][c + i] = o[i];
         __syncthreads();
-        if (x < Dv) out[((long long)b * H + h) * Dv + x] = LaT<DT>::st((red[0][x] + red[1][x]) + (red[2][x] + red[3][x]));
+        if (x < Dv) out[((long long)b * H + h) * Dv + x] = LaT<DT>::st(groups == 2 ? red[0][x] + red[1][x] : (red[0][x] + red[1][x]) + (red[2][x] + red[3][x]));
         if (!more) return;
         int next = 0x7fffffff;
         for (int j = b + 1 + x; j < B; j += 256)

@@ -1608,7 +1608,8 @@ def linear_attention_fwd(q, k, v, log_decay, state=None, lens=None, scale=None, 
     q [B,T,Hq,Dk], k [B,T,Hk,Dk], v [B,T,Hv,Dv] (fp32 / bf16 / fp16, column blocks of a packed projection may be passed as views; head widths
     up to 128); log_decay fp32 [H] (one decay per head) or [B,T,H] (one per token; -inf clears the state, e.g. where an episode begins).
     Hq, Hk and Hv divide H; head h reads shared head h // (H // Hx).  state: S before the first token (None: 0).  lens int32 [B]: row b has
-    lens[b] tokens; what is behind them is not read, out is 0 there and the last state is the one after them.  scale: 1 / sqrt(Dk) by default."""
+    lens[b] tokens; what is behind them is not read, out is 0 there and the last state is the one after them.  scale: 1 / sqrt(Dk) by default.
+    Tokens are taken 64 at a time: a NaN or infinity in a row makes its outputs undefined from the beginning of that 64."""
     H, Hq, Hk, Hv, Dk, Dv, dt = _la_heads(q, k, v, log_decay, 2)
     _same_device(q, k, v, log_decay, state, lens)
     B, T = q.shape[:2]
@@ -1622,7 +1623,7 @@ def linear_attention_fwd(q, k, v, log_decay, state=None, lens=None, scale=None, 
     ws = q.new_empty(nb, dtype=torch.uint8) if nb else None
     st = _I64x12(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *_g_strides(log_decay, 2))
     check(lib.v2a_linattn_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), _p(state), _p(lens), out.data_ptr(), _p(last), st, B, T, H,
-                              Hq, Hk, Hv, Dk, Dv, dt, Dk ** -0.5 if scale is None else scale, _p(ws), nb, _stream_of(q)), "linear_attention_fwd")
+                              Hq, Hk, Hv, Dk, Dv, dt, Dk ** -0.5 if scale is None else float(scale), _p(ws), nb, _stream_of(q)), "linear_attention_fwd")
     return out, last
 
 
@@ -1653,7 +1654,7 @@ def linear_attention_bwd(q, k, v, log_decay, dout, state=None, lens=None, scale=
     st = _I64x15(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *_g_strides(log_decay, 2), *dout.stride()[:3])
     check(lib.v2a_linattn_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), _p(state), _p(lens), dout.data_ptr(), _p(dstate), dq.data_ptr(),
                               dk.data_ptr(), dv.data_ptr(), dg.data_ptr(), _p(ds0), st, B, T, H, Hq, Hk, Hv, Dk, Dv, dt, tok,
-                              Dk ** -0.5 if scale is None else scale, _p(ws), nb, _stream_of(q)), "linear_attention_bwd")
+                              Dk ** -0.5 if scale is None else float(scale), _p(ws), nb, _stream_of(q)), "linear_attention_bwd")
     return dq, dk, dv, dg, ds0
 
 
@@ -1677,7 +1678,7 @@ def linear_attention_step(q, k, v, log_decay, state, slots=None, scale=None):
     out = q.new_empty((B, H, Dv))
     st = _I64x8(*q.stride()[:2], *k.stride()[:2], *v.stride()[:2], *_g_strides(log_decay, 1))
     check(lib.v2a_linattn_step(q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), state.data_ptr(), _p(slots), out.data_ptr(), st, B, N, H, Hq, Hk,
-                               Hv, Dk, Dv, dt, Dk ** -0.5 if scale is None else scale, _stream_of(q)), "linear_attention_step")
+                               Hv, Dk, Dv, dt, Dk ** -0.5 if scale is None else float(scale), _stream_of(q)), "linear_attention_step")
     return out
 
 
@@ -1709,7 +1710,7 @@ def embed_fwd(ids, table, scale=1.0, pos=None):
     out = table.new_empty((*ids.shape, D))
     if N:
         check(lib.v2a_embed_fwd(ids.data_ptr(), wide, table.data_ptr(), _p(pos), out.data_ptr(), N, T, V, D, table.stride(0), 0 if pos is None else pos.stride(0),
-                                dt, scale, _stream_of(table)), "embed_fwd")
+                                dt, float(scale), _stream_of(table)), "embed_fwd")
     return out
 
 
@@ -1733,6 +1734,6 @@ def embed_bwd(ids, dout, vocab, scale=1.0, pos_rows=None):
     dpos = None if pos_rows is None else dout.new_empty((pos_rows, D))
     nb = lib.v2a_embed_bwd_workspace_bytes(N, vocab, D, dt)
     ws = dout.new_empty(nb, dtype=torch.uint8) if nb else None
-    check(lib.v2a_embed_bwd(ids.data_ptr(), wide, dout.data_ptr(), dtable.data_ptr(), _p(dpos), N, max(T, 1), vocab, D, pos_rows or 0, dt, scale, _p(ws), nb,
+    check(lib.v2a_embed_bwd(ids.data_ptr(), wide, dout.data_ptr(), dtable.data_ptr(), _p(dpos), N, max(T, 1), vocab, D, pos_rows or 0, dt, float(scale), _p(ws), nb,
                             _stream_of(dout)), "embed_bwd")
     return dtable, dpos
