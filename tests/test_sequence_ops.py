@@ -43,6 +43,21 @@ def test_linear_attention_refuses(msg, kw, change):
             ops.linear_attention_step(*s, torch.zeros(2, 4, 8, 16))
 
 
+def test_operands_by_keyword():
+    """The first operand may be named like the others: the call gets as far as the check for a GPU."""
+    from v2a_hip import ops
+    q, k, v, g = _la()
+    ids = torch.zeros(2, 5, dtype=torch.int64)
+    for call in (lambda: ops.linear_attention_fwd(q=q, k=k, v=v, log_decay=g), lambda: ops.linear_attention_fwd(k=k, v=v, log_decay=g, q=q),
+                 lambda: ops.linear_attention_bwd(q=q, k=k, v=v, log_decay=g, dout=v),
+                 lambda: ops.linear_attention_step(q=q[:, 0], k=k[:, 0], v=v[:, 0], log_decay=g, state=torch.zeros(2, 4, 8, 16)),
+                 lambda: ops.embed_fwd(ids=ids, table=torch.zeros(7, 8)), lambda: ops.embed_bwd(ids=ids, dout=torch.zeros(2, 5, 8), vocab=7)):
+        with pytest.raises(ValueError, match="need CUDA"):
+            call()
+    with pytest.raises(TypeError, match="'q'"):
+        ops.linear_attention_fwd(k=k, v=v, log_decay=g)
+
+
 def test_arguments_beside_the_operands_are_checked():
     """On the meta device: the same checks, past the one for a GPU."""
     from v2a_hip import ops

@@ -1542,13 +1542,16 @@ _device_now = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_d
 
 def _on_device_of_first(fn):
     """Decorator: the first operand names the GPU the call runs on (the current one or not)."""
+    name = fn.__code__.co_varnames[0]
+
     @functools.wraps(fn)
-    def call(t, *a, **kw):
-        i = t.get_device()
+    def call(*a, **kw):
+        t = a[0] if a else kw.get(name)
+        i = -1 if t is None else t.get_device()
         if i >= 0 and i != _device_now():
             with torch.cuda.device(i):
-                return fn(t, *a, **kw)
-        return fn(t, *a, **kw)
+                return fn(*a, **kw)
+        return fn(*a, **kw)
     return call
 
 
