@@ -460,6 +460,16 @@ def test_embedding_of_views_and_of_nothing():
     assert not dtab.any() and not dpos.any() and not ops().embed_fwd(none, table, pos=pos).any()
 
 
+def test_token_hash_encoder_looks_up_the_same_values():
+    from diffuser.libero.lb_train_utils import HashTextEncoder, HashTokenizer
+    tok, enc = HashTokenizer(), HashTextEncoder(dim=64)
+    ids = tok(["open the top drawer", "close it", ""])["input_ids"]
+    want = enc(ids).last_hidden_state
+    enc = enc.cuda()
+    for x in (ids.cuda(), ids.t().contiguous().t().cuda(), ids):          # ids that stay on the host index the table on the GPU too
+        assert torch.equal(enc(x).last_hidden_state.cpu(), want)
+
+
 def test_embedding_past_32_bit_offsets():
     V = 2 ** 31 // 64 + 10
     table = torch.empty(V, 64, dtype=BF, device="cuda")
