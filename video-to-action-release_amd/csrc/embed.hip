@@ -52,7 +52,8 @@ struct EmShape {
     int D, lpr, ncol;      // lanes that share a row (power of two, at most 64), column blocks of lpr pieces
 };
 
-// A group of lpr lanes takes a row; each lane has RPT rows under way at once
+// A group of lpr lanes takes a row; each lane has RPT rows under way at once: 62891 rows of 384 fp32 from a table of 259 are written in 20 us
+// (97 MB, 4.8 TB/s of writes), 8192 rows of 512 bf16 from 49408 in 7.5 us, 20 rows in 3.6 us (an empty launch: 3.7).
 template <int DT, int W>
 __global__ __launch_bounds__(256) void embed_fwd_kernel(const void* ids, int wide, const void* table_, const void* pos_, void* out_, EmShape e, long long ldt,
                                                         long long ldp, float scale) {
@@ -157,7 +158,8 @@ struct EmSortLds {
     unsigned base[EM_BINS], tmp[EM_WAVES];
 };
 
-// up to EM_SMALL tokens: one workgroup, all digits, through LDS
+// Up to EM_SMALL tokens: one workgroup, all digits, through LDS; bound by its barriers and ballots.8192 tokens
+// with 16 bits take 20 us, beside which the zero fill of 51 MB is hidden.
 __device__ void em_sort_small(const EmSort& s, EmSortLds& L, unsigned (*xch)[EM_SMALL]) {
     constexpr int KPT = EM_SMALL / EM_SORT_T;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, bins = 1 << s.bits;
@@ -229,7 +231,7 @@ __global__ __launch_bounds__(EM_SORT_T) void embed_hist_kernel(EmSort s, int p) 
     __shared__ unsigned count[EM_BINS];
     em_hist(s, p, blockIdx.x, count);
 }
-// the tokens of a tile to their places of pass p; a workgroup adds up the at most EM_TILES histograms itself
+// the tokens of a tile to their places of pass p; a workgroup adds up the at most EM_TILES histograms itself (62891 tokens, 9 bits: 11 us)
 __global__ __launch_bounds__(EM_SORT_T) void embed_scatter_kernel(EmSort s, int p) {
     __shared__ EmSortLds L;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, bins = 1 << s.bits;
@@ -343,7 +345,8 @@ __global__ __launch_bounds__(EM_SORT_T) void embed_first_kernel(EmSort s, EmGrad
 }
 
 // Pieces of `ts` neighbours of the sorted list, one per group of lpr lanes.  part [pieces][2][Dp]: 0 = a row that began before the piece
-// (through to its end or past the piece), 1 = a row that begins inside and goes on behind it.
+// (through to its end or past the piece), 1 = a row that begins inside and goes on behind it.  Bound by the read of dout: 62891 rows of 384 fp32
+// in 21.6 us (4.5 TB/s), 8192 rows of 512 bf16 in 7.7.
 template <int DT, int W>
 __global__ __launch_bounds__(256) void embed_pieces_kernel(const unsigned* key, const unsigned* pos, EmGrad g, EmShape e, float* part, int Dp, unsigned ts) {
     typedef typename EmT<DT>::T E;

@@ -359,6 +359,13 @@ struct LaScan {
     int NC, cps, nseg, ndv, local, vq, vo, vst;
 };
 
+// One workgroup walks the chunks of one segment of one (row, head) and one tile of 16 NT NW state columns, wave w with columns 16 NT w .. of
+// the state in accumulators.  OUT: the outputs as well; otherwise the states alone (of a segment that starts at 0, or before every chunk for the
+// gradient).  Columns of the state never meet, so a tile of them costs k again but no exchange; scores are computed once a workgroup, by units,
+// and shared through LDS.  Bound by the issue of vector, LDS and matrix instructions rather than by memory, since a chunk's stages depend on one
+// another and the tiles leave room for one or two workgroups on a CU: 1 x 32768 tokens x 8 heads of 128, bf16, runs the local pass in 44 us
+// (3.1 TB/s of k and v) and OUT in 93 (2.9 TB/s of rows, 25 % of the MFMA and 41 % of the vector issue slots taken); 8 x 2048 tokens x 8 heads
+// 64 / 128, fp32 in planes, 34 and 74 us; 64 rows of 10 tokens x 8 heads of 48, fp32, 10 us.
 template <int DT, int DK, int NT, int NW, bool OUT> constexpr int la_scan_lds() {
     return LaTile<DT, DK>::BYTES * (OUT ? 2 : 1) + LaTile<DT, 16 * NT * NW>::BYTES + (OUT ? 6 * la_unit_bytes<DT>() : 0);
 }
@@ -692,7 +699,8 @@ __global__ __launch_bounds__(64 * NW, (la_scan_waves<DT, DK, NT, NW, OUT>())) vo
 }
 
 // Local states of the segments -> states before them: S_0 = init, S_{s+1} = decay_s S_s + local_s, in place; W neighbours a lane, eight segments
-// a round and the next round's loads ahead of this one's stores
+// a round and the next round's loads ahead of this one's stores.  A chain of nseg steps a lane, bound by its latency: 22 us for 8 heads of 128
+// in 64 segments (67 MB, 3 TB/s), 5.6 us for 64 heads 64 / 128 in 4.
 template <int W>
 __global__ __launch_bounds__(64) void la_combine(LaScan p, int nseg, long long SS) {
     typedef typename std::conditional<W == 4, f32x4, float>::type V;
@@ -745,6 +753,9 @@ struct LaBwd {
 // shared through LDS; the next chunk's rows are on their way meanwhile.
 // TH 2: two waves share each block of 16 rows and take half of the chunk's tokens each (E in both): where the LDS allows one workgroup of narrow
 // heads on a CU, its D / 16 waves alone would leave the matrix units waiting.
+// Bound by the latency of a chunk's dependent stages, with the four tiles filling the LDS of a CU (one workgroup of 128-wide heads): 4 x 4096
+// tokens x 8 heads of 128, bf16, decays per token: 160 us, 285 MB of HBM traffic at 1.8 TB/s, 14 % of the MFMA and 35 % of the vector issue
+// slots; fp32 4 x 2048 x 4 heads of 128 167 us; 8 x 2048 x 8 heads of 64 bf16 70 us, fp32 141.  64 rows of 16 tokens x 4 heads of 64, fp32: 14 us.
 template <int DT, int D> constexpr int la_bwd_halves() { return D == 32 || (D == 64 && DT != 1) ? 2 : 1; }
 template <int DT, int D>
 __global__ __launch_bounds__((4 * D * la_bwd_halves<DT, D>())) void la_bwd_chunks(LaArgs a, LaBwd p) {
@@ -1163,7 +1174,7 @@ __global__ __launch_bounds__((4 * D * la_bwd_halves<DT, D>())) void la_bwd_chunk
             }
 }
 
-// gradients of shared heads: the heads of a group summed in order, rounded once
+// gradients of shared heads: the heads of a group summed in order, rounded once (5 x 777 tokens, 6 heads of 40 to 2: 4.7 us, mostly the launch)
 template <int DT>
 __global__ void la_share(const float* src, void* dst_, long long rows, int Hx, int rep, int D) {
     typedef typename LaT<DT>::T E;
@@ -1178,7 +1189,7 @@ __global__ void la_share(const float* src, void* dst_, long long rows, int Hx, i
     }
 }
 
-// d decay of a per-head decay: the sum over all tokens, one workgroup per head, in fp64
+// d decay of a per-head decay: the sum over all chunks and rows, one workgroup per head, in fp64 (64 rows x 1 chunk: 3 us, the launch)
 __global__ __launch_bounds__(256) void la_dg_heads(const float* dgt, float* dg, long long rows, int H) {
     __shared__ double red[4];
     double s = 0.0;
@@ -1192,7 +1203,8 @@ __global__ __launch_bounds__(256) void la_dg_heads(const float* dgt, float* dg, 
 // ---------------------------------------------------------------------------------------------------------------------- single tokens
 // One workgroup per (row, head): reads and writes the Dk x Dv state once, which is all of the traffic that counts.  lv lanes of 16 bytes cover
 // a state row, the other lanes take further rows, eight of them under way per lane.  Rows that name the same slot are taken by the first of
-// them, in row order, as successive tokens.
+// them, in row order, as successive tokens.  Bound by memory: 512 rows x 16 heads of 128 x 128 take 230 us, 4.7 of the 5.1 TB/s that a copy of
+// that size reaches; one row of 8 heads of 48 x 48 takes 4.9 us, an empty launch 3.7.  Streaming (nontemporal) accesses: 231 us against 247.
 template <int DT, int W>
 __global__ __launch_bounds__(256) void la_step_kernel(const void* q_, const void* k_, const void* v_, const float* g, float* state, const int* slots,
                                                       void* out_, long long qb_, long long qh_, long long kb_, long long kh_, long long vb_, long long vh_,
