@@ -158,7 +158,7 @@ struct EmSortLds {
     unsigned base[EM_BINS], tmp[EM_WAVES];
 };
 
-// Up to EM_SMALL tokens: one workgroup, all digits, through LDS; bound by its barriers and ballots.8192 tokens
+// Up to EM_SMALL tokens: one workgroup, all digits, through LDS; bound by its barriers and ballots.  8192 tokens
 // with 16 bits take 20 us, beside which the zero fill of 51 MB is hidden.
 __device__ void em_sort_small(const EmSort& s, EmSortLds& L, unsigned (*xch)[EM_SMALL]) {
     constexpr int KPT = EM_SMALL / EM_SORT_T;
