@@ -711,21 +711,25 @@ __global__ __launch_bounds__(64) void la_combine(LaScan p, int nseg, long long S
     float* q = m.seg + bh * nseg * SS + e;
     const float* f = m.seg_decay + bh * nseg;
     V x[8], y[8];
-    auto get = [&](int i0, V (&v)[8]) {
+    float fx[8], fy[8];      // loaded with the states: behind the stores, which might be to them, each would be waited for by itself
+    auto get = [&](int i0, V (&v)[8], float (&w)[8]) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = i0 + j + 1 < nseg ? *(const V*)(q + (i0 + j) * SS) : V{};
+        for (int j = 0; j < 8; ++j) {
+            v[j] = i0 + j + 1 < nseg ? *(const V*)(q + (i0 + j) * SS) : V{};
+            w[j] = i0 + j + 1 < nseg ? f[i0 + j] : 0.f;
+        }
     };
-    get(0, x);
+    get(0, x, fx);
     for (int i0 = 0; i0 < nseg; i0 += 8) {
-        get(i0 + 8, y);
+        get(i0 + 8, y, fy);
 #pragma unroll
         for (int j = 0; j < 8; ++j)
             if (i0 + j < nseg) {
                 *(V*)(q + (i0 + j) * SS) = s;
-                s = s * f[i0 + j] + x[j];
+                s = s * fx[j] + x[j];
             }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = y[j];
+        for (int j = 0; j < 8; ++j) { x[j] = y[j]; fx[j] = fy[j]; }
     }
 }
 
