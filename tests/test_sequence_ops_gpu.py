@@ -112,6 +112,7 @@ SHAPES = [
     (1, 400, 3, 3, 1, 3, 33, 128, "head", True),
     (2, 260, 2, 1, 2, 2, 32, 20, "token", True),
     (1, 192, 2, 2, 2, 1, 80, 48, "token", True),
+    (2, 900, 40, 40, 8, 40, 40, 36, "token", True),          # segments of four chunks
 ]
 
 

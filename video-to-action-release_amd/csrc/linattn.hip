@@ -353,6 +353,9 @@ struct LaDir {                  // one direction of the recurrence
 struct LaScan {
     LaDir dir[2];
     float* chunk;               // state before each chunk in scan order, [B H][NC][Dk][Dv] (NULL: not kept)
+    // segments of two chunks (NULL: not kept): state before the second one, [B H][nseg][Dk][Dv], in the local pass without what came before the
+    // segment, whose share is inner_decay [B H][nseg] of the state there; the forward direction's
+    float *inner, *inner_decay;
     float* last;                // state behind the last chunk (NULL)
     void* out;
     int ndir;                   // 2: both directions, alternate workgroups
@@ -395,7 +398,7 @@ __global__ __launch_bounds__(64 * NW, (la_scan_waves<DT, DK, NT, NW, OUT>())) vo
     const int dvt = blk % p.ndv;
     blk /= p.ndv;
     const int seg = blk % p.nseg, bh = blk / p.nseg, b = bh / a.H, h = bh % a.H;
-    if (!OUT && p.local && seg == p.nseg - 1) return;      // nothing follows it
+    if (!OUT && p.local && seg == p.nseg - 1 && (rev || !p.inner || seg * 2 + 1 == p.NC)) return;      // nothing follows it
     const int len = la_len(a, b), Dk = a.Dk, Dv = a.Dv, dv0 = dvt * DVT + wid * NT * 16;
     const int hq = h / (a.H / a.Hq), hk = h / (a.H / a.Hk), hv = h / (a.H / a.Hv);
     const int yroom = Dv - dvt * DVT < DVT ? Dv - dvt * DVT : DVT;
@@ -513,6 +516,14 @@ __global__ __launch_bounds__(64 * NW, (la_scan_waves<DT, DK, NT, NW, OUT>())) vo
     auto fetch_q = [&](int i) { if constexpr (OUT) if (i < vend) rq.load(Q + first(i) * a.qs[1], a.qs[1], valid(i), Dk, p.vq); };
     auto fetch_g = [&](int i) { if (wid == NW - 1 && i < vend && lane < valid(i)) rg = g[(first(i) + lane) * a.gs[1]]; };
     auto gates = [&](int i) { if (wid == NW - 1 && i < vend) la_gates(gts[i & 1], rg, lane < valid(i), lane); };
+    float fac = 1.f;
+    auto keep = [&](int i) __attribute__((always_inline)) {               // the state before a chunk, where it is wanted
+        if (float* st = p.local ? (!rev && p.inner && i > ibeg ? p.inner + ((long long)bh * p.nseg + seg) * SS : nullptr)
+                                : p.chunk && i > 0 ? p.chunk + ((long long)bh * p.NC + i) * SS : nullptr) {
+            put_state(st);
+            if (p.local && threadIdx.x == 0 && dvt == 0) p.inner_decay[(long long)bh * p.nseg + seg] = fac;
+        }
+    };
     auto skip = [&](int i) __attribute__((always_inline)) {               // a chunk without tokens
         const int c = chunk_of(i);
         if constexpr (OUT) {
@@ -521,9 +532,8 @@ __global__ __launch_bounds__(64 * NW, (la_scan_waves<DT, DK, NT, NW, OUT>())) vo
             for (int r = wid * 16 + (lane & 15); r < rows; r += 16 * NW)
                 for (int d = dvt * DVT + (lane >> 4) * 4; d < dvt * DVT + DVT && d < Dv; d += 16)
                     la_store4<DT>(out + (long long)r * a.H * Dv + d, f32x4{0.f, 0.f, 0.f, 0.f}, Dv - d, p.vo);
-        } else if (p.chunk && i > 0) put_state(p.chunk + ((long long)bh * p.NC + c) * SS);
+        } else keep(i);
     };
-    float fac = 1.f;
     fetch_g(vbeg);
     fetch_x(vbeg);
     fetch_y(vbeg);
@@ -533,7 +543,7 @@ __global__ __launch_bounds__(64 * NW, (la_scan_waves<DT, DK, NT, NW, OUT>())) vo
     fetch_g(vbeg + 1);
     for (int i = vbeg; i < vend; ++i) {
         const int c = chunk_of(i), nv = valid(i);
-        if (!OUT && p.chunk && i > 0) put_state(p.chunk + ((long long)bh * p.NC + c) * SS);
+        if constexpr (!OUT) keep(i);
         E* out = (E*)p.out + (((long long)b * a.T + (long long)c * LA_C) * a.H + h) * Dv;
         const int rows = a.T - c * LA_C < LA_C ? a.T - c * LA_C : LA_C;
         const long long ot = (long long)a.H * Dv;
@@ -710,31 +720,40 @@ __global__ __launch_bounds__(64) void la_combine(LaScan p, int nseg, long long S
     V s = m.init ? *(const V*)(m.init + bh * SS + e) : V{};
     float* q = m.seg + bh * nseg * SS + e;
     const float* f = m.seg_decay + bh * nseg;
-    V x[8], y[8];
-    float fx[8], fy[8];      // loaded with the states: behind the stores, which might be to them, each would be waited for by itself
-    auto get = [&](int i0, V (&v)[8], float (&w)[8]) {
+    // decays are loaded with the states: behind the stores, which might be to them, each would be waited for by itself
+    struct Round { V x[8], z[8]; float f[8], fz[8]; } now, next;
+    float* inner = blockIdx.z == 0 && p.inner ? p.inner + bh * nseg * SS + e : nullptr;
+    auto get = [&](int i0, Round& r) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            v[j] = i0 + j + 1 < nseg ? *(const V*)(q + (i0 + j) * SS) : V{};
-            w[j] = i0 + j + 1 < nseg ? f[i0 + j] : 0.f;
+            const int i = i0 + j;
+            r.x[j] = i + 1 < nseg ? *(const V*)(q + i * SS) : V{};
+            r.f[j] = i + 1 < nseg ? f[i] : 0.f;
+            if (inner) {
+                const bool on = i < nseg && 2 * i + 1 < p.NC;
+                r.z[j] = on ? *(const V*)(inner + i * SS) : V{};
+                r.fz[j] = on ? p.inner_decay[bh * nseg + i] : 0.f;
+            }
         }
     };
-    get(0, x, fx);
+    get(0, now);
     for (int i0 = 0; i0 < nseg; i0 += 8) {
-        get(i0 + 8, y, fy);
+        get(i0 + 8, next);
 #pragma unroll
         for (int j = 0; j < 8; ++j)
             if (i0 + j < nseg) {
                 *(V*)(q + (i0 + j) * SS) = s;
-                s = s * fx[j] + x[j];
+                if (inner) *(V*)(inner + (i0 + j) * SS) = s * now.fz[j] + now.z[j];
+                s = s * now.f[j] + now.x[j];
             }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) { x[j] = y[j]; fx[j] = fy[j]; }
+        now = next;
     }
 }
 
 struct LaBwd {
-    const float* s_chunk;                // state before each chunk, [B H][NC][Dk][Dv] (chunk 0: s_first)
+    // state before chunk c: s_chunk[c % 2] + (b h * ns + c >> shift) Dk Dv (chunk 0: s_first)
+    const float* s_chunk[2];
+    int ns, shift;
     const float *s_first, *e_last;       // before the sequence / gradient of the state behind it; NULL: 0
     const float* e_seg;                  // gradient of the state behind each segment, [B H][nseg][Dk][Dv], segments from the end (the last one: e_last)
     float* e_first;                      // gradient of the state before the sequence; NULL: not wanted
@@ -869,7 +888,7 @@ __global__ __launch_bounds__((4 * D * la_bwd_halves<DT, D>())) void la_bwd_chunk
     };
     auto fetch_g = [&](int c) { if (wid == NW - 1 && c >= clo && lane < valid(c)) rgn = g[((long long)c * LA_C + lane) * a.gs[1]]; };
     auto gates = [&](int c) { if (wid == NW - 1 && c >= clo) la_gates(gts[c & 1], rgn, lane < valid(c), lane); };
-    auto state_of = [&](int c) { return c == 0 ? (p.s_first ? p.s_first + bh * SS : nullptr) : p.s_chunk + ((long long)bh * p.NC + c) * SS; };
+    auto state_of = [&](int c) { return c == 0 ? (p.s_first ? p.s_first + bh * SS : nullptr) : p.s_chunk[c & 1] + ((long long)bh * p.ns + (c >> p.shift)) * SS; };
     f32x4 xs[KK][2];
     if (cfirst >= clo) {
         fetch_g(cfirst);
@@ -1179,16 +1198,20 @@ __global__ __launch_bounds__((4 * D * la_bwd_halves<DT, D>())) void la_bwd_chunk
 }
 
 // gradients of shared heads: the heads of a group summed in order, rounded once (5 x 777 tokens, 6 heads of 40 to 2: 4.7 us, mostly the launch)
+struct LaShare { const float* src; void* dst; int Hx, rep, D; };
+struct LaShares { LaShare of[3]; };      // q, k, v; src NULL: not shared
 template <int DT>
-__global__ void la_share(const float* src, void* dst_, long long rows, int Hx, int rep, int D) {
+__global__ __launch_bounds__(256) void la_share(LaShares all, long long rows) {
     typedef typename LaT<DT>::T E;
-    E* dst = (E*)dst_;
-    const long long n = rows * Hx * D;
-    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (long long)gridDim.x * blockDim.x) {
-        const long long r = i / D;
-        const int c = (int)(i - r * D);
+    const LaShare m = all.of[blockIdx.y];
+    if (!m.src) return;
+    E* dst = (E*)m.dst;
+    const long long n = rows * m.Hx * m.D;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
+        const long long r = i / m.D;
+        const int c = (int)(i - r * m.D);
         float s = 0.f;
-        for (int j = 0; j < rep; ++j) s += src[(r * rep + j) * D + c];
+        for (int j = 0; j < m.rep; ++j) s += m.src[(r * m.rep + j) * m.D + c];
         dst[i] = LaT<DT>::st(s);
     }
 }
@@ -1418,7 +1441,9 @@ LaFwdWs la_fwd_ws(const LaPlan& p, size_t BH, size_t SS) {
     }
     return w;
 }
-struct LaBwdWs { size_t seg, decay, seg2, decay2, sch, q, k, v, part, total; };
+// Segments of two chunks: the states before the chunks come out of the local pass and the sum over segments, not of a further pass over k and v
+bool la_pairs(const LaPlan& p) { return p.nseg > 1 && p.cps == 2; }
+struct LaBwdWs { size_t seg, decay, seg2, decay2, sch, inner, inner_decay, q, k, v, part, total; };
 LaBwdWs la_bwd_ws(const LaPlan& p, size_t B, size_t T, size_t H, int Hq, int Hk, int Hv, size_t Dk, size_t Dv, int per_token) {
     LaBwdWs w{};
     const size_t SS = Dk * Dv, BH = B * H, n = B * T * H;
@@ -1428,7 +1453,9 @@ LaBwdWs la_bwd_ws(const LaPlan& p, size_t B, size_t T, size_t H, int Hq, int Hk,
     w.decay = take(p.nseg > 1 ? BH * p.nseg * 4 : 0);
     w.seg2 = take(p.nseg > 1 ? BH * p.nseg * SS * 4 : 0);
     w.decay2 = take(p.nseg > 1 ? BH * p.nseg * 4 : 0);
-    w.sch = take(p.NC > 1 ? BH * p.NC * SS * 4 : 0);
+    w.sch = take(p.NC > 1 && !la_pairs(p) ? BH * p.NC * SS * 4 : 0);
+    w.inner = take(la_pairs(p) ? BH * p.nseg * SS * 4 : 0);
+    w.inner_decay = take(la_pairs(p) ? BH * p.nseg * 4 : 0);
     w.q = take((size_t)Hq < H ? n * Dk * 4 : 0);
     w.k = take((size_t)Hk < H ? n * Dk * 4 : 0);
     w.v = take((size_t)Hv < H ? n * Dv * 4 : 0);
@@ -1499,10 +1526,11 @@ int v2a_linattn_bwd(const void* q, const void* k, const void* v, const float* g,
         p.dir[1] = LaDir{dstate_out, at(w.seg2), at(w.decay2), 1, vq, vd, 0};
         if (pl.nseg > 1) {                   // states before the segments, and gradients of those behind them
             p.ndir = 2;
+            if (la_pairs(pl)) { p.inner = at(w.inner); p.inner_decay = at(w.inner_decay); }
             rc = la_segments(a, p, pl, dtype, s);
             if (rc != V2A_OK) return rc;
         }
-        if (pl.NC > 1) {                     // states before the chunks
+        if (pl.NC > 1 && !la_pairs(pl)) {    // states before the chunks
             p.chunk = at(w.sch);
             rc = la_recur<false>(a, p, pl, dtype, s);
             if (rc != V2A_OK) return rc;
@@ -1515,7 +1543,9 @@ int v2a_linattn_bwd(const void* q, const void* k, const void* v, const float* g,
         }
         if (T > 0) {
             LaBwd d{};
-            d.s_chunk = at(w.sch); d.s_first = state; d.e_last = dstate_out; d.e_seg = at(w.seg2); d.e_first = dstate;
+            d.s_chunk[0] = at(la_pairs(pl) ? w.seg : w.sch); d.s_chunk[1] = at(la_pairs(pl) ? w.inner : w.sch);
+            d.ns = la_pairs(pl) ? pl.nseg : pl.NC; d.shift = la_pairs(pl);
+            d.s_first = state; d.e_last = dstate_out; d.e_seg = at(w.seg2); d.e_first = dstate;
             d.cps = pl.cps; d.nseg = pl.nseg;
             d.fq = Hq < H; d.fk = Hk < H; d.fv = Hv < H;
             d.dq = d.fq ? (void*)at(w.q) : dq;
@@ -1534,10 +1564,9 @@ int v2a_linattn_bwd(const void* q, const void* k, const void* v, const float* g,
 #undef BWD
             V2A_CHECK_LAUNCH();
             const long long rows = (long long)B * T;
-#define CALL(DT)                                                                                                                               \
-    if (d.fq) hipLaunchKernelGGL((la_share<DT>), dim3(1024), dim3(256), 0, s, at(w.q), dq, rows, Hq, H / Hq, Dk);                              \
-    if (d.fk) hipLaunchKernelGGL((la_share<DT>), dim3(1024), dim3(256), 0, s, at(w.k), dk, rows, Hk, H / Hk, Dk);                              \
-    if (d.fv) hipLaunchKernelGGL((la_share<DT>), dim3(1024), dim3(256), 0, s, at(w.v), dv, rows, Hv, H / Hv, Dv)
+            const LaShares sh = {{{d.fq ? at(w.q) : nullptr, dq, Hq, H / Hq, Dk}, {d.fk ? at(w.k) : nullptr, dk, Hk, H / Hk, Dk},
+                                  {d.fv ? at(w.v) : nullptr, dv, Hv, H / Hv, Dv}}};
+#define CALL(DT) if (d.fq || d.fk || d.fv) hipLaunchKernelGGL((la_share<DT>), dim3(1024, 3), dim3(256), 0, s, sh, rows)
             LA_BY_TYPE(dtype, CALL);
 #undef CALL
         }
