@@ -410,6 +410,8 @@ def test_two_streams_and_threads_at_once():
 EMB = [  # ids shape, V, D, pos
     ((1,), 1, 1, True), ((1, 20), 1000, 512, True), ((3, 7), 5, 33, True), ((130,), 300, 50, False), ((2, 3, 41), 70, 96, True),
     ((9, 1031), 259, 40, False), ((4, 4100), 70000, 8, True), ((2, 600), 2, 257, False), ((5, 64), 65536, 16, False), ((40000,), 300, 12, True),
+    ((8, 1000), 49408, 8, True), ((3000,), 7, 12, False), ((1500,), 9, 8, False), ((7, 300), 2 ** 20 + 3, 4, False), ((8192,), 1024, 8, False),
+    ((8193,), 1023, 8, False), ((100,), 2 ** 21, 4, True),
 ]
 
 

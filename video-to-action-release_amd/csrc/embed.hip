@@ -1,10 +1,9 @@
 // Token embedding: out[i] = scale * table[id_i] + pos[i mod T], and its gradient: dtable[r] = scale * sum of dout over the tokens r,
 // dpos[t] = sum over the sequences.  Ids outside [0, V) are empty: a zero row, no gradient.  Memory-bound: one read and one write per value.
 //
-// The gradient has no atomics and one order of summation: the tokens are sorted by id (stable, so equal ids stay in token order), a row's
-// tokens are then neighbours, and fixed pieces of the sorted list are summed independently.
-//   launch 1   sort (or the histogram of its first digit) in the first workgroups, dpos and the zero fill of dtable in the others: the
-//              fill and dpos need no order and hide behind the latency-bound sort
+// The gradient has no atomics and one order of summation: the tokens are sorted (stable: equal ids are neighbours, in token order), and fixed pieces of the sorted list are summed independently.
+//   launch 1   sort (or the histogram of its first digit) in the first workgroups, dpos and the zero fill of dtable in the others, which need
+//              no order and run beside it
 //   (launches  further steps of the sort: two per digit where there are more than EM_SMALL tokens)
 //   next       every piece of the list: rows that lie inside a piece are written, rows that cross a border leave fp32 partial sums
 //   last       rows that cross borders: their partial sums, in piece order
@@ -12,7 +11,7 @@
 
 namespace {
 
-constexpr int EM_SORT_T = 1024, EM_WAVES = EM_SORT_T / 64, EM_KPT = 4, EM_SUB = EM_SORT_T * EM_KPT, EM_SMALL = 2 * EM_SUB, EM_BINS = 1024, EM_TILES = 64;
+constexpr int EM_SORT_T = 1024, EM_WAVES = EM_SORT_T / 64, EM_KPT = 4, EM_SUB = EM_SORT_T * EM_KPT, EM_SMALL = 2 * EM_SUB, EM_BINS = 1024, EM_TILES = 32;
 
 template <int DT> struct EmT { typedef unsigned short T; static constexpr int EPC = 8; };
 template <> struct EmT<0> { typedef float T; static constexpr int EPC = 4; };
@@ -98,22 +97,28 @@ __global__ __launch_bounds__(256) void embed_fwd_kernel(const void* ids, int wid
 struct EmSort {
     const void* ids;
     int wide, bits, passes;                 // digits of `bits` bits, low first
+    int split;                              // up to EM_SMALL tokens: low bits that name the workgroup
     unsigned N, V, tile, ntiles;            // tokens per workgroup of the many-workgroup form
     unsigned *key, *pos, *key2, *pos2;      // ping and pong
     unsigned* hist;                         // [ntiles][2^bits]
 };
 
-// Stable rank of each of this wave's 64 * KPT keys (key j of lane l is number 64 j + l) among the wave's equal digits, which also counts
-// them: lanes with the digit's bits all equal find each other by ballots.
+// Stable rank of each of this wave's 64 * kpt keys (key j of lane l is number 64 j + l) among the wave's equal digits, which also counts
+// them: lanes with the digit's bits all equal find each other by ballots (a bit, drawn out over the word, against the ballot of it).
 template <int KPT>
-__device__ __forceinline__ void em_wave_rank(const unsigned (&dig)[KPT], const bool (&on)[KPT], int bits, unsigned short* count, int lane, unsigned (&rank)[KPT]) {
+__device__ __forceinline__ void em_wave_rank(const unsigned (&dig)[KPT], const bool (&on)[KPT], int kpt, int bits, unsigned short* count, int lane, unsigned (&rank)[KPT]) {
 #pragma unroll
     for (int j = 0; j < KPT; ++j) {
-        unsigned long long same = __ballot(on[j]);
+        if (j >= kpt) break;
+        const unsigned long long all = __ballot(on[j]);
+        unsigned lo = (unsigned)all, hi = (unsigned)(all >> 32);
         for (int b = 0; b < bits; ++b) {
-            const unsigned long long m = __ballot((dig[j] >> b) & 1);
-            same &= (dig[j] >> b) & 1 ? m : ~m;
+            const int bit = (int)(dig[j] << (31 - b)) >> 31;
+            const unsigned long long m = __ballot(bit);
+            lo &= ~((unsigned)m ^ bit);
+            hi &= ~((unsigned)(m >> 32) ^ bit);
         }
+        const unsigned long long same = (unsigned long long)hi << 32 | lo;
         const unsigned below = __popcll(same & ((1ull << lane) - 1));
         const unsigned start = on[j] ? count[dig[j]] : 0u;
         rank[j] = start + below;
@@ -135,7 +140,11 @@ __device__ __forceinline__ unsigned em_scan(unsigned v, unsigned* tmp) {
     if (lane == 63) tmp[w] = x;
     __syncthreads();
     unsigned before = 0;
-    for (int i = 0; i < w; ++i) before += tmp[i];
+#pragma unroll
+    for (int i = 0; i < EM_WAVES; ++i) {      // all read at once
+        const unsigned t = tmp[i];
+        before += i < w ? t : 0u;
+    }
     __syncthreads();
     return before + x - v;
 }
@@ -158,58 +167,102 @@ struct EmSortLds {
     unsigned base[EM_BINS], tmp[EM_WAVES];
 };
 
-// Up to EM_SMALL tokens: one workgroup, all digits, through LDS; bound by its barriers and ballots.  8192 tokens
-// with 16 bits take 20 us, beside which the zero fill of 51 MB is hidden.
-__device__ void em_sort_small(const EmSort& s, EmSortLds& L, unsigned (*xch)[EM_SMALL]) {
+// Up to EM_SMALL tokens: a workgroup takes those whose id ends in the bits `blk`, lays them behind the tokens of the workgroups before it
+// (equal ids have to meet, not to be in order) and sorts them by the other bits, all digits through LDS.  Empty places go with the last workgroup,
+// whose largest ids they are.  Bound by the six vector instructions per key and bit of the ballots: 8192 tokens of 49408 rows, half of them one,
+// take 11.5 us (17.3 by one workgroup with two digits); with a zero fill of 51 MB beside it 15.
+__device__ void em_sort_small(const EmSort& s, EmSortLds& L, unsigned (*xch)[EM_SMALL], unsigned blk) {
     constexpr int KPT = EM_SMALL / EM_SORT_T;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, bins = 1 << s.bits;
-    unsigned key[KPT], pos[KPT];
+    const unsigned last = (1u << s.split) - 1;
+    unsigned key[KPT], pos[KPT], n = s.N, start = 0;
     bool on[KPT];
+    int kpt = (n + EM_SORT_T - 1) / EM_SORT_T;
+    auto place = [&](int j) { return (unsigned)(w * 64 * kpt + j * 64 + lane); };
 #pragma unroll
     for (int j = 0; j < KPT; ++j) {
-        const unsigned i = w * 64 * KPT + j * 64 + lane;
-        on[j] = i < s.N;
+        const unsigned i = place(j);
+        on[j] = j < kpt && i < n;
         pos[j] = i;
         key[j] = on[j] ? em_key(s.ids, s.wide, i, s.V) : 0u;
+    }
+    if (s.split) {
+        unsigned own = 0, low = 0;
+        unsigned long long mine[KPT];
+#pragma unroll
+        for (int j = 0; j < KPT; ++j) {
+            const unsigned b = key[j] == s.V ? last : key[j] & last;
+            mine[j] = __ballot(on[j] && b == blk);
+            own += __popcll(mine[j]);
+            low += __popcll(__ballot(on[j] && b < blk));
+        }
+        if (lane == 0) L.tmp[w] = own | low << 16;
+        __syncthreads();
+        unsigned at = 0, sum = 0;
+#pragma unroll
+        for (int i = 0; i < EM_WAVES; ++i) {
+            const unsigned t = L.tmp[i];
+            at += i < w ? t & 0xffffu : 0u;
+            sum += t;
+        }
+        n = sum & 0xffffu;
+        start = sum >> 16;
+        if (n == 0) return;
+#pragma unroll
+        for (int j = 0; j < KPT; ++j) {
+            if (mine[j] >> lane & 1) {
+                const unsigned d = at + __popcll(mine[j] & ((1ull << lane) - 1));
+                xch[0][d] = key[j];
+                xch[1][d] = pos[j];
+            }
+            at += __popcll(mine[j]);
+        }
+        kpt = (n + EM_SORT_T - 1) / EM_SORT_T;
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < KPT; ++j) {
+            const unsigned i = place(j);
+            on[j] = j < kpt && i < n;
+            key[j] = on[j] ? xch[0][i] : 0u;
+            pos[j] = on[j] ? xch[1][i] : 0u;
+        }
     }
     for (int p = 0; p < s.passes; ++p) {
         for (int i = threadIdx.x; i < EM_WAVES * EM_BINS / 2; i += EM_SORT_T) ((unsigned*)L.count)[i] = 0u;
         __syncthreads();
         unsigned dig[KPT], rank[KPT];
 #pragma unroll
-        for (int j = 0; j < KPT; ++j) dig[j] = (key[j] >> (p * s.bits)) & (bins - 1);
-        em_wave_rank(dig, on, s.bits, L.count[w], lane, rank);
+        for (int j = 0; j < KPT; ++j) dig[j] = (key[j] >> (s.split + p * s.bits)) & (bins - 1);
+        em_wave_rank(dig, on, kpt, s.bits, L.count[w], lane, rank);
         __syncthreads();
         unsigned total = 0;
         if (threadIdx.x < bins)
             total = em_waves_scan(L.count);
         L.base[threadIdx.x] = em_scan(total, L.tmp);
         __syncthreads();
+        const bool done = p == s.passes - 1;      // the last places are the list's
 #pragma unroll
         for (int j = 0; j < KPT; ++j)
             if (on[j]) {
                 const unsigned d = L.base[dig[j]] + L.count[w][dig[j]] + rank[j];
-                xch[0][d] = key[j];
-                xch[1][d] = pos[j];
+                if (done) {
+                    s.key[start + d] = key[j];
+                    s.pos[start + d] = pos[j];
+                } else {
+                    xch[0][d] = key[j];
+                    xch[1][d] = pos[j];
+                }
             }
+        if (done) return;
         __syncthreads();
 #pragma unroll
-        for (int j = 0; j < KPT; ++j) {
-            const unsigned i = w * 64 * KPT + j * 64 + lane;
+        for (int j = 0; j < KPT; ++j)
             if (on[j]) {
+                const unsigned i = place(j);
                 key[j] = xch[0][i];
                 pos[j] = xch[1][i];
             }
-        }
         __syncthreads();
-    }
-#pragma unroll
-    for (int j = 0; j < KPT; ++j) {
-        const unsigned i = w * 64 * KPT + j * 64 + lane;
-        if (on[j]) {
-            s.key[i] = key[j];
-            s.pos[i] = pos[j];
-        }
     }
 }
 
@@ -231,35 +284,41 @@ __global__ __launch_bounds__(EM_SORT_T) void embed_hist_kernel(EmSort s, int p) 
     __shared__ unsigned count[EM_BINS];
     em_hist(s, p, blockIdx.x, count);
 }
-// the tokens of a tile to their places of pass p; a workgroup adds up the at most EM_TILES histograms itself (62891 tokens, 9 bits: 11 us)
+// the tokens of a tile to their places of pass p; a workgroup adds up the at most EM_TILES histograms itself.  62891 tokens, 9 bits:
+// 8.4 us in tiles of 2048, 9.1 in 1024, 10.4 in 4096
 __global__ __launch_bounds__(EM_SORT_T) void embed_scatter_kernel(EmSort s, int p) {
     __shared__ EmSortLds L;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, bins = 1 << s.bits;
     unsigned before = 0, total = 0;
     if (threadIdx.x < bins)
-#pragma unroll 8
-        for (unsigned t = 0; t < s.ntiles; ++t) {
-            const unsigned n = s.hist[(size_t)t * bins + threadIdx.x];
-            if (t < blockIdx.x) before += n;
-            total += n;
+        for (unsigned t0 = 0; t0 < s.ntiles; t0 += 16) {
+            unsigned n[16];
+#pragma unroll
+            for (unsigned j = 0; j < 16; ++j) n[j] = t0 + j < s.ntiles ? s.hist[(size_t)(t0 + j) * bins + threadIdx.x] : 0u;
+#pragma unroll
+            for (unsigned j = 0; j < 16; ++j) {
+                if (t0 + j < blockIdx.x) before += n[j];
+                total += n[j];
+            }
         }
     const unsigned start = em_scan(total, L.tmp) + before;
     L.base[threadIdx.x] = start;
     const unsigned a = blockIdx.x * s.tile, end = s.N - a < s.tile ? s.N : a + s.tile;
+    const int kpt = s.tile < (unsigned)EM_SUB ? s.tile / EM_SORT_T : EM_KPT;
     for (unsigned a0 = a; a0 < end; a0 += EM_SUB) {
         for (int i = threadIdx.x; i < EM_WAVES * EM_BINS / 2; i += EM_SORT_T) ((unsigned*)L.count)[i] = 0u;
         unsigned key[EM_KPT], pos[EM_KPT], dig[EM_KPT], rank[EM_KPT];
         bool on[EM_KPT];
 #pragma unroll
         for (int j = 0; j < EM_KPT; ++j) {
-            const unsigned i = a0 + w * 64 * EM_KPT + j * 64 + lane;
-            on[j] = i < end;
+            const unsigned i = a0 + w * 64 * kpt + j * 64 + lane;
+            on[j] = j < kpt && i < end;
             key[j] = !on[j] ? 0u : p == 0 ? em_key(s.ids, s.wide, i, s.V) : s.key[i];
             pos[j] = !on[j] ? 0u : p == 0 ? i : s.pos[i];
             dig[j] = (key[j] >> (p * s.bits)) & (bins - 1);
         }
         __syncthreads();
-        em_wave_rank(dig, on, s.bits, L.count[w], lane, rank);
+        em_wave_rank(dig, on, kpt, s.bits, L.count[w], lane, rank);
         __syncthreads();
         unsigned n = 0;
         if (threadIdx.x < bins)
@@ -295,7 +354,7 @@ __global__ __launch_bounds__(EM_SORT_T) void embed_first_kernel(EmSort s, EmGrad
         float part[EM_WAVES][64 * W];
     } sm;
     if (blockIdx.x < g.nsort) {
-        if (s.N <= (unsigned)EM_SMALL) em_sort_small(s, sm.sort.l, sm.sort.xch);
+        if (s.N <= (unsigned)EM_SMALL) em_sort_small(s, sm.sort.l, sm.sort.xch, blockIdx.x);
         else em_hist(s, 0, blockIdx.x, sm.count);
         return;
     }
@@ -321,15 +380,21 @@ __global__ __launch_bounds__(EM_SORT_T) void embed_first_kernel(EmSort s, EmGrad
 #pragma unroll
         for (int i = 0; i < W; ++i) acc[i] = 0.f;
         if (t < e.T && c < e.D)
-#pragma unroll 4
-            for (unsigned b = w; b < Bn; b += EM_WAVES) {
-                const unsigned r = b * e.T + t;
-                if (em_key(s.ids, s.wide, r, e.V) < e.V) {
-                    float x[W];
-                    em_ld<DT, W>((const E*)g.dout + (size_t)r * e.D + c, x);
+            for (unsigned b0 = w; b0 < Bn; b0 += 4 * EM_WAVES) {
+                float x[4][W];
+                bool on[4];
 #pragma unroll
-                    for (int i = 0; i < W; ++i) acc[i] += x[i];
+                for (unsigned j = 0; j < 4; ++j) {
+                    const unsigned b = b0 + j * EM_WAVES;
+                    on[j] = b < Bn && em_key(s.ids, s.wide, b * e.T + t, e.V) < e.V;
                 }
+#pragma unroll
+                for (unsigned j = 0; j < 4; ++j)
+                    if (on[j]) em_ld<DT, W>((const E*)g.dout + (size_t)((b0 + j * EM_WAVES) * e.T + t) * e.D + c, x[j]);
+#pragma unroll
+                for (unsigned j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int i = 0; i < W; ++i) acc[i] += on[j] ? x[j][i] : 0.f;
             }
 #pragma unroll
         for (int i = 0; i < W; ++i) sm.part[w][i * 64 + lane] = acc[i];
@@ -420,7 +485,8 @@ __global__ __launch_bounds__(256) void embed_pieces_kernel(const unsigned* key, 
 // Rows that cross pieces: the piece in which one begins adds its part 1 and the parts 0 of the pieces behind it, in order.  One wave per
 // (piece, 256 columns), most of which have nothing to do; a run's end is found first, 64 borders at a time, so that the sum has known bounds and
 // loads under way.  Runs over more than EM_LONG pieces are left to the whole workgroup: wave w adds pieces w, w + 16, .., the sums of the waves
-// in order.  (All runs by the workgroup, one after the other, took 22 us where many short ones lie close together, against 10.)
+// in order.  (All runs by the workgroup, one after the other, took 22 us where many short ones lie close together, against 8 to 9, most
+// of it the launch and the dependent reads before the sum.)
 constexpr int EM_JOIN = 16, EM_LONG = 32;
 template <int DT>
 __global__ __launch_bounds__(64 * EM_JOIN) void embed_join_kernel(const unsigned* key, EmGrad g, EmShape e, const float* part, int Dp, unsigned ts) {
@@ -433,6 +499,19 @@ __global__ __launch_bounds__(64 * EM_JOIN) void embed_join_kernel(const unsigned
     const int c0 = blockIdx.y * 256, c = c0 + lane * 4;
     const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
     auto add = [](float4& s, const float4& x) { s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w; };
+    // parts 0 of pieces i, i + step, .. before `to`, eight under way; places behind `to` load the last piece again and leave it out
+    auto sums = [&](float4& s, unsigned i, unsigned to, unsigned step) {
+        for (; i < to; i += 8 * step) {
+            float4 x[8];
+#pragma unroll
+            for (unsigned j = 0; j < 8; ++j) {
+                const unsigned k = i + j * step;
+                x[j] = *(const float4*)(part + (size_t)(k < to ? k : to - 1) * 2 * Dp + c);
+            }
+#pragma unroll
+            for (unsigned j = 0; j < 8; ++j) add(s, i + j * step < to ? x[j] : zero);
+        }
+    };
     unsigned end = 0, cur = 0;
     if (b < e.N) {
         cur = key[b - 1];
@@ -454,8 +533,7 @@ __global__ __launch_bounds__(64 * EM_JOIN) void embed_join_kernel(const unsigned
     if (lane == 0) { ends[w] = wide ? end : 0u; ids[w] = cur; }
     if (end && !wide && c < e.D) {
         float4 s = *(const float4*)(part + (t * 2 + 1) * Dp + c);
-#pragma unroll 8
-        for (unsigned i = (unsigned)t + 1; i < end; ++i) add(s, *(const float4*)(part + (size_t)i * 2 * Dp + c));
+        sums(s, (unsigned)t + 1, __builtin_amdgcn_readfirstlane(end), 1);
         const float x[4] = {s.x, s.y, s.z, s.w};
         E* q = (E*)g.dtable + (size_t)cur * e.D + c;
 #pragma unroll
@@ -463,14 +541,13 @@ __global__ __launch_bounds__(64 * EM_JOIN) void embed_join_kernel(const unsigned
             if (c + r < e.D) q[r] = em_r<DT>(x[r] * g.scale);
     }
     __syncthreads();
-    for (int o = 0; o < EM_JOIN; ++o) {
-        if (ends[o] == 0) continue;
+    for (unsigned long long left = __ballot(lane < EM_JOIN && ends[lane & (EM_JOIN - 1)] != 0); left; left &= left - 1) {
+        const int o = __ffsll(left) - 1;
         const size_t t0 = (size_t)blockIdx.x * EM_JOIN + o;
         float4 s = zero;
         if (c < e.D) {
             if (w == 0) s = *(const float4*)(part + (t0 * 2 + 1) * Dp + c);
-#pragma unroll 8
-            for (unsigned i = (unsigned)t0 + 1 + w; i < ends[o]; i += EM_JOIN) add(s, *(const float4*)(part + (size_t)i * 2 * Dp + c));
+            sums(s, (unsigned)t0 + 1 + w, __builtin_amdgcn_readfirstlane(ends[o]), EM_JOIN);
         }
         *(float4*)&sum[w][lane * 4] = s;
         __syncthreads();
@@ -505,6 +582,12 @@ unsigned em_piece(long long N, int D, int dtype) {
     unsigned ts = 8;
     while (ts < 64 && N * ncol / (ts * 2) >= 4096) ts *= 2;
     return ts;
+}
+// Bits by which up to EM_SMALL tokens are shared out among workgroups: so many that one digit is left, and three where a workgroup alone would
+// have several tokens a thread (8192 tokens, 300 ids: 11.5 us against 12.7)
+int em_split(long long N, int bits) {
+    const int one = bits <= 10 ? 0 : bits < 16 ? bits - 10 : 6, share = N > EM_SORT_T && bits > 3 ? 3 : 0;
+    return one > share ? one : share;
 }
 struct EmWs { size_t key, pos, key2, pos2, hist, part, total; int Dp; unsigned ts; };
 EmWs em_ws(long long N, int D, int dtype) {
@@ -569,18 +652,20 @@ int v2a_embed_bwd(const void* ids, int ids64, const void* dout, void* dtable, vo
     q.ids = ids; q.wide = ids64; q.N = (unsigned)N; q.V = (unsigned)V;
     int bits = 1;
     while ((V >> bits) > 0) ++bits;               // keys 0 .. V
+    if (N <= EM_SMALL) q.split = em_split(N, bits);
+    bits -= q.split;
     q.passes = cdiv(bits, 10);
     q.bits = cdiv(bits, q.passes);
     q.key = (unsigned*)(base + w.key); q.pos = (unsigned*)(base + w.pos);
     q.key2 = (unsigned*)(base + w.key2); q.pos2 = (unsigned*)(base + w.pos2);
     q.hist = (unsigned*)(base + w.hist);
-    q.tile = EM_SUB;
+    q.tile = EM_SORT_T;
     while (cdiv(N, q.tile) > EM_TILES) q.tile *= 2;
     q.ntiles = cdiv(N, q.tile);
     EmGrad g{};
     g.dout = dout; g.dtable = dtable; g.dpos = dpos; g.scale = scale;
     g.P = dpos ? (unsigned)pos_rows : 0u;
-    g.nsort = N == 0 ? 0 : N <= EM_SMALL ? 1 : q.ntiles;
+    g.nsort = N == 0 ? 0 : N <= EM_SMALL ? 1 << q.split : q.ntiles;
     const int W = vec ? (dtype == 0 ? 4 : 8) : 1;
     const long long units = (long long)g.P * cdiv(D, 64 * W), ndpos = units < 4096 ? units : 4096;
     const long long fill = ((long long)V * D * (dtype == 0 ? 4 : 2) + 65535) / 65536;
