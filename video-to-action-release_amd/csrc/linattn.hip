@@ -369,8 +369,10 @@ struct LaScan {
 // another and the tiles leave room for one or two workgroups on a CU: 1 x 32768 tokens x 8 heads of 128, bf16, runs the local pass in 44 us
 // (3.1 TB/s of k and v) and OUT in 93 (2.9 TB/s of rows, 25 % of the MFMA and 41 % of the vector issue slots taken); 8 x 2048 tokens x 8 heads
 // 64 / 128, fp32 in planes, 34 and 74 us; 64 rows of 10 tokens x 8 heads of 48, fp32, 10 us.
+// Tiles are kept twice where two workgroups still fit a CU: the waves then meet once a chunk, not before the tiles are overwritten as well
+template <int DT, bool OUT> constexpr int la_scan_tiles() { return !OUT && DT == 1 ? 2 : 1; }
 template <int DT, int DK, int NT, int NW, bool OUT> constexpr int la_scan_lds() {
-    return LaTile<DT, DK>::BYTES * (OUT ? 2 : 1) + LaTile<DT, 16 * NT * NW>::BYTES + (OUT ? 6 * la_unit_bytes<DT>() : 0);
+    return (LaTile<DT, DK>::BYTES * (OUT ? 2 : 1) + LaTile<DT, 16 * NT * NW>::BYTES) * la_scan_tiles<DT, OUT>() + (OUT ? 6 * la_unit_bytes<DT>() : 0);
 }
 // waves per SIMD that the LDS allows, two at most: the register bound of the launch
 template <int DT, int DK, int NT, int NW, bool OUT> constexpr int la_scan_waves() {
@@ -547,7 +549,10 @@ __global__ __launch_bounds__(64 * NW, (la_scan_waves<DT, DK, NT, NW, OUT>())) vo
         E* out = (E*)p.out + (((long long)b * a.T + (long long)c * LA_C) * a.H + h) * Dv;
         const int rows = a.T - c * LA_C < LA_C ? a.T - c * LA_C : LA_C;
         const long long ot = (long long)a.H * Dv;
-        __syncthreads();
+        if constexpr (la_scan_tiles<DT, OUT>() == 2) {
+            sx = sm + (i & 1) * (TX::BYTES + TY::BYTES);
+            sy = sx + TX::BYTES;
+        } else __syncthreads();
         rx.store(sx);
         ry.store(sy);
         if constexpr (OUT) rq.store(sq);
