@@ -996,7 +996,7 @@ __global__ __launch_bounds__((4 * D * la_bwd_halves<DT, D>())) void la_bwd_chunk
 #pragma unroll
             for (int u = 0; u < 6; ++u) {
                 const int jt = 3 - la_unit_tile(u), is = 32 - la_unit_step(u) * 32;
-                constexpr int per = NW == 8 ? 1 : NW == 4 ? 2 : 3;
+                constexpr int per = NW >= 6 ? 1 : NW == 4 ? 2 : 3;
                 const int at = u % per;
                 if (la_unit_wave(u, NW) != wid || jt * 16 >= nv || is >= nv) continue;
                 f32x4 c0 = {0.f, 0.f, 0.f, 0.f}, c1 = {0.f, 0.f, 0.f, 0.f};
@@ -1565,6 +1565,7 @@ int v2a_linattn_bwd(const void* q, const void* k, const void* v, const float* g,
 #define BWD(DT, D) hipLaunchKernelGGL((la_bwd_chunks<DT, D>), grid, dim3(4 * D * la_bwd_halves<DT, D>()), 0, s, a, d)
             if (Dm <= 32) { if (dtype == 0) BWD(0, 32); else if (dtype == 1) BWD(1, 32); else BWD(2, 32); }
             else if (Dm <= 64) { if (dtype == 0) BWD(3, 64); else if (dtype == 1) BWD(1, 64); else BWD(2, 64); }
+            else if (Dm <= 96) { if (dtype == 0) BWD(0, 96); else if (dtype == 1) BWD(1, 96); else BWD(2, 96); }
             else { if (dtype == 0) BWD(0, 128); else if (dtype == 1) BWD(1, 128); else BWD(2, 128); }
 #undef BWD
             V2A_CHECK_LAUNCH();
