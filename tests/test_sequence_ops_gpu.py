@@ -113,6 +113,7 @@ SHAPES = [
     (2, 260, 2, 1, 2, 2, 32, 20, "token", True),
     (1, 192, 2, 2, 2, 1, 80, 48, "token", True),
     (2, 900, 40, 40, 8, 40, 40, 36, "token", True),          # segments of four chunks
+    (2, 333, 3, 3, 1, 3, 72, 96, "token", True), (1, 130, 2, 1, 2, 2, 96, 80, "head", True), (1, 450, 2, 2, 2, 1, 66, 91, "token", False),
 ]
 
 

@@ -417,9 +417,9 @@ __global__ __launch_bounds__(64 * NW, (la_scan_waves<DT, DK, NT, NW, OUT>())) vo
     f32x4 S[DK / 16][NT];
     constexpr int CS = OUT && NT == 2 ? 8 : 4, NC0 = CS == 8 ? 4 : 16;
     const int d0 = OUT ? (lane >> 4) * 8 : lane & 15, c0 = OUT ? dv0 + CS * ((lane & 15) >> 2) + (lane & 3) : dv0 + (lane >> 4) * 4;
-    // OUT exchanges the state through LDS, half of the rows at a time (in whole 32-row blocks), so that memory sees whole rows
-    constexpr int NH = DK == 32 ? 1 : 2, HR = DK / NH, PER = HR * DVT / 4 / NTH;
-    static_assert(!OUT || HR * DVT * 4 <= la_scan_lds<DT, DK, NT, NW, OUT>(), "half a state fits");
+    // OUT exchanges the state through LDS, a part of the rows at a time (in whole 32-row blocks), so that memory sees whole rows
+    constexpr int NH = DK == 32 ? 1 : DK == 96 ? 3 : 2, HR = DK / NH, PER = HR * DVT / 4 / NTH;
+    static_assert(!OUT || HR * DVT * 4 <= la_scan_lds<DT, DK, NT, NW, OUT>(), "the part fits");
     auto get_state = [&](const float* s0) __attribute__((always_inline)) {
         if constexpr (OUT) {
 #pragma unroll
@@ -1354,10 +1354,12 @@ size_t la_up(size_t n) { return (n + 255) & ~(size_t)255; }
 struct LaPlan {
     int dvt, ndv, NC, cps, nseg;
 };
+// Both widths from 65 to 96: tiles of 96 and six waves
+bool la_96(int Dk, int Dv) { return Dk > 64 && Dk <= 96 && Dv > 64 && Dv <= 96; }
 LaPlan la_plan(int BH, int T, int Dk, int Dv, int dtype, int target) {
     constexpr int least = 2;
     LaPlan p;
-    p.dvt = Dv <= 32 ? 32 : Dv <= 64 || (dtype == 0 && Dk > 64) ? 64 : 128;
+    p.dvt = Dv <= 32 ? 32 : la_96(Dk, Dv) ? 96 : Dv <= 64 || (dtype == 0 && Dk > 64) ? 64 : 128;
     p.ndv = cdiv(Dv, p.dvt);
     p.NC = cdiv(T, LA_C);
     p.nseg = 1;
@@ -1406,6 +1408,12 @@ template <int DT, int DK, bool OUT> int la_scan_dv(const LaArgs& a, const LaScan
 template <int DT, bool OUT> int la_scan_dk(const LaArgs& a, const LaScan& p, int dvt, hipStream_t s) {
     if (a.Dk <= 32) return la_scan_dv<DT, 32, OUT>(a, p, dvt, s);
     if (a.Dk <= 64) return la_scan_dv<DT, 64, OUT>(a, p, dvt, s);
+    if constexpr (DT != 0)
+        if (dvt == 96) {
+            hipLaunchKernelGGL((la_scan<DT, 96, 1, 6, OUT>), dim3((unsigned)((long long)a.B * a.H * p.nseg * p.ndir)), dim3(384), 0, s, a, p);
+            V2A_CHECK_LAUNCH();
+            return V2A_OK;
+        }
     if constexpr (DT == 0) return V2A_ERR_ARG;      // la_plain_fp32
     else return la_scan_dv<DT, 128, OUT>(a, p, dvt, s);
 }
