@@ -131,6 +131,14 @@ def test_c_entries_return_error_codes_before_any_launch():
     assert lib.v2a_embed_bwd(None, 1, None, None, None, 6, 3, 0, 8, 0, 0, 1.0, None, 0, None) == -1
 
 
+def test_workspaces_of_long_calls_without_rows():
+    from v2a_hip._lib import lib
+    assert lib.v2a_linattn_fwd_workspace_bytes(0, 5000, 4, 64, 64, 1) == 0
+    for T in (0, 1, 300, 5000):
+        assert lib.v2a_linattn_bwd_workspace_bytes(0, T, 4, 4, 4, 4, 64, 64, 1, 1) == 0
+    assert lib.v2a_linattn_bwd_workspace_bytes(1, 5000, 4, 4, 4, 4, 64, 64, 1, 1) > 0
+
+
 def test_oracle_gradient_against_differences():
     """The oracle's hand-written gradient against central differences of its own forward (fp64, step 1e-5: error ~1e-10 of the value)."""
     gen = torch.Generator().manual_seed(3)

@@ -213,6 +213,13 @@ def test_no_tokens_and_no_rows():
     assert ops().linear_attention_step(*(x[:, 0] if x.dim() == 4 else x for x in z(0, 5)), torch.zeros(0, 4, 8, 16).cuda()).shape == (0, 4, 16)
 
 
+def test_long_sequences_of_no_rows():
+    q, v, g = torch.zeros(0, 700, 4, 8).cuda(), torch.zeros(0, 700, 4, 16).cuda(), torch.zeros(4).cuda()
+    assert ops().linear_attention_fwd(q, q, v, g)[0].shape == (0, 700, 4, 16)
+    dq, dk, dv, dg, _ = ops().linear_attention_bwd(q, q, v, g, v)
+    assert dq.shape == q.shape and dv.shape == v.shape and dg.shape == (4,) and not dg.any()
+
+
 def check_step(c, t, S, slots=None, scale=None):
     """One call against the recurrence, rows of one slot in order."""
     B, H = c["q"].shape[0], c["g"].shape[-1]

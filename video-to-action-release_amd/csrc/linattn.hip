@@ -1354,30 +1354,41 @@ size_t la_up(size_t n) { return (n + 255) & ~(size_t)255; }
 struct LaPlan {
     int dvt, ndv, NC, cps, nseg;
 };
-// Both widths from 65 to 96: tiles of 96 and six waves
-bool la_96(int Dk, int Dv) { return Dk > 64 && Dk <= 96 && Dv > 64 && Dv <= 96; }
-LaPlan la_plan(int BH, int T, int Dk, int Dv, int dtype, int target) {
+// State columns per workgroup; both widths from 65 to 96: tiles of 96 and six waves
+int la_dvt(int Dk, int Dv, int dtype) {
+    return Dv <= 32 ? 32 : Dk > 64 && Dk <= 96 && Dv > 64 && Dv <= 96 ? 96 : Dv <= 64 || (dtype == 0 && Dk > 64) ? 64 : 128;
+}
+// `wg` workgroups without segments, `room` for as many at once; a chunk costs `more` tenths with segments of what it costs without (the pass for
+// their states), and a segment about one chunk of its own.  One or two rounds of the chip, whichever ends first: a round that is nearly empty takes
+// as long as a full one.
+LaPlan la_plan(int T, int Dk, int Dv, int dtype, long wg, int room, int more) {
     constexpr int least = 2;
     LaPlan p;
-    p.dvt = Dv <= 32 ? 32 : la_96(Dk, Dv) ? 96 : Dv <= 64 || (dtype == 0 && Dk > 64) ? 64 : 128;
+    p.dvt = la_dvt(Dk, Dv, dtype);
     p.ndv = cdiv(Dv, p.dvt);
     p.NC = cdiv(T, LA_C);
     p.nseg = 1;
     p.cps = p.NC;
-    const long wg = (long)BH * p.ndv;
-    if (p.NC >= 2 * least && wg < target) {
-        p.cps = cdiv(p.NC, cdiv(target, wg));
-        if (p.cps < least) p.cps = least;
-        p.nseg = cdiv(p.NC, p.cps);
-    }
+    long best = 10l * p.NC;
+    if (p.NC >= 2 * least && wg > 0 && wg < room)
+        for (int k = 1; k <= 2; ++k) {
+            int cps = cdiv(p.NC, (int)(k * room / wg));
+            if (cps < least) cps = least;
+            const int nseg = cdiv(p.NC, cps);
+            const long cost = (long)more * cdiv(nseg * wg, room) * (cps + 1);
+            if (nseg > 1 && cost < best) { best = cost; p.cps = cps; p.nseg = nseg; }
+        }
     return p;
 }
 // as many workgroups as fit the chip at once, by their LDS: two on a CU where they take 80 KB at most, else one.  More segments than that only
 // add states: 8 x 2048 tokens x 8 heads fp32 took 137 us with 256 workgroups, 144 with 512, 167 with 1024; 1 x 32768 x 8 bf16 182, 153, 180
 LaPlan la_plan_fwd(int BH, int T, int Dk, int Dv, int dtype) {
-    return la_plan(BH, T, Dk, Dv, dtype, dtype == 1 || (Dk <= 64 && Dv <= 64) ? 512 : 256);
+    return la_plan(T, Dk, Dv, dtype, (long)BH * cdiv(Dv, la_dvt(Dk, Dv, dtype)), dtype == 1 || (Dk <= 64 && Dv <= 64) ? 512 : 256, 15);
 }
-LaPlan la_plan_bwd(int BH, int T, int Dk, int Dv, int dtype) { return la_plan(BH, T, Dk, Dv, dtype, Dk <= 32 && Dv <= 32 ? 512 : dtype == 1 && Dk <= 64 && Dv <= 64 ? 512 : 256); }
+// by the gradient kernel, whose workgroups have all columns
+LaPlan la_plan_bwd(int BH, int T, int Dk, int Dv, int dtype) {
+    return la_plan(T, Dk, Dv, dtype, BH, (Dk <= 32 && Dv <= 32) || (dtype == 1 && Dk <= 64 && Dv <= 64) ? 512 : 256, 12);
+}
 
 int la_vec(const void* p, const long long* st, int B, int T, int H, int D, int dtype) {
     const long long es = dtype == 0 ? 4 : 2;
