@@ -366,9 +366,9 @@ struct LaScan {
 // the state in accumulators.  OUT: the outputs as well; otherwise the states alone (of a segment that starts at 0, or before every chunk for the
 // gradient).  Columns of the state never meet, so a tile of them costs k again but no exchange; scores are computed once a workgroup, by units,
 // and shared through LDS.  Bound by the issue of vector, LDS and matrix instructions rather than by memory, since a chunk's stages depend on one
-// another and the tiles leave room for one or two workgroups on a CU: 1 x 32768 tokens x 8 heads of 128, bf16, runs the local pass in 44 us
-// (3.1 TB/s of k and v) and OUT in 93 (2.9 TB/s of rows, 25 % of the MFMA and 41 % of the vector issue slots taken); 8 x 2048 tokens x 8 heads
-// 64 / 128, fp32 in planes, 34 and 74 us; 64 rows of 10 tokens x 8 heads of 48, fp32, 10 us.
+// another and the tiles leave room for one or two workgroups on a CU: 1 x 32768 tokens x 8 heads of 128, bf16, runs the local pass in 42 us
+// (168 MB with the states it leaves, 4 TB/s) and OUT in 91 (302 MB, 3.3 TB/s, 25 % of the MFMA and 41 % of the vector issue slots taken); 8 x 2048 tokens x 8 heads
+// 64 / 128, fp32 in planes, 36 and 74 us; 64 rows of 10 tokens x 8 heads of 48, fp32, 10 us.
 // Tiles are kept twice where two workgroups still fit a CU: the waves then meet once a chunk, not before the tiles are overwritten as well
 template <int DT, bool OUT> constexpr int la_scan_tiles() { return !OUT && DT == 1 ? 2 : 1; }
 template <int DT, int DK, int NT, int NW, bool OUT> constexpr int la_scan_lds() {
@@ -714,8 +714,8 @@ __global__ __launch_bounds__(64 * NW, (la_scan_waves<DT, DK, NT, NW, OUT>())) vo
 }
 
 // Local states of the segments -> states before them: S_0 = init, S_{s+1} = decay_s S_s + local_s, in place; W neighbours a lane, eight segments
-// a round and the next round's loads ahead of this one's stores.  A chain of nseg steps a lane, bound by its latency: 22 us for 8 heads of 128
-// in 64 segments (67 MB, 3 TB/s), 5.6 us for 64 heads 64 / 128 in 4.
+// a round and the next round's loads ahead of this one's stores.  A chain of nseg steps a lane, bound by memory: 17 to 20 us for 8 heads of
+// 128 in 64 segments (67 MB), 5.7 us for 64 heads 64 / 128 in 4.
 template <int W>
 __global__ __launch_bounds__(64) void la_combine(LaScan p, int nseg, long long SS) {
     typedef typename std::conditional<W == 4, f32x4, float>::type V;
@@ -782,8 +782,8 @@ struct LaBwd {
 // TH 2: two waves share each block of 16 rows and take half of the chunk's tokens each (E in both): where the LDS allows one workgroup of narrow
 // heads on a CU, its D / 16 waves alone would leave the matrix units waiting.
 // Bound by the latency of a chunk's dependent stages, with the four tiles filling the LDS of a CU (one workgroup of 128-wide heads): 4 x 4096
-// tokens x 8 heads of 128, bf16, decays per token: 160 us, 285 MB of HBM traffic at 1.8 TB/s, 14 % of the MFMA and 35 % of the vector issue
-// slots; fp32 4 x 2048 x 4 heads of 128 167 us; 8 x 2048 x 8 heads of 64 bf16 70 us, fp32 141.  64 rows of 16 tokens x 4 heads of 64, fp32: 14 us.
+// tokens x 8 heads of 128, bf16, decays per token: 156 us, 285 MB of HBM traffic at 1.8 TB/s, 14 % of the MFMA and 35 % of the vector issue
+// slots; fp32 4 x 2048 x 4 heads of 128 96 us; 8 x 2048 x 8 heads of 64 bf16 66 us, fp32 131; 8 x 2048 x 4 heads of 96 bf16 69, 80 / 96 fp32 137.  64 rows of 16 tokens x 4 heads of 64, fp32: 14 us.
 template <int DT, int D> constexpr int la_bwd_halves() { return D == 32 || (D == 64 && DT != 1) ? 2 : 1; }
 template <int DT, int D>
 __global__ __launch_bounds__((4 * D * la_bwd_halves<DT, D>())) void la_bwd_chunks(LaArgs a, LaBwd p) {
@@ -1202,7 +1202,7 @@ __global__ __launch_bounds__((4 * D * la_bwd_halves<DT, D>())) void la_bwd_chunk
             }
 }
 
-// gradients of shared heads: the heads of a group summed in order, rounded once (5 x 777 tokens, 6 heads of 40 to 2: 4.7 us, mostly the launch)
+// gradients of shared heads: the heads of a group summed in order, rounded once (5 x 777 tokens, 6 heads of 40 to 2, q and k: 4.7 us, mostly the launch)
 struct LaShare { const float* src; void* dst; int Hx, rep, D; };
 struct LaShares { LaShare of[3]; };      // q, k, v; src NULL: not shared
 template <int DT>
