@@ -12,6 +12,7 @@ gradients per step (issued as two asynchronous slice all-reduces: the Conditiona
 backward), averaged by folding 1/world into the optimiser's gradient scale.
 """
 import copy
+import weakref
 import numpy as np
 import torch
 from . import ops
@@ -119,7 +120,16 @@ class PolicyTrainer:
             mi = [i for i, n in enumerate(self.names) if n.startswith("model.")]
             if mi and mi[-1] - mi[0] + 1 == len(mi):         # (the model.* group is contiguous in the arena, first or last)
                 self._presum_range = self.opt.chunk_range(mi[0], mi[-1] + 1)
-                self.eng.on_unet_wgrads_done = self._presum
+                # held weakly: the engine must not keep its trainer alive.  A bound method here closes a cycle (trainer -> engine -> hook ->
+                # trainer), and the graph, streams and arenas of a dropped trainer would go when the cyclic collector happens to run, in the
+                # middle of the next trainer's capture for instance.
+                hook = weakref.WeakMethod(self._presum)
+
+                def presum_hook():
+                    f = hook()
+                    if f is not None:
+                        f()
+                self.eng.on_unet_wgrads_done = presum_hook
         self._pack_serial = -1
         self._packs_fused = False
         self._pack_side = None
