@@ -348,7 +348,7 @@ class GoalGaussianDiffusion(nn.Module):
         step()                                    # eager once: weight packs, workspaces, allocator warm
         torch.cuda.synchronize()
         graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(graph, **ops.graph_capture_mode()):
+        with ops.capture_graph(graph, **ops.graph_capture_mode()):
             step()
         g["graph"] = graph
         return g

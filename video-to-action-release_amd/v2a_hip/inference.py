@@ -89,7 +89,7 @@ class GraphedPredictAction:
             self._run()                                   # warm-up (packs, workspace)
             torch.cuda.synchronize()
             self.graph = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(self.graph, **ops.graph_capture_mode()):
+            with ops.capture_graph(self.graph, **ops.graph_capture_mode()):
                 self._run()
         self.graph.replay()
         if self.pp is not None:

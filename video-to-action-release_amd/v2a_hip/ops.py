@@ -4,8 +4,10 @@ PyTorch is used for device memory and streams only; every arithmetic op below is
 libv2a_hip.so launched on torch's current stream with raw pointers.
 All activations are channels-last fp32: images [N,H,W,C], sequences [N,T,C], video [B,F,H,W,C].
 """
+import contextlib
 import ctypes
 import functools
+import gc
 import os
 import threading
 import weakref
@@ -133,6 +135,31 @@ def graph_capture_mode():
     except Exception:
         pass
     return {}
+
+
+_captures, _capture_lock, _gc_was_on = 0, threading.Lock(), True
+
+
+@contextlib.contextmanager
+def capture_graph(graph, **kw):
+    """`torch.cuda.graph(graph, **kw)` with the cyclic garbage collector held off until the capture has ended: a capture allocates enough
+    container objects to set the collector off, and what it may find then -- a graph, stream or event in a dropped reference cycle of the
+    program -- would be destroyed by calls to the runtime in the middle of the capture.  Captures may overlap (several host threads): the last
+    one to end restores the program's own setting."""
+    global _captures, _gc_was_on
+    with _capture_lock:
+        if _captures == 0:
+            _gc_was_on = gc.isenabled()
+            gc.disable()
+        _captures += 1
+    try:
+        with torch.cuda.graph(graph, **kw):
+            yield
+    finally:
+        with _capture_lock:
+            _captures -= 1
+            if _captures == 0 and _gc_was_on:
+                gc.enable()
 
 
 _h_twin_regs = 0
