@@ -38,11 +38,7 @@ class HashTextEncoder(nn.Module):
         self.eval()
 
     def forward(self, input_ids, attention_mask=None):
-        if self.table.is_cuda and input_ids.is_cuda:
-            from v2a_hip import ops
-            h = ops.embed_fwd(input_ids.contiguous(), self.table, pos=self.pos)        # the sum below, bit for bit
-        else:
-            h = self.table[input_ids] + self.pos[:input_ids.shape[1]][None]
+        h = self.table[input_ids] + self.pos[:input_ids.shape[1]][None]
         return SimpleNamespace(last_hidden_state=h)
 
 
