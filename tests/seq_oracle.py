@@ -73,3 +73,49 @@ def embed_grads(ids, dout, vocab, scale, pos_rows=None):
         dpos = torch.zeros(pos_rows, D, dtype=torch.float64)
         dpos[:T] = d.reshape(-1, T, D).sum(0)
     return dtable, dpos
+
+
+def decay_parts(q, k, v, g, dout, state=None, lens=None, scale=None, dlast=None, chunk=64):
+    """Magnitude of what a chunk-wise sum for d decay adds up at each token -> [B,T,H]: for the chunk of `chunk` tokens that the token lies in,
+    exp(G) <|S|, |E|> (state before the chunk, gradient of the one behind it), the products of its tokens with that state and that gradient,
+    and twice its pair products (each is added in one row's sum and taken off in another's)."""
+    B, T = q.shape[:2]
+    H = g.shape[-1]
+    scale = q.shape[-1] ** -0.5 if scale is None else abs(scale)
+    q, k, v = (_heads(x, H).abs() for x in (q, k, v))
+    do = dout.double().cpu().abs() * scale
+    g = g.double().cpu().expand(B, T, H)
+    n = torch.full((B,), T) if lens is None else lens.long().cpu().clamp(0, T)
+    on = torch.arange(T)[None, :] < n[:, None]
+    q, k, v, do = (torch.where(on[..., None, None], x, torch.zeros(()).double()) for x in (q, k, v, do))
+    a = torch.where(on[..., None], torch.exp(g), torch.ones(()).double())
+    S = torch.zeros(B, H, q.shape[-1], v.shape[-1], dtype=torch.float64) if state is None else state.double().cpu().abs()
+    E = torch.zeros_like(S) if dlast is None else dlast.double().cpu().abs()
+    before, behind, starts = [], {}, list(range(0, T, chunk))
+    for t in range(T):
+        if t % chunk == 0:
+            before.append(S)
+        S = a[:, t, :, None, None] * S + k[:, t, :, :, None] * v[:, t, :, None, :]
+    for t in reversed(range(T)):
+        if t == T - 1 or (t + 1) % chunk == 0:
+            behind[t // chunk] = E
+        E = a[:, t, :, None, None] * (E + q[:, t, :, :, None] * do[:, t, :, None, :])
+    out = torch.zeros(B, T, H, dtype=torch.float64)
+    for c, t0 in enumerate(starts):
+        t1 = min(T, t0 + chunk)
+        ac = a[:, t0:t1]
+        L = t1 - t0
+        W = torch.zeros(B, H, L, L, dtype=torch.float64)                       # decay from token j to token i, j <= i
+        for i in range(L):
+            W[:, :, i, i] = 1
+            if i:
+                W[:, :, i, :i] = W[:, :, i - 1, :i] * ac[:, i, :, None]
+        head = torch.cumprod(ac, 1)                                            # from before the chunk to token i
+        tail = W[:, :, -1].transpose(1, 2)                                     # from token j to the chunk's end
+        qc, kc, vc, dc = (x[:, t0:t1] for x in (q, k, v, do))
+        R = head * (torch.matmul(dc[:, :, :, None], before[c].transpose(-1, -2)[:, None])[..., 0, :] * qc).sum(-1)
+        C = tail * (torch.matmul(vc[:, :, :, None], behind[c].transpose(-1, -2)[:, None])[..., 0, :] * kc).sum(-1)
+        M = W * torch.einsum("bihd,bjhd->bhij", qc, kc) * torch.einsum("bihd,bjhd->bhij", dc, vc)
+        Z = head[:, -1] * (before[c] * behind[c]).sum((-1, -2))
+        out[:, t0:t1] = (Z + R.sum(1) + C.sum(1) + 2 * M.sum((-1, -2)))[:, None]
+    return out
