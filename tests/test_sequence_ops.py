@@ -160,3 +160,15 @@ def test_oracle_gradient_against_differences():
         want = (loss(up) - loss(down)) / 2e-5
         got = (gr * d).sum()
         assert abs(got - want) <= 1e-7 * (gr * d).abs().sum(), i
+
+
+def test_a_refusal_of_slots_names_them():
+    from v2a_hip import ops
+
+    class OnGpu(torch.Tensor):
+        is_cuda = True
+
+    s = [x[:, 0].as_subclass(OnGpu) if x.dim() == 4 else x.as_subclass(OnGpu) for x in _la()]
+    for slots in (torch.zeros(2, dtype=torch.int64), torch.zeros(3, dtype=torch.int32), torch.zeros(4, dtype=torch.int32)[::2]):
+        with pytest.raises(ValueError, match="slots"):
+            ops.linear_attention_step.__wrapped__(*s, torch.zeros(3, 4, 8, 16), slots=slots)

@@ -1621,9 +1621,9 @@ def _la_state(t, shape, what):
         raise ValueError(f"{what}: need contiguous fp32 {list(shape)}")
 
 
-def _la_lens(lens, B):
+def _la_lens(lens, B, what="lens"):
     if lens.dtype != torch.int32 or lens.shape != (B,) or not lens.is_contiguous():
-        raise ValueError(f"lens: need contiguous int32 [{B}]")
+        raise ValueError(f"{what}: need contiguous int32 [{B}]")
 
 
 def _g_strides(g, lead):
@@ -1702,7 +1702,7 @@ def linear_attention_step(q, k, v, log_decay, state, slots=None, scale=None):
     N = state.shape[0]
     _la_state(state, (N, H, Dk, Dv), "state")
     if slots is not None:
-        _la_lens(slots, B)
+        _la_lens(slots, B, "slots, like lens")
     elif N != B:
         raise ValueError("state: need one row per row of q, or slots")
     out = q.new_empty((B, H, Dv))
