@@ -56,7 +56,7 @@ def _ipc_export(ptr: int):
     off, size = ctypes.c_uint64(), ctypes.c_uint64()
     check(lib.v2a_dp_ipc_export(ptr, h, ctypes.byref(off), ctypes.byref(size)), "dp_ipc_export")
     if (1 << 31) <= size.value < (1 << 32):
-        # measured on this runtime (ROCm 7.2, tools/probes/r5/ipc_open_size_probe.py, profiles/r05_dp_direct.txt): a peer that maps an
+        # measured on this runtime (ROCm 7.2, profiles/r05_dp_direct.txt): a peer that maps an
         # allocation of 2 GiB <= size < 4 GiB never returns from hipIpcOpenMemHandle; 0.5 / 1 / 1.5 / 1.99 and 4 / 8 / 16 GiB map at once
         raise RuntimeError(f"the memory to share is a window of an allocation of {size.value} bytes: peers cannot map allocations of 2 to 4 GiB "
                            f"on this runtime (hipIpcOpenMemHandle does not return).  Build the arena with v2a_hip.dp.alloc_arena()")
