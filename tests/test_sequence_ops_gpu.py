@@ -277,6 +277,15 @@ def test_step_idle_rows_and_repeated_slots():
     assert not o.any() and torch.equal(S.cpu(), pool)
 
 
+def test_step_on_a_pool_without_states():
+    """N = 0: there is no slot to name, every row is idle."""
+    c = make(7, 3, 1, 2, 2, 1, 2, 12, 20, F32)
+    for slots in ([0, -1, 5], [2 ** 31 - 1, 0, 0]):
+        o = ops().linear_attention_step(*(cu(c[x][:, 0]) for x in ("q", "k", "v", "g")), torch.zeros(0, 2, 12, 20).cuda(),
+                                        slots=torch.tensor(slots, dtype=torch.int32).cuda())
+        assert o.shape == (3, 2, 20) and not o.any()
+
+
 @pytest.mark.parametrize("dt", [F32, BF, FP], ids=["fp32", "bf16", "fp16"])
 def test_prompt_then_tokens_is_the_whole_sequence(dt):
     c = make(11, 3, 140, 6, 6, 2, 3, 48, 64, dt)

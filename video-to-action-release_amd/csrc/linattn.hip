@@ -1605,7 +1605,7 @@ int v2a_linattn_step(const void* q, const void* k, const void* v, const float* g
                      int N, int H, int Hq, int Hk, int Hv, int Dk, int Dv, int dtype, float scale, hipStream_t s) {
     if (!strides || !la_dims(B, 1, H, Hq, Hk, Hv, Dk, Dv, dtype) || N < 0 || (!slots && N < B)) return V2A_ERR_ARG;
     if (B == 0) return V2A_OK;
-    if (!q || !k || !v || !g || !state || !out) return V2A_ERR_ARG;
+    if (!q || !k || !v || !g || (!state && N > 0) || !out) return V2A_ERR_ARG;      // N = 0: every row is idle
     const int64_t* t = strides;
     const bool vec = Dv % 4 == 0 && ((uintptr_t)state & 15) == 0;
     int lv = 1;
