@@ -218,7 +218,8 @@ int v2a_dropout(const float* x, float* y, size_t n, float p, uint64_t seed, uint
  * per control tick:  S_t = exp(g_t) S_{t-1} + k_t v_t^T  (fp32, [Dk][Dv] per batch row and head),  out_t = scale * S_t^T q_t.
  *   q [B,T,Hq,Dk], k [B,T,Hk,Dk], v [B,T,Hv,Dv], dout [B,T,H,Dv]: dtype 0 fp32 / 1 bf16 / 2 fp16, any strides over (batch, token, head), last
  *     dimension contiguous.  Hq, Hk, Hv divide H: head h reads shared head h / (H / Hx).  Dk, Dv <= 128.
- *   g: fp32 log decays, strides over (batch, token, head); stride 0 over batch and token is one decay per head.  -inf clears the state.
+ *   g: fp32 log decays, strides over (batch, token, head); stride 0 over batch and token is one decay per head.  -inf (a factor of 0) clears a
+ *     finite state.  B * H * (T / 64 + 1) < 2^23.
  *   state / dstate [B,H,Dk,Dv] fp32: the state before the first token (NULL = 0) and its gradient; state_out / dstate_out: after the last.
  *   lens (NULL = T): int32 [B]; tokens from lens[b] on are not read, their out / gradient rows are 0 (values outside [0, T] are clamped).
  *   out [B,T,H,Dv], dq / dk / dv like q / k / v: contiguous, in dtype.  dg: fp32, [B,T,H] with per_token_decay, else [H]; may be NULL.

@@ -367,8 +367,8 @@ struct LaScan {
 // gradient).  Columns of the state never meet, so a tile of them costs k again but no exchange; scores are computed once a workgroup, by units,
 // and shared through LDS.  Bound by the issue of vector, LDS and matrix instructions rather than by memory, since a chunk's stages depend on one
 // another and the tiles leave room for one or two workgroups on a CU: 1 x 32768 tokens x 8 heads of 128, bf16, runs the local pass in 42 us
-// (168 MB with the states it leaves, 4 TB/s) and OUT in 91 (302 MB, 3.3 TB/s, 25 % of the MFMA and 41 % of the vector issue slots taken); 8 x 2048 tokens x 8 heads
-// 64 / 128, fp32 in planes, 36 and 74 us; 64 rows of 10 tokens x 8 heads of 48, fp32, 10 us.
+// (165 MB read and written, 4 TB/s, 29 % of the MFMA and 48 % of the vector issue slots taken) and OUT in 92 (303 MB, 3.3 TB/s, 26 % and 39 %);
+// 8 x 2048 tokens x 8 heads 64 / 128, fp32 in planes, 36 and 77 us; 64 rows of 10 tokens x 8 heads of 48, fp32, 10 us.
 // Tiles are kept twice where two workgroups still fit a CU: the waves then meet once a chunk, not before the tiles are overwritten as well
 template <int DT, bool OUT> constexpr int la_scan_tiles() { return !OUT && DT == 1 ? 2 : 1; }
 template <int DT, int DK, int NT, int NW, bool OUT> constexpr int la_scan_lds() {
@@ -782,8 +782,8 @@ struct LaBwd {
 // TH 2: two waves share each block of 16 rows and take half of the chunk's tokens each (E in both): where the LDS allows one workgroup of narrow
 // heads on a CU, its D / 16 waves alone would leave the matrix units waiting.
 // Bound by the latency of a chunk's dependent stages, with the four tiles filling the LDS of a CU (one workgroup of 128-wide heads): 4 x 4096
-// tokens x 8 heads of 128, bf16, decays per token: 156 us, 285 MB of HBM traffic at 1.8 TB/s, 14 % of the MFMA and 35 % of the vector issue
-// slots; fp32 4 x 2048 x 4 heads of 128 96 us; 8 x 2048 x 8 heads of 64 bf16 66 us, fp32 131; 8 x 2048 x 4 heads of 96 bf16 69, 80 / 96 fp32 137.  64 rows of 16 tokens x 4 heads of 64, fp32: 14 us.
+// tokens x 8 heads of 128, bf16, decays per token: 159 us, 284 MB read and 103 written (2.4 TB/s), 20 % of the MFMA and 37 % of the vector issue
+// slots; fp32 4 x 2048 x 4 heads of 128 97 us; 8 x 2048 x 8 heads of 64 bf16 66 us, fp32 134; 8 x 2048 x 4 heads of 96 bf16 68, 80 / 96 fp32 136.  64 rows of 16 tokens x 4 heads of 64, fp32: 14 us.
 template <int DT, int D> constexpr int la_bwd_halves() { return D == 32 || (D == 64 && DT != 1) ? 2 : 1; }
 template <int DT, int D>
 __global__ __launch_bounds__((4 * D * la_bwd_halves<DT, D>())) void la_bwd_chunks(LaArgs a, LaBwd p) {
@@ -1381,7 +1381,8 @@ LaPlan la_plan(int T, int Dk, int Dv, int dtype, long wg, int room, int more) {
     return p;
 }
 // as many workgroups as fit the chip at once, by their LDS: two on a CU where they take 80 KB at most, else one.  More segments than that only
-// add states: 8 x 2048 tokens x 8 heads fp32 took 137 us with 256 workgroups, 144 with 512, 167 with 1024; 1 x 32768 x 8 bf16 182, 153, 180
+// add states: 8 x 2048 tokens x 8 heads 64 / 128 fp32 takes 119 us with 256 workgroups, 132 with 512, 158 with 1024; 1 x 32768 x 8 heads of 128 bf16
+// 181, 158, 193 (sums of the three kernels)
 LaPlan la_plan_fwd(int BH, int T, int Dk, int Dv, int dtype) {
     return la_plan(T, Dk, Dv, dtype, (long)BH * cdiv(Dv, la_dvt(Dk, Dv, dtype)), dtype == 1 || (Dk <= 64 && Dv <= 64) ? 512 : 256, 15);
 }

@@ -1639,7 +1639,10 @@ def linear_attention_fwd(q, k, v, log_decay, state=None, lens=None, scale=None, 
     up to 128); log_decay fp32 [H] (one decay per head) or [B,T,H] (one per token; -inf clears the state, e.g. where an episode begins).
     Hq, Hk and Hv divide H; head h reads shared head h // (H // Hx).  state: S before the first token (None: 0).  lens int32 [B]: row b has
     lens[b] tokens; what is behind them is not read, out is 0 there and the last state is the one after them.  scale: 1 / sqrt(Dk) by default.
-    Tokens are taken 64 at a time: a NaN or infinity in a row makes its outputs undefined from the beginning of that 64."""
+    Tokens are taken 64 at a time: a NaN or infinity in a row makes its outputs undefined from the beginning of that 64.  A decay of -inf is a
+    factor of 0: it clears any finite state, but neither NaN nor infinity.  B * H * (T // 64 + 1) stays below 2^23.
+    Like all of this module the call stands outside autograd: out does not require grad whatever the inputs do; the gradient is
+    linear_attention_bwd."""
     H, Hq, Hk, Hv, Dk, Dv, dt = _la_heads(q, k, v, log_decay, 2)
     _same_device(q, k, v, log_decay, state, lens)
     B, T = q.shape[:2]
@@ -1661,7 +1664,7 @@ def linear_attention_fwd(q, k, v, log_decay, state=None, lens=None, scale=None, 
 def linear_attention_bwd(q, k, v, log_decay, dout, state=None, lens=None, scale=None, dstate=None):
     """Gradient of linear_attention_fwd (same q .. scale): dout [B,T,H,Dv] in q's type, dstate = gradient of the last state (None: 0)
     -> (dq, dk, dv in q's type, d log_decay fp32 in log_decay's shape, gradient of `state` or None without one).  Nothing but the inputs is
-    kept from the forward.  Sums over shared heads and over broadcast decays have a fixed order."""
+    kept from the forward.  Sums over shared heads and over broadcast decays have a fixed order.  A decay whose exp is 0 gets the gradient 0."""
     H, Hq, Hk, Hv, Dk, Dv, dt = _la_heads(q, k, v, log_decay, 2)
     _same_device(q, k, v, log_decay, dout, state, lens, dstate)
     B, T = q.shape[:2]
@@ -1693,7 +1696,8 @@ def linear_attention_step(q, k, v, log_decay, state, slots=None, scale=None):
     """One token for each of B rows: S <- exp(log_decay) S + k v^T in place, -> out [B,H,Dv] = scale * S^T q (the recurrent form of
     linear_attention_fwd).  q [B,Hq,Dk], k [B,Hk,Dk], v [B,Hv,Dv], log_decay [H] or [B,H]; state fp32 [N,H,Dk,Dv], contiguous.
     slots int32 [B]: row b uses state[slots[b]] (None: state[b], N = B).  A slot outside [0, N) is an idle row: out 0, no state touched.
-    Rows that name the same slot are taken in row order, as successive tokens."""
+    Rows that name the same slot are taken in row order, as successive tokens.  A decay of -inf clears a slot's finite state; one that holds NaN or
+    infinity (memory never written) has to be zeroed.  B * H stays below 2^23.  Outside autograd, and without a gradient of its own."""
     H, Hq, Hk, Hv, Dk, Dv, dt = _la_heads(q, k, v, log_decay, 1)
     _same_device(q, k, v, log_decay, state, slots)
     B = q.shape[0]
@@ -1723,7 +1727,7 @@ def _ids(ids):
 def embed_fwd(ids, table, scale=1.0, pos=None):
     """out[..., t, :] = scale * table[ids[..., t]] + pos[t]  (fp32 arithmetic, rounded once to table's type).  ids int64 / int32 [..., T];
     table [V,D] fp32 / bf16 / fp16 (rows may be strided); pos [>= T, D] in table's type or None.  An id outside [0, V) is an empty place: a
-    zero row."""
+    zero row.  Outside autograd (a table that requires grad is read, nothing is recorded): the gradient is embed_bwd."""
     N, T, wide = _ids(ids)
     _same_device(ids, table, pos)
     dt = _SEQ_DT.get(table.dtype)
